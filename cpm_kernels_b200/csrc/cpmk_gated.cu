@@ -1,0 +1,328 @@
+// Gated feed-forward block: h = act(x Wg^T) * (x Wu^T), y = h Wd^T, and its backward pass, in fp16 and bf16 with fp32 sums.
+//
+//   backward   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
+#include "cpmk_common.cuh"
+#include "cpmk_types.cuh"
+
+namespace cpmk {
+namespace {
+
+// ------------------------------------------------------------------------------------------------
+// the activation
+// ------------------------------------------------------------------------------------------------
+// Both activations are v s(z(v)) with the logistic function s: z = v (silu), z = 2 c (v + 0.044715 v^3), c = sqrt(2 / pi) (gelu:
+// (1 + tanh t) / 2 = s(2 t)).  Derivative: s + v s (1 - s) z'(v).  Beyond |v| = 30 the logistic is 0 or 1 in fp32 (|z| > 1900), so z
+// and z' are taken of the clamped value: the cube cannot overflow and 0 * inf does not arise.
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float v) {
+    if (ACT == CPMK_ACT_SILU) return v * logistic(v);
+    const float c = fminf(fmaxf(v, -30.f), 30.f);
+    return v * logistic(1.5957691216057308f * fmaf(0.044715f * c * c, c, c));
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_value_slope(float v, float &value, float &slope) {
+    if (ACT == CPMK_ACT_SILU) {
+        const float s = logistic(v);
+        value = v * s;
+        slope = fmaf(value, 1.f - s, s);
+    } else {
+        const float c = fminf(fmaxf(v, -30.f), 30.f), c2 = c * c;
+        const float s = logistic(1.5957691216057308f * fmaf(0.044715f * c2, c, c));
+        value = v * s;
+        slope = fmaf(value * (1.f - s), 1.5957691216057308f * fmaf(3.f * 0.044715f, c2, 1.f), s);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Generic product: out[r, c] = sum_k P[r, k] Q[c, k] with any strides, 64 x 64 outputs per block of 256 threads, 4 x 4 per thread.
+// ------------------------------------------------------------------------------------------------
+enum { kEpiStore = 0, kEpiGated = 1, kEpiDact = 2 };
+
+struct SimtParams {
+    int32_t R, C, K;
+    int64_t tiles_c;
+    int64_t p_rs, p_ks, q_rs, q_ks;      // element strides of the rows and of k
+    const void *p[2], *q[2];             // kEpiStore: sum over both pairs when p[1] is given; kEpiGated: q[0] gate, q[1] up
+    void *out[3];                        // kEpiStore: out; kEpiGated: h, g, u (g, u may be null); kEpiDact: dg, du
+    const void *in[2];                   // kEpiDact: g, u
+};
+constexpr int kSimtTile = 64, kSimtK = 16;
+
+template <typename T, int EPI, int ACT>
+__global__ void __launch_bounds__(256) gated_simt_kernel(const SimtParams prm) {
+    __shared__ float sp[kSimtK][kSimtTile + 1], sq[EPI == kEpiGated ? 2 : 1][kSimtK][kSimtTile + 1];
+    const int r0 = (int)(blockIdx.x / prm.tiles_c) * kSimtTile, c0 = (int)(blockIdx.x % prm.tiles_c) * kSimtTile;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    float acc[4][4] = {}, acc2[4][4] = {};
+    const int pairs = EPI == kEpiStore && prm.p[1] ? 2 : 1;
+    for (int pair = 0; pair < pairs; ++pair) {
+        const T *P = static_cast<const T *>(prm.p[pair]), *Q = static_cast<const T *>(prm.q[pair]), *Q1 = static_cast<const T *>(prm.q[1]);
+        for (int k0 = 0; k0 < prm.K; k0 += kSimtK) {
+            for (int e = threadIdx.x; e < kSimtK * kSimtTile; e += 256) {
+                // the thread index runs along the contiguous axis
+                const int lp = prm.p_ks == 1 ? e % kSimtK : e / kSimtTile, i = prm.p_ks == 1 ? e / kSimtK : e % kSimtTile;
+                sp[lp][i] = k0 + lp < prm.K && r0 + i < prm.R ? to_f32(P[(r0 + i) * prm.p_rs + (k0 + lp) * prm.p_ks]) : 0.f;
+                const int lq = prm.q_ks == 1 ? e % kSimtK : e / kSimtTile, j = prm.q_ks == 1 ? e / kSimtK : e % kSimtTile;
+                const bool in = k0 + lq < prm.K && c0 + j < prm.C;
+                const int64_t at = (c0 + j) * prm.q_rs + (k0 + lq) * prm.q_ks;
+                sq[0][lq][j] = in ? to_f32(Q[at]) : 0.f;
+                if (EPI == kEpiGated) sq[EPI == kEpiGated ? 1 : 0][lq][j] = in ? to_f32(Q1[at]) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int l = 0; l < kSimtK; ++l) {
+                float pv[4], qv[4], qw[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    pv[i] = sp[l][ty + 16 * i];
+                    qv[i] = sq[0][l][tx + 16 * i];
+                    if (EPI == kEpiGated) qw[i] = sq[EPI == kEpiGated ? 1 : 0][l][tx + 16 * i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        acc[i][j] = fmaf(pv[i], qv[j], acc[i][j]);
+                        if (EPI == kEpiGated) acc2[i][j] = fmaf(pv[i], qw[j], acc2[i][j]);
+                    }
+            }
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = r0 + ty + 16 * i, c = c0 + tx + 16 * j;
+            if (r >= prm.R || c >= prm.C) continue;
+            const int64_t at = (int64_t)r * prm.C + c;
+            if (EPI == kEpiStore) {
+                static_cast<T *>(prm.out[0])[at] = from_f32<T>(acc[i][j]);
+            } else if (EPI == kEpiGated) {
+                static_cast<T *>(prm.out[0])[at] = from_f32<T>(act_value<ACT>(acc[i][j]) * acc2[i][j]);
+                if (prm.out[1]) {
+                    static_cast<T *>(prm.out[1])[at] = from_f32<T>(acc[i][j]);
+                    static_cast<T *>(prm.out[2])[at] = from_f32<T>(acc2[i][j]);
+                }
+            } else {
+                float value, slope;
+                act_value_slope<ACT>(to_f32(static_cast<const T *>(prm.in[0])[at]), value, slope);
+                static_cast<T *>(prm.out[0])[at] = from_f32<T>(acc[i][j] * to_f32(static_cast<const T *>(prm.in[1])[at]) * slope);
+                static_cast<T *>(prm.out[1])[at] = from_f32<T>(acc[i][j] * value);
+            }
+        }
+}
+
+// dg = dh u act'(g), du = dh act(g) for a dh that lies in memory (the backward pass of the gated linear on its own).
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) gated_dact_kernel(int64_t count, const T *__restrict__ dh, const T *__restrict__ g, const T *__restrict__ u,
+                                                         T *__restrict__ dg, T *__restrict__ du) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const float d = to_f32(dh[i]);
+        float value, slope;
+        act_value_slope<ACT>(to_f32(g[i]), value, slope);
+        dg[i] = from_f32<T>(d * to_f32(u[i]) * slope);
+        du[i] = from_f32<T>(d * value);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+struct Call {
+    DeviceInfo info;
+    int32_t dtype, act;
+    cudaStream_t stream;
+};
+
+template <int EPI>
+int32_t launch_simt(const Call &call, SimtParams prm) {
+    prm.tiles_c = ceil_div64(prm.C, kSimtTile);
+    const int64_t tiles = prm.tiles_c * ceil_div64(prm.R, kSimtTile);
+    CPMK_REQUIRE(tiles < (int64_t(1) << 31), "too many output tiles");
+    const dim3 grid((unsigned)tiles);
+    const bool silu = EPI != kEpiStore && call.act == CPMK_ACT_SILU;
+    if (call.dtype == CPMK_F16) {
+        if (silu) gated_simt_kernel<__half, EPI, CPMK_ACT_SILU><<<grid, 256, 0, call.stream>>>(prm);
+        else gated_simt_kernel<__half, EPI, CPMK_ACT_GELU><<<grid, 256, 0, call.stream>>>(prm);
+    } else {
+        if (silu) gated_simt_kernel<__nv_bfloat16, EPI, CPMK_ACT_SILU><<<grid, 256, 0, call.stream>>>(prm);
+        else gated_simt_kernel<__nv_bfloat16, EPI, CPMK_ACT_GELU><<<grid, 256, 0, call.stream>>>(prm);
+    }
+    CPMK_LAUNCH_CHECK();
+    return CPMK_OK;
+}
+
+// out (R, C) = P Q^T summed over one or two pairs of operands.  p_t / q_t: the operand is stored (K, rows) instead of (rows, K).
+int32_t product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1, const void *q1,
+                void *out) {
+    SimtParams prm = {};
+    prm.R = R; prm.C = C; prm.K = K;
+    prm.p_rs = p_t ? 1 : K; prm.p_ks = p_t ? R : 1;
+    prm.q_rs = q_t ? 1 : K; prm.q_ks = q_t ? C : 1;
+    prm.p[0] = p0; prm.p[1] = p1; prm.q[0] = q0; prm.q[1] = q1;
+    prm.out[0] = out;
+    return launch_simt<kEpiStore>(call, prm);
+}
+
+int32_t gated_product(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u) {
+    SimtParams prm = {};
+    prm.R = tokens; prm.C = n; prm.K = k;
+    prm.p_rs = k; prm.p_ks = 1; prm.q_rs = k; prm.q_ks = 1;
+    prm.p[0] = x; prm.q[0] = wg; prm.q[1] = wu;
+    prm.out[0] = h; prm.out[1] = g; prm.out[2] = u;
+    return launch_simt<kEpiGated>(call, prm);
+}
+
+// dg, du from dh = dy Wd, which is not stored; Wd is (m, n)
+int32_t dact_product(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg,
+                     void *du) {
+    SimtParams prm = {};
+    prm.R = tokens; prm.C = n; prm.K = m;
+    prm.p_rs = m; prm.p_ks = 1; prm.q_rs = 1; prm.q_ks = n;
+    prm.p[0] = dy; prm.q[0] = wd;
+    prm.in[0] = g; prm.in[1] = u;
+    prm.out[0] = dg; prm.out[1] = du;
+    return launch_simt<kEpiDact>(call, prm);
+}
+
+int32_t dact(const Call &call, int64_t count, const void *dh, const void *g, const void *u, void *dg, void *du) {
+    const int64_t blocks = ceil_div64(count, 256);
+    const dim3 grid((unsigned)(blocks < 8 * call.info.sm_count ? blocks : 8 * call.info.sm_count));
+#define CPMK_DACT(T, ACT) \
+    gated_dact_kernel<T, ACT><<<grid, 256, 0, call.stream>>>(count, static_cast<const T *>(dh), static_cast<const T *>(g), static_cast<const T *>(u), \
+                                                             static_cast<T *>(dg), static_cast<T *>(du))
+    if (call.dtype == CPMK_F16) {
+        if (call.act == CPMK_ACT_SILU) CPMK_DACT(__half, CPMK_ACT_SILU);
+        else CPMK_DACT(__half, CPMK_ACT_GELU);
+    } else {
+        if (call.act == CPMK_ACT_SILU) CPMK_DACT(__nv_bfloat16, CPMK_ACT_SILU);
+        else CPMK_DACT(__nv_bfloat16, CPMK_ACT_GELU);
+    }
+#undef CPMK_DACT
+    CPMK_LAUNCH_CHECK();
+    return CPMK_OK;
+}
+
+bool even_address(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+
+int32_t begin(Call *call, int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t act, cpmk_stream_t stream) {
+    const int32_t rc = current_device_info(&call->info);
+    if (rc) return rc;
+    CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 1, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
+    CPMK_REQUIRE(dtype == CPMK_F16 || dtype == CPMK_BF16, "the gated block takes fp16 and bf16 (dtype %d)", dtype);
+    CPMK_REQUIRE(act == CPMK_ACT_GELU || act == CPMK_ACT_SILU, "unknown activation %d", act);
+    call->dtype = dtype;
+    call->act = act;
+    call->stream = as_stream(stream);
+    return CPMK_OK;
+}
+
+// dx, dWg, dWu from dg, du
+int32_t projections_backward(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, const void *dg,
+                             const void *du, void *dx, void *dwg, void *dwu) {
+    int32_t rc = CPMK_OK;
+    if (dx) rc = product(call, tokens, k, n, false, true, dg, wg, du, wu, dx);
+    if (!rc && dwg) rc = product(call, n, k, tokens, true, true, dg, x, nullptr, nullptr, dwg);
+    if (!rc && dwu) rc = product(call, n, k, tokens, true, true, du, x, nullptr, nullptr, dwu);
+    return rc;
+}
+
+// without tokens the weights' gradients are zero
+int32_t clear_gradients(const Call &call, void *dwg, void *dwu, void *dwd, int64_t nk, int64_t mn) {
+    if (dwg) CPMK_CUDA_TRY(cudaMemsetAsync(dwg, 0, (size_t)nk * 2, call.stream));
+    if (dwu) CPMK_CUDA_TRY(cudaMemsetAsync(dwu, 0, (size_t)nk * 2, call.stream));
+    if (dwd) CPMK_CUDA_TRY(cudaMemsetAsync(dwd, 0, (size_t)mn * 2, call.stream));
+    return CPMK_OK;
+}
+
+}  // namespace
+}  // namespace cpmk
+
+using namespace cpmk;
+
+extern "C" {
+
+int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int64_t *bytes) {
+    DeviceInfo info;
+    const int32_t rc = current_device_info(&info);
+    if (rc) return rc;
+    CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 0 && bytes, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
+    *bytes = 0;
+    return CPMK_OK;
+}
+
+int32_t cpmk_gated_linear_forward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *x, const void *w_gate,
+                                  const void *w_up, void *h, void *g, void *u, void *scratch, cpmk_stream_t stream) {
+    Call call;
+    const int32_t rc = begin(&call, tokens, k, n, 1, dtype, activation, stream);
+    if (rc) return rc;
+    if (tokens == 0) return CPMK_OK;
+    CPMK_REQUIRE(x && w_gate && w_up && h, "null pointer");
+    CPMK_REQUIRE((g == nullptr) == (u == nullptr), "g and u are wanted together or not at all");
+    CPMK_REQUIRE(even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(h) && even_address(g) && even_address(u),
+                 "tensors must be 2-byte aligned");
+    CPMK_REQUIRE(aligned16(scratch), "scratch must be 16-byte aligned");
+    return gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u);
+}
+
+int32_t cpmk_gated_linear_backward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *dh, const void *x,
+                                   const void *w_gate, const void *w_up, const void *g, const void *u, void *dg, void *du, void *dx, void *dw_gate,
+                                   void *dw_up, cpmk_stream_t stream) {
+    Call call;
+    int32_t rc = begin(&call, tokens, k, n, 1, dtype, activation, stream);
+    if (rc) return rc;
+    if (tokens == 0) return clear_gradients(call, dw_gate, dw_up, nullptr, (int64_t)n * k, 0);
+    CPMK_REQUIRE(dh && x && w_gate && w_up && g && u && dg && du, "null pointer");
+    CPMK_REQUIRE(even_address(dh) && even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(g) && even_address(u) &&
+                     even_address(dg) && even_address(du) && even_address(dx) && even_address(dw_gate) && even_address(dw_up),
+                 "tensors must be 2-byte aligned");
+    rc = dact(call, (int64_t)tokens * n, dh, g, u, dg, du);
+    if (rc) return rc;
+    return projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up);
+}
+
+int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *x,
+                                        const void *w_gate, const void *w_up, const void *w_down, void *h, void *g, void *u, void *y, void *scratch,
+                                        cpmk_stream_t stream) {
+    Call call;
+    int32_t rc = begin(&call, tokens, k, n, m, dtype, activation, stream);
+    if (rc) return rc;
+    if (tokens == 0) return CPMK_OK;
+    CPMK_REQUIRE(x && w_gate && w_up && w_down && h && y, "null pointer");
+    CPMK_REQUIRE((g == nullptr) == (u == nullptr), "g and u are wanted together or not at all");
+    CPMK_REQUIRE(even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(w_down) && even_address(h) && even_address(g) &&
+                     even_address(u) && even_address(y),
+                 "tensors must be 2-byte aligned");
+    CPMK_REQUIRE(aligned16(scratch), "scratch must be 16-byte aligned");
+    rc = gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u);
+    if (rc) return rc;
+    return product(call, tokens, m, n, false, false, h, w_down, nullptr, nullptr, y);
+}
+
+int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *dy,
+                                         const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *g, const void *u,
+                                         const void *h, void *dg, void *du, void *dx, void *dw_gate, void *dw_up, void *dw_down, cpmk_stream_t stream) {
+    Call call;
+    int32_t rc = begin(&call, tokens, k, n, m, dtype, activation, stream);
+    if (rc) return rc;
+    if (tokens == 0) return clear_gradients(call, dw_gate, dw_up, dw_down, (int64_t)n * k, (int64_t)m * n);
+    CPMK_REQUIRE(dy && x && w_gate && w_up && w_down && g && u && dg && du && (h || !dw_down), "null pointer");
+    CPMK_REQUIRE(even_address(dy) && even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(w_down) && even_address(g) &&
+                     even_address(u) && even_address(h) && even_address(dg) && even_address(du) && even_address(dx) && even_address(dw_gate) &&
+                     even_address(dw_up) && even_address(dw_down),
+                 "tensors must be 2-byte aligned");
+    if (dx || dw_gate || dw_up) {
+        rc = dact_product(call, tokens, n, m, dy, w_down, g, u, dg, du);
+        if (rc) return rc;
+        rc = projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up);
+        if (rc) return rc;
+    }
+    if (dw_down) return product(call, m, n, tokens, true, true, dy, h, nullptr, nullptr, dw_down);
+    return CPMK_OK;
+}
+
+}  // extern "C"

@@ -63,7 +63,19 @@ SIGNATURES = {
     "cpmk_gemv_calc_scale": [_i, _i, _p, _p, _p],
     "cpmk_gemv_round": [_i, _i, _p, _p, _p, _p],
     "cpmk_gemv_broadcast_mat_int8": [_i, _i, _i, _p, _p, _p, _p, _p, _p],
+    "cpmk_layernorm_rows_forward": [_i, _i, _i, _p, ctypes.c_float, _i, _p, _p, _p, _p, _p, _p],
+    "cpmk_layernorm_rows_backward_scratch": [_i, _i, POINTER(ctypes.c_int64)],
+    "cpmk_layernorm_rows_backward": [_i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p],
+    "cpmk_gated_scratch": [_i, _i, _i, _i, POINTER(ctypes.c_int64)],
+    "cpmk_gated_linear_forward": [_i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p],
+    "cpmk_gated_linear_backward": [_i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+    "cpmk_gated_feed_forward_forward": [_i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+    "cpmk_gated_feed_forward_backward": [_i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
 }
+
+# codes of the `dtype` and `activation` arguments
+F16, BF16, F32 = 0, 1, 2
+ACTIVATIONS = {"gelu": 0, "silu": 1}
 
 for _name, _args in SIGNATURES.items():
     lib.bind(_name, _args, c_int32)

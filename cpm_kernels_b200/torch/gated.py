@@ -1,0 +1,130 @@
+"""``gated_linear`` and ``gated_feed_forward``: the gated feed-forward block act(x Wg^T) * (x Wu^T), times Wd^T, with autograd.
+
+What a caller of cpm_kernels composes from ``bmm`` (torch/gemm.py:233-239), ``gelu`` (torch/gelu.py:46-47) and a product of tensors,
+with both projections, the activation and the product in one pass, and the activation's derivative in the epilogue of the product
+before it on the way back.  fp16 and bf16, fp32 sums."""
+import torch
+
+from ..kernels import gated_linear_forward, gated_linear_backward, gated_feed_forward_forward, gated_feed_forward_backward, gated_scratch
+from ..library import cpmk
+
+_DTYPES = {torch.float16: cpmk.F16, torch.bfloat16: cpmk.BF16}
+
+
+def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str) -> None:
+    assert x.is_cuda and x.is_contiguous() and x.ndim >= 1 and x.dtype in _DTYPES
+    assert x.size(-1) >= 1 and x.numel() // x.size(-1) < 2 ** 31
+    for w in (w_gate, w_up):
+        assert w.is_cuda and w.device == x.device and w.is_contiguous() and w.ndim == 2 and w.dtype == x.dtype
+        assert w.size(0) >= 1 and w.size(1) == x.size(-1)
+    assert w_gate.size(0) == w_up.size(0)
+    assert activation in cpmk.ACTIVATIONS
+
+
+def _scratch(tokens: int, k: int, n: int, m: int, device) -> torch.Tensor:
+    return torch.empty((gated_scratch(tokens, k, n, m),), dtype=torch.uint8, device=device)
+
+
+def _ptr(t) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
+def _linear_forward(x, w_gate, w_up, activation: str, save: bool):
+    n, k = w_gate.shape
+    tokens = x.numel() // k
+    h = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    gu = torch.empty((2, tokens, n), dtype=x.dtype, device=x.device) if save else None
+    with torch.cuda.device(x.device):
+        scratch = _scratch(tokens, k, n, 0, x.device)
+        gated_linear_forward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                             h.data_ptr(), _ptr(gu[0]) if save else 0, _ptr(gu[1]) if save else 0, scratch.data_ptr(),
+                             torch.cuda.current_stream().cuda_stream)
+    return h, gu
+
+
+class OpGatedLinear(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str):
+        h, gu = _linear_forward(x, w_gate, w_up, activation, True)
+        ctx.save_for_backward(x, w_gate, w_up, gu)
+        ctx.activation = activation
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output: torch.Tensor):
+        x, w_gate, w_up, gu = ctx.saved_tensors
+        dh = grad_output.contiguous()
+        n, k = w_gate.shape
+        tokens = x.numel() // k
+        dgu = torch.empty_like(gu)
+        dx, dw_gate, dw_up = (torch.empty_like(t) if need else None for t, need in zip((x, w_gate, w_up), ctx.needs_input_grad))
+        with torch.cuda.device(x.device):
+            gated_linear_backward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation], dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+                                  w_up.data_ptr(), gu[0].data_ptr(), gu[1].data_ptr(), dgu[0].data_ptr(), dgu[1].data_ptr(), _ptr(dx), _ptr(dw_gate),
+                                  _ptr(dw_up), torch.cuda.current_stream().cuda_stream)
+        return dx, dw_gate, dw_up, None
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "gelu") -> torch.Tensor:
+    """``act(x w_gate^T) * (x w_up^T)`` for x (..., K) and weights (N, K): (..., N).  ``activation``: "gelu" (the tanh form of ``gelu``)
+    or "silu", applied to the fp32 sums.  fp16 or bf16.  Differentiable (once) in x and both weights; a call that is differentiated
+    keeps the two projections, in the tensors' type."""
+    _check(x, w_gate, w_up, activation)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+        return OpGatedLinear.apply(x, w_gate, w_up, activation)
+    return _linear_forward(x, w_gate, w_up, activation, False)[0]
+
+
+def _block_forward(x, w_gate, w_up, w_down, activation: str, save: bool):
+    n, k = w_gate.shape
+    m = w_down.size(0)
+    tokens = x.numel() // k
+    y = torch.empty((*x.shape[:-1], m), dtype=x.dtype, device=x.device)
+    hgu = torch.empty((3 if save else 1, tokens, n), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        scratch = _scratch(tokens, k, n, m, x.device)
+        gated_feed_forward_forward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                                   w_down.data_ptr(), hgu[0].data_ptr(), hgu[1].data_ptr() if save else 0, hgu[2].data_ptr() if save else 0,
+                                   y.data_ptr(), scratch.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    return y, hgu
+
+
+class OpGatedFeedForward(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str):
+        y, hgu = _block_forward(x, w_gate, w_up, w_down, activation, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, hgu)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output: torch.Tensor):
+        x, w_gate, w_up, w_down, hgu = ctx.saved_tensors
+        dy = grad_output.contiguous()
+        n, k = w_gate.shape
+        m = w_down.size(0)
+        tokens = x.numel() // k
+        dgu = torch.empty((2, tokens, n), dtype=x.dtype, device=x.device)
+        dx, dw_gate, dw_up, dw_down = (torch.empty_like(t) if need else None for t, need in zip((x, w_gate, w_up, w_down), ctx.needs_input_grad))
+        with torch.cuda.device(x.device):
+            gated_feed_forward_backward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation], dy.data_ptr(), x.data_ptr(),
+                                        w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), hgu[1].data_ptr(), hgu[2].data_ptr(),
+                                        hgu[0].data_ptr(), dgu[0].data_ptr(), dgu[1].data_ptr(), _ptr(dx), _ptr(dw_gate), _ptr(dw_up),
+                                        _ptr(dw_down), torch.cuda.current_stream().cuda_stream)
+        return dx, dw_gate, dw_up, dw_down, None
+
+
+def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "gelu") -> torch.Tensor:
+    """``gated_linear(x, w_gate, w_up, activation)`` times ``w_down^T``: x (..., K), w_gate and w_up (N, K), w_down (M, N) -> (..., M).
+    The hidden activations between the two are rounded to the tensors' type.  Differentiable (once) in x and the three weights; a call
+    that is differentiated keeps the two projections and the hidden activations."""
+    _check(x, w_gate, w_up, activation)
+    assert w_down.is_cuda and w_down.device == x.device and w_down.is_contiguous() and w_down.ndim == 2 and w_down.dtype == x.dtype
+    assert w_down.size(0) >= 1 and w_down.size(1) == w_gate.size(0)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+        return OpGatedFeedForward.apply(x, w_gate, w_up, w_down, activation)
+    return _block_forward(x, w_gate, w_up, w_down, activation, False)[0]

@@ -35,6 +35,19 @@ enum {
 
 typedef void *cpmk_stream_t;
 
+/* Element types of the entry points that take more than fp16 (their `dtype` argument). */
+enum {
+    CPMK_F16 = 0,          /* IEEE binary16 */
+    CPMK_BF16 = 1,         /* bfloat16      */
+    CPMK_F32 = 2           /* IEEE binary32 */
+};
+
+/* Activations of the gated linear (its `activation` argument). */
+enum {
+    CPMK_ACT_GELU = 0,     /* v / 2 (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))): the form of cpmk_gelu_forward */
+    CPMK_ACT_SILU = 1      /* v / (1 + exp(-v)) */
+};
+
 int32_t cpmk_abi_version(void);
 const char *cpmk_last_error(void);
 
@@ -297,6 +310,66 @@ int32_t cpmk_gemv_round(int32_t batch, int32_t n, const void *vec, const void *s
 /* kernels/gemv.py:56-79 gemv_broadcast_mat_int8 -> cuda/gemv.cu:57-76.  dim_in multiple of 4. */
 int32_t cpmk_gemv_broadcast_mat_int8(int32_t batch, int32_t dim_out, int32_t dim_in, const void *scale_mat, const void *mat,
                                      const void *scale_vec, const void *vec, void *out, cpmk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Layer norm over rows
+ * ------------------------------------------------------------------------------------------ */
+
+/* Layer norm of every row of x (rows, n), element type `dtype` for x, weight, bias and y:
+ *   m = mean of the row (0 when rd_mean = 0: the RMS form), r = 1 / sqrt(mean of (x - m)^2 + eps), y = (x - m) r weight + bias.
+ * weight (n), bias (n) or NULL.  mean, rstd: (rows) fp32, written for the backward pass, or both NULL.  Statistics in fp32, one
+ * rounding of y.  The token-major counterpart of the layer norm inside cpmk_layernorm_quantize_cols (kernels/layernorm.py:18-38
+ * normalises the middle axis of (batch, n, m)).   y must not overlap x. */
+int32_t cpmk_layernorm_rows_forward(int32_t rows, int32_t n, int32_t dtype, const void *x, float eps, int32_t rd_mean, const void *weight,
+                                    const void *bias, void *y, void *mean, void *rstd, cpmk_stream_t stream);
+
+/* Bytes of device scratch that cpmk_layernorm_rows_backward wants for these sizes on the current device. */
+int32_t cpmk_layernorm_rows_backward_scratch(int32_t rows, int32_t n, int64_t *bytes);
+
+/* Gradients of cpmk_layernorm_rows_forward for the output gradient dy (rows, n), from x and the statistics that the forward call
+ * wrote: with xh = (x - m) r and g = dy weight,
+ *   dx = r (g - mean(g) [only when rd_mean] - xh mean(g xh)),   dweight = sum over rows of dy xh,   dbias = sum over rows of dy.
+ * Each of dx, dweight, dbias may be NULL; outputs must not overlap inputs.  Sums in fp32 in an order that depends on the sizes and the device
+ * only.  `scratch` (16-byte aligned) is the caller's and not kept; calls that overlap need scratch of their own. */
+int32_t cpmk_layernorm_rows_backward(int32_t rows, int32_t n, int32_t dtype, const void *dy, const void *x, int32_t rd_mean, const void *weight,
+                                     const void *mean, const void *rstd, void *dx, void *dweight, void *dbias, void *scratch, cpmk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Gated feed-forward block
+ * ------------------------------------------------------------------------------------------
+ * dtype is CPMK_F16 or CPMK_BF16 for every tensor of a call; products are accumulated in fp32.  Any sizes: extents k, n, m that are
+ * multiples of 8 with 16-byte aligned pointers run on the tensor cores, others on a generic kernel.  Outputs must not overlap inputs. */
+
+/* Bytes of device scratch that cpmk_gated_linear_forward (m = 0) and cpmk_gated_feed_forward_forward want for these sizes on the
+ * current device (0: none).  `scratch` (16-byte aligned) is the caller's and not kept; calls that overlap need scratch of their own. */
+int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int64_t *bytes);
+
+/* h = act(x w_gate^T) * (x w_up^T): both projections, the activation and the product in one pass; the activation is applied to the
+ * fp32 sums.  x (tokens, k); w_gate, w_up (n, k); h (tokens, n).  g, u: (tokens, n), the two projections rounded to `dtype`, written
+ * for the backward pass, or both NULL.  The two linears, the gelu and the elementwise product of a gated block, which the reference's
+ * callers run as bmm, bmm, gelu (torch/gemm.py:233-239, torch/gelu.py:46-47) and a multiplication. */
+int32_t cpmk_gated_linear_forward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *x, const void *w_gate,
+                                  const void *w_up, void *h, void *g, void *u, void *scratch, cpmk_stream_t stream);
+
+/* Gradients of cpmk_gated_linear_forward for the output gradient dh (tokens, n), from x, the weights and the g, u that it wrote:
+ *   dg = dh u act'(g), du = dh act(g)  (tokens, n), always written;  dx = dg w_gate + du w_up;  dw_gate = dg^T x;  dw_up = du^T x.
+ * dx, dw_gate, dw_up may be NULL. */
+int32_t cpmk_gated_linear_backward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *dh, const void *x,
+                                   const void *w_gate, const void *w_up, const void *g, const void *u, void *dg, void *du, void *dx, void *dw_gate,
+                                   void *dw_up, cpmk_stream_t stream);
+
+/* y = h w_down^T after cpmk_gated_linear_forward: x (tokens, k), w_gate and w_up (n, k), w_down (m, n), y (tokens, m).  h (tokens, n)
+ * is written as well (the backward pass reads it). */
+int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *x,
+                                        const void *w_gate, const void *w_up, const void *w_down, void *h, void *g, void *u, void *y, void *scratch,
+                                        cpmk_stream_t stream);
+
+/* Gradients of cpmk_gated_feed_forward_forward for dy (tokens, m): dh = dy w_down stays on chip, dg and du (tokens, n) come out of that
+ * product's epilogue (they are written when dx, dw_gate or dw_up is wanted); dw_down = dy^T h (h may be NULL when dw_down is); the rest
+ * as cpmk_gated_linear_backward. */
+int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *dy,
+                                         const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *g, const void *u,
+                                         const void *h, void *dg, void *du, void *dx, void *dw_gate, void *dw_up, void *dw_down, cpmk_stream_t stream);
 
 #ifdef __cplusplus
 }
