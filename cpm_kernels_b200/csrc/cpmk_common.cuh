@@ -80,6 +80,24 @@ int32_t launch_gelu(int64_t count, const void *in, void *out, cudaStream_t strea
 // fp16 (esz 2) / 8-bit (esz 1) / int32 (esz 4), 128-byte swizzle or none.  Returns false when the driver refuses.
 bool encode_tiled_3d(void *map_out, int esz, const void *ptr, const uint64_t dims[3], const uint64_t strides[2], const uint32_t box[3], bool swizzle128);
 
+// Launches `kernel` so that its blocks may start before the kernel in front of it on the stream has finished, when that one lets them
+// (launch_dependents).  The kernel must call wait_for_prior_grid before it touches anything that work in front of it writes or
+// reads.  Only for a kernel that follows another of the same call: what precedes the call has then finished.
+template <typename... Params, typename... Args>
+cudaError_t launch_after_prior(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 inline cudaStream_t as_stream(cpmk_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -6,16 +6,18 @@
 // All sums and statistics are fp32; the deviations are taken from the mean before they are squared (no cancellation between
 // sum x^2 and n m^2), and every output is rounded once.
 #include "cpmk_common.cuh"
+#include "cpmk_ptx.cuh"
 #include "cpmk_types.cuh"
 
 namespace cpmk {
 namespace {
 
-// Three forms of each pass, chosen by the row's length and alignment (layout_of):
-//   * 16-byte vectors, the row in registers: G threads share a row, NV vectors each.  Rows of up to 1024 16-bit elements take one
-//     warp (no block-wide step), longer ones a block.
+// Bound by memory: forward 2, backward 3 tensors of traffic.  A fixed number of blocks walks the rows, the row held in registers, the
+// next row requested before the current one's sums are known.  Forms of each pass, chosen by the row's length and alignment (layout_of):
+//   * G threads share a row, NV 16-byte vectors each (VEC = 16 / element size).  Short rows take one warp (no block-wide step), longer
+//     ones a block.
 //   * the same with single elements (VEC = 1), for rows whose length or address is no multiple of 16 bytes.
-//   * rows too long for that: a block walks the row several times (they are in L1 and L2 after the first).
+//   * rows too long for that: a block walks the row several times (it is in L1 and L2 after the first).
 template <typename T, int VEC> struct Pack;
 template <typename T> struct Pack<T, 1> {
     T v[1];
@@ -29,6 +31,22 @@ template <typename T, int VEC> struct alignas(16) Pack {
     __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(v); }
     __device__ __forceinline__ void clear() { *reinterpret_cast<uint4 *>(v) = make_uint4(0u, 0u, 0u, 0u); }
 };
+
+// VEC floats between registers and shared memory (16-byte aligned when VEC > 1)
+template <int VEC>
+__device__ __forceinline__ void load_floats(float (&v)[VEC], const float *p) {
+    if constexpr (VEC == 1) v[0] = *p;
+    else
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4 *>(v + e) = *reinterpret_cast<const float4 *>(p + e);
+}
+template <int VEC>
+__device__ __forceinline__ void store_floats(float *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) *p = v[0];
+    else
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4 *>(p + e) = *reinterpret_cast<const float4 *>(v + e);
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -48,59 +66,83 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
     return warp_sum(lane < warps ? red[lane] : 0.f);
 }
 
+// Asks L2 for a row that the block reads next: one request per 128-byte line, no registers.
+template <typename T>
+__device__ __forceinline__ void prefetch_row(const T *row, int32_t n) {
+    const int64_t bytes = (int64_t)n * (int64_t)sizeof(T);
+    for (int64_t at = (int64_t)threadIdx.x * 128; at < bytes; at += (int64_t)blockDim.x * 128)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char *>(row) + at));
+}
+
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-// BLOCK: the whole block shares one row; otherwise each warp has its own.
-template <typename T, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 128) ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_mean,
-                                                                            const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ b,
-                                                                            T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-    __shared__ float red[2][32];
-    const int64_t row = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;                            // whole warps only
+// BLOCK: the whole block shares one row; otherwise each warp has its own.  MANY: more than 512 threads share it; with 64 registers a
+// thread the next row is asked for in L2 instead of in registers.
+template <typename T, int VEC, int NV, bool BLOCK, bool MANY>
+__global__ void __launch_bounds__(MANY ? 1024 : BLOCK ? 512 : 128, MANY ? 1 : VEC * NV > 16 ? 1 : BLOCK ? 2 : 8)
+ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_mean, const T *__restrict__ x, const T *__restrict__ w,
+                       const T *__restrict__ b, T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
+    __shared__ float red[2][2][32];
     const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, stride = (BLOCK ? blockDim.x : 32) * VEC;
-    const T *xr = x + row * n;
+    const int64_t first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int64_t step = BLOCK ? gridDim.x : (int64_t)gridDim.x * 4;
     Pack<T, VEC> in[NV];
+    auto request = [&](int64_t row) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int i = t * VEC + j * stride;
-        if (i < n) in[j].load(xr + i);
-        else in[j].clear();
-    }
-    float v[NV][VEC], mean = 0.f;
-    if (rd_mean) {
-        float s = 0.f;
+        for (int j = 0; j < NV; ++j) {
+            const int i = t * VEC + j * stride;
+            if (i < n) in[j].load(x + row * n + i);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < NV; ++j) in[j].clear();
+    if (first < rows) request(first);
+    int parity = 0;
+    for (int64_t row = first; row < rows; row += step, parity ^= 1) {
+        float v[NV][VEC], mean = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s += to_f32(in[j].v[e]);
-        mean = row_sum<BLOCK>(s, red[0]) * inv_n;
-    }
-    float q = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            v[j][e] = to_f32(in[j].v[e]) - mean;
-            if (t * VEC + j * stride < n) q = fmaf(v[j][e], v[j][e], q);
+            for (int e = 0; e < VEC; ++e) v[j][e] = to_f32(in[j].v[e]);
+        if (row + step < rows) {
+            if (MANY) prefetch_row(x + (row + step) * n, n);
+            else request(row + step);
         }
-    const float rstd = 1.f / sqrtf(row_sum<BLOCK>(q, red[1]) * inv_n + eps);
-    if (t == 0 && rstd_out) {
-        mean_out[row] = mean;
-        rstd_out[row] = rstd;
-    }
+        if (rd_mean) {
+            float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int i = t * VEC + j * stride;
-        if (i >= n) break;
-        Pack<T, VEC> pw, pb, out;
-        pw.load(w + i);
-        if (b) pb.load(b + i);
-        else pb.clear();
+            for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf(v[j][e] * rstd, to_f32(pw.v[e]), to_f32(pb.v[e])));
-        out.store(y + row * n + i);
+                for (int e = 0; e < VEC; ++e) s += v[j][e];
+            mean = row_sum<BLOCK>(s, red[parity][0]) * inv_n;
+        }
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                v[j][e] -= mean;
+                if (t * VEC + j * stride < n) q = fmaf(v[j][e], v[j][e], q);
+            }
+        const float rstd = 1.f / sqrtf(row_sum<BLOCK>(q, red[parity][1]) * inv_n + eps);
+        if (t == 0 && rstd_out) {
+            mean_out[row] = mean;
+            rstd_out[row] = rstd;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = t * VEC + j * stride;
+            if (i >= n) break;
+            Pack<T, VEC> pw, pb, out;
+            pw.load(w + i);                              // out of L1 after the first row
+            if (b) pb.load(b + i);
+            else pb.clear();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf(v[j][e] * rstd, to_f32(pw.v[e]), to_f32(pb.v[e])));
+            out.store(y + row * n + i);
+        }
+        if (MANY && row + step < rows) request(row + step);
     }
 }
 
@@ -138,28 +180,25 @@ __global__ void __launch_bounds__(kWideThreads) ln_rows_forward_wide_kernel(int3
 // ------------------------------------------------------------------------------------------------
 // A fixed number of blocks walks the rows (block p takes rows p, p + blocks, ...); each thread keeps the sums dy xh and dy of its
 // columns in registers, and the block leaves one fp32 row of partial sums for dw and one for db: x and dy are read once.
-// ln_rows_columns_kernel adds the blocks' rows.  Up to two vectors per thread the next row's x and dy are requested before the current
-// row's sums are known; with four, those registers (and the weight's) are not there, and the block's other half hides the latency.
+// ln_rows_columns_kernel adds the blocks' rows.
 template <typename T, int VEC, int NV, bool BLOCK, bool COLUMNS>
 __global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 1 : 2)
 ln_rows_backward_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const T *__restrict__ dy, const T *__restrict__ x,
                         const float *__restrict__ mean_in, const float *__restrict__ rstd_in, const T *__restrict__ w, T *__restrict__ dx,
-                        float *__restrict__ partial) {
+                        float *__restrict__ partial, int32_t pitch) {
     __shared__ float red[2][2][32];
-    extern __shared__ float columns[];                   // warps with rows of their own: the block's sums, 2 n
-    constexpr bool kAhead = VEC * NV <= 16;
+    extern __shared__ float columns[];                   // warps with rows of their own: their sums, 2 n each
+    if (COLUMNS) launch_dependents();
     const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, stride = (BLOCK ? blockDim.x : 32) * VEC;
     const int64_t first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     const int64_t step = BLOCK ? gridDim.x : (int64_t)gridDim.x * (blockDim.x >> 5);
-    Pack<T, VEC> kept[kAhead ? NV : 1], px[NV], pd[NV];
+    Pack<T, VEC> pw[NV], px[NV], pd[NV];
     float sw[NV][VEC], sb[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int i = t * VEC + j * stride;
-        if (kAhead) {
-            if (i < n) kept[kAhead ? j : 0].load(w + i);
-            else kept[kAhead ? j : 0].clear();
-        }
+        if (i < n) pw[j].load(w + i);
+        else pw[j].clear();
         px[j].clear();
         pd[j].clear();
 #pragma unroll
@@ -178,10 +217,9 @@ ln_rows_backward_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const
             }
         }
     };
-    if (kAhead && first < rows) request(first);
+    if (first < rows) request(first);
     int parity = 0;
     for (int64_t row = first; row < rows; row += step, parity ^= 1) {
-        if (!kAhead) request(row);
         Pack<T, VEC> cx[NV], cd[NV];
         const float r = rstd, m = mean;
         float s1 = 0.f, s2 = 0.f;
@@ -190,18 +228,13 @@ ln_rows_backward_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const
             cx[j] = px[j];
             cd[j] = pd[j];
         }
-        if (kAhead && row + step < rows) request(row + step);
+        if (row + step < rows) request(row + step);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            Pack<T, VEC> pw;
-            const int i = t * VEC + j * stride;
-            if (kAhead) pw = kept[kAhead ? j : 0];
-            else if (i < n) pw.load(w + i);
-            else pw.clear();
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float d = to_f32(cd[j].v[e]);      // zero beyond the row's end
-                const float xh = (to_f32(cx[j].v[e]) - m) * r, g = d * to_f32(pw.v[e]);
+                const float xh = (to_f32(cx[j].v[e]) - m) * r, g = d * to_f32(pw[j].v[e]);
                 s1 += g;
                 s2 = fmaf(g, xh, s2);
                 if (COLUMNS) {
@@ -228,49 +261,125 @@ ln_rows_backward_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const
         for (int j = 0; j < NV; ++j) {
             const int i = t * VEC + j * stride;
             if (i >= n) break;
-            Pack<T, VEC> pw, out;
-            if (kAhead) pw = kept[kAhead ? j : 0];
-            else pw.load(w + i);
+            Pack<T, VEC> out;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float xh = (to_f32(cx[j].v[e]) - m) * r, g = to_f32(cd[j].v[e]) * to_f32(pw.v[e]);
+                const float xh = (to_f32(cx[j].v[e]) - m) * r, g = to_f32(cd[j].v[e]) * to_f32(pw[j].v[e]);
                 out.v[e] = from_f32<T>(r * (g - c1 - xh * c2));
             }
             out.store(dx + row * n + i);
         }
     }
     if (!COLUMNS) return;
-    float *mine = partial + (int64_t)blockIdx.x * 2 * n;
-    if (BLOCK) {
+    float *mine = partial + (int64_t)blockIdx.x * 2 * pitch;
+    const int warps = blockDim.x >> 5;
+    float *to = BLOCK ? mine : columns + (threadIdx.x >> 5) * 2 * n;
+    const int second = BLOCK ? pitch : n;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+        const int i = t * VEC + j * stride;
+        if (i < n) {                                     // 16 bytes at a time: single floats, 32 bytes apart across a warp, took 5 us
+            store_floats<VEC>(to + i, sw[j]);
+            store_floats<VEC>(to + second + i, sb[j]);
+        }
+    }
+    if (BLOCK) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
+        float s = 0.f;
+        for (int v = 0; v < warps; ++v) s += columns[v * 2 * n + i];
+        mine[i < n ? i : pitch + i - n] = s;
+    }
+}
+
+// The same for rows of up to 16384 elements or 4096 vectors whose column sums do not fit the registers: 1024 threads, the block's sums
+// in shared memory (each thread adds to its own columns), the next row asked for in L2.  Per row 16 bytes of shared-memory traffic a
+// column, half of what the SM moves while the row's 6 (16-bit) to 12 (fp32) bytes a column arrive.
+template <typename T, int VEC, int NV, bool COLUMNS>
+__global__ void __launch_bounds__(1024, 1) ln_rows_backward_long_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const T *__restrict__ dy,
+                                                                        const T *__restrict__ x, const float *__restrict__ mean_in,
+                                                                        const float *__restrict__ rstd_in, const T *__restrict__ w, T *__restrict__ dx,
+                                                                        float *__restrict__ partial, int32_t pitch) {
+    __shared__ float red[2][2][32];
+    extern __shared__ float columns[];                   // 2 n
+    if (COLUMNS) launch_dependents();
+    const int t = threadIdx.x, stride = 1024 * VEC, lane = t & 31;
+    if (COLUMNS)
+        for (int i = t; i < 2 * n; i += 1024) columns[i] = 0.f;
+    __syncthreads();
+    int parity = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, parity ^= 1) {
+        const float m = mean_in[row], r = rstd_in[row];
+        Pack<T, VEC> px[NV], pd[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = t * VEC + j * stride;
+            if (i < n) {
+                px[j].load(x + row * n + i);
+                pd[j].load(dy + row * n + i);
+            }
+        }
+        if (row + gridDim.x < rows) {
+            prefetch_row(x + (row + gridDim.x) * n, n);
+            prefetch_row(dy + (row + gridDim.x) * n, n);
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = t * VEC + j * stride;
+            if (i >= n) break;
+            Pack<T, VEC> pw;
+            pw.load(w + i);
+            float aw[VEC], ab[VEC];
+            if (COLUMNS) {
+                load_floats<VEC>(aw, columns + i);
+                load_floats<VEC>(ab, columns + n + i);
+            }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int i = t * VEC + j * stride + e;
-                if (i < n) {
-                    mine[i] = sw[j][e];
-                    mine[n + i] = sb[j][e];
+                const float d = to_f32(pd[j].v[e]), xh = (to_f32(px[j].v[e]) - m) * r, g = d * to_f32(pw.v[e]);
+                s1 += g;
+                s2 = fmaf(g, xh, s2);
+                if (COLUMNS) {
+                    aw[e] = fmaf(d, xh, aw[e]);
+                    ab[e] += d;
                 }
             }
-        return;
-    }
-    // one warp after the other adds its sums: the order does not depend on timing
-    for (int turn = 0; turn < (int)(blockDim.x >> 5); ++turn) {
-        if ((int)(threadIdx.x >> 5) == turn) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int i = t * VEC + j * stride + e;
-                    if (i < n) {
-                        columns[i] = turn ? columns[i] + sw[j][e] : sw[j][e];
-                        columns[n + i] = turn ? columns[n + i] + sb[j][e] : sb[j][e];
-                    }
-                }
+            if (COLUMNS) {
+                store_floats<VEC>(columns + i, aw);
+                store_floats<VEC>(columns + n + i, ab);
+            }
+        }
+        if (!dx) continue;
+        float c1 = warp_sum(s1), c2 = warp_sum(s2);
+        if (lane == 0) {
+            red[parity][0][t >> 5] = c1;
+            red[parity][1][t >> 5] = c2;
         }
         __syncthreads();
+        c1 = rd_mean ? warp_sum(red[parity][0][lane]) * inv_n : 0.f;
+        c2 = warp_sum(red[parity][1][lane]) * inv_n;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = t * VEC + j * stride;
+            if (i >= n) break;
+            Pack<T, VEC> pw, out;
+            pw.load(w + i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float xh = (to_f32(px[j].v[e]) - m) * r, g = to_f32(pd[j].v[e]) * to_f32(pw.v[e]);
+                out.v[e] = from_f32<T>(r * (g - c1 - xh * c2));
+            }
+            out.store(dx + row * n + i);
+        }
     }
-    for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) mine[i] = columns[i];
+    if (!COLUMNS) return;
+    __syncthreads();
+    float *mine = partial + (int64_t)blockIdx.x * 2 * pitch;
+    for (int i = t; i < n; i += 1024) {
+        mine[i] = columns[i];
+        mine[pitch + i] = columns[n + i];
+    }
 }
 
 // Long rows: the block's partial sums lie in its own rows of `partial`, where each thread adds to the columns it owns.
@@ -278,9 +387,10 @@ template <typename T, bool COLUMNS>
 __global__ void __launch_bounds__(kWideThreads) ln_rows_backward_wide_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const T *__restrict__ dy,
                                                                              const T *__restrict__ x, const float *__restrict__ mean_in,
                                                                              const float *__restrict__ rstd_in, const T *__restrict__ w,
-                                                                             T *__restrict__ dx, float *__restrict__ partial) {
+                                                                             T *__restrict__ dx, float *__restrict__ partial, int32_t pitch) {
     __shared__ float red[2][32];
-    float *mine = COLUMNS ? partial + (int64_t)blockIdx.x * 2 * n : nullptr;
+    if (COLUMNS) launch_dependents();
+    float *mine = COLUMNS ? partial + (int64_t)blockIdx.x * 2 * pitch : nullptr;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * n, *dyr = dy + row * n;
         const float mean = mean_in[row], rstd = rstd_in[row];
@@ -291,7 +401,7 @@ __global__ void __launch_bounds__(kWideThreads) ln_rows_backward_wide_kernel(int
             s2 = fmaf(g, xh, s2);
             if (COLUMNS) {
                 mine[i] = row == blockIdx.x ? d * xh : fmaf(d, xh, mine[i]);
-                mine[n + i] = row == blockIdx.x ? d : mine[n + i] + d;
+                mine[pitch + i] = row == blockIdx.x ? d : mine[pitch + i] + d;
             }
         }
         if (!dx) continue;
@@ -304,22 +414,39 @@ __global__ void __launch_bounds__(kWideThreads) ln_rows_backward_wide_kernel(int
     }
 }
 
-// dw and db: the sums of the blocks' partial rows, 32 columns and 32 lanes of rows per block, lanes added by a fixed tree.
+// dw and db: the sums of the blocks' partial rows.  A block has 32 columns: 8 threads of four columns, 64 lanes of rows, the lanes
+// added by a fixed tree.  Launched so that it starts while the rows are still walked, and waits for them.
+constexpr int kColumnThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(1024) ln_rows_columns_kernel(int32_t parts, int32_t n, const float *__restrict__ partial, T *__restrict__ dw,
-                                                               T *__restrict__ db) {
-    __shared__ float sums[32][33];
+__global__ void __launch_bounds__(kColumnThreads) ln_rows_columns_kernel(int32_t parts, int32_t n, int32_t pitch, const float *__restrict__ partial,
+                                                                         T *__restrict__ dw, T *__restrict__ db) {
+    __shared__ float sums[64][33];
     T *out = blockIdx.y == 0 ? dw : db;
+    wait_for_prior_grid();
     if (!out) return;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + tx;
-    float s = 0.f;
-    if (c < n)
-        for (int p = ty; p < parts; p += 32) s += partial[((int64_t)p * 2 + blockIdx.y) * n + c];
-    sums[ty][tx] = s;
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const float *at = partial + (int64_t)blockIdx.y * pitch + blockIdx.x * 32 + tx * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = ty; p < parts; p += 64) {
+        const float4 v = *reinterpret_cast<const float4 *>(at + (int64_t)p * 2 * pitch);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+    }
+    sums[ty][tx * 4] = s.x;
+    sums[ty][tx * 4 + 1] = s.y;
+    sums[ty][tx * 4 + 2] = s.z;
+    sums[ty][tx * 4 + 3] = s.w;
     __syncthreads();
-    s = warp_sum(sums[tx][ty]);                          // warp ty holds column ty of the block
-    if (tx == 0 && (int)blockIdx.x * 32 + ty < n) out[blockIdx.x * 32 + ty] = from_f32<T>(s);
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {                        // warp v adds columns v and v + 16
+        const int c = (threadIdx.x >> 5) + 16 * k;
+        const float v = warp_sum(sums[lane][c] + sums[lane + 32][c]);
+        if (lane == 0 && (int)blockIdx.x * 32 + c < n) out[blockIdx.x * 32 + c] = from_f32<T>(v);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -329,20 +456,23 @@ struct Layout {
     int vec, nv, threads;                // threads: that share a row; 0: the kernel for long rows
 };
 
-// `most`: threads per row at most; `per_warp`: elements (single ones) or vectors per lane up to which a warp takes a row.  Above that
-// as few per thread as the threads allow.
+// `per_warp`: vectors per lane (times four: single elements) up to which a warp takes a row; `most`: the same per thread of a block of
+// 512.  Above a warp's reach as few per thread as 128, then 512 threads allow.
 Layout layout_of(int32_t n, int per_vector, bool aligned, int per_warp, int most) {
     const bool v = aligned && n % per_vector == 0;
     const int vec = v ? per_vector : 1, units = n / vec, each = v ? 1 : 4;       // 1, 2, 4 vectors; 4, 8, 16 single elements
+    auto threads = [&](int nv) { return (units + nv * 32 - 1) / (nv * 32) * 32; };
     for (int i = 1; i <= per_warp; i *= 2)
         if (units <= 32 * i * each) return {vec, i * each, 32};
-    if (units <= 128 * each) return {vec, each, (units + each * 32 - 1) / (each * 32) * 32};
-    for (int i = 2; i <= 4; i *= 2)
-        if (units <= most * i * each) return {vec, i * each, (units + i * each * 32 - 1) / (i * each * 32) * 32};
+    if (units <= 128 * each) return {vec, each, threads(each)};
+    for (int i = 2; i <= most; i *= 2)
+        if (units <= 512 * i * each) return {vec, i * each, threads(i * each)};
+    if (units <= 1024 * 4 * each) return {vec, 4 * each, 1024};
     return {1, 0, 0};
 }
-// backward: a warp takes up to two vectors per lane (a column's two sums are registers too), a block of 512 threads the rest
-Layout backward_layout(int32_t n, int per_vector, bool aligned) { return layout_of(n, per_vector, aligned, 2, 512); }
+Layout forward_layout(int32_t n, int per_vector, bool aligned) { return layout_of(n, per_vector, aligned, 2, 4); }
+// a column's two sums are registers too: at most two vectors a thread
+Layout backward_layout(int32_t n, int per_vector, bool aligned) { return layout_of(n, per_vector, aligned, 2, 2); }
 
 // Blocks of the backward pass: about 512 threads per SM (the register file holds no more), but at least four rows for each that
 // walks rows, so that the partial rows stay small beside the input.  Depends on the sizes and the device only: `threads` is taken for
@@ -354,12 +484,12 @@ int backward_blocks(const DeviceInfo &info, int32_t rows, int32_t n) {
     const int64_t blocks = ceil_div64(rows, warps ? 32 : 4), most = (int64_t)info.sm_count * (threads >= 512 ? 1 : 512 / threads);
     return (int)(blocks < most ? blocks : most);
 }
+int32_t column_pitch(int32_t n) { return (n + 31) / 32 * 32; }         // (n < 2^31 - 32: checked)
 
-int32_t check_common(int32_t rows, int32_t n, int32_t dtype) {
-    DeviceInfo info;
-    const int32_t rc = current_device_info(&info);
+int32_t check_common(DeviceInfo *info, int32_t rows, int32_t n, int32_t dtype) {
+    const int32_t rc = current_device_info(info);
     if (rc) return rc;
-    CPMK_REQUIRE(rows >= 0 && n >= 1, "bad size: rows=%d n=%d", rows, n);
+    CPMK_REQUIRE(rows >= 0 && n >= 1 && n <= 0x7fffffff - 32, "bad size: rows=%d n=%d", rows, n);
     CPMK_REQUIRE(dtype == CPMK_F16 || dtype == CPMK_BF16 || dtype == CPMK_F32, "unknown element type %d", dtype);
     return CPMK_OK;
 }
@@ -367,56 +497,65 @@ int32_t check_common(int32_t rows, int32_t n, int32_t dtype) {
 bool aligned_to(const void *p, int64_t a) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(a - 1)) == 0; }
 
 template <typename T>
-int32_t forward(int32_t rows, int32_t n, const void *xv, float eps, int rd_mean, const void *wv, const void *bv, void *yv, float *mean, float *rstd,
-                cudaStream_t stream) {
+int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv, float eps, int rd_mean, const void *wv, const void *bv, void *yv,
+                float *mean, float *rstd, cudaStream_t stream) {
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv), *b = static_cast<const T *>(bv);
     T *y = static_cast<T *>(yv);
     constexpr int kVec = 16 / (int)sizeof(T);
-    const Layout l = layout_of(n, kVec, aligned16(x) && aligned16(w) && aligned16(b) && aligned16(y), 4, 1024);
+    const Layout l = forward_layout(n, kVec, aligned16(x) && aligned16(w) && aligned16(b) && aligned16(y));
     const float inv_n = 1.f / (float)n;
-#define CPMK_LN_FORWARD(VEC, NV) \
-    else if (l.vec == VEC && l.nv == NV && l.threads == 32) \
-        ln_rows_forward_kernel<T, VEC, NV, false><<<(rows + 3) / 4, 128, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd); \
-    else if (l.vec == VEC && l.nv == NV) \
-        ln_rows_forward_kernel<T, VEC, NV, true><<<rows, l.threads, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd)
+    // as many blocks as the SMs hold (launch bounds: 1024 threads of 64 registers, 512 of 128 with four vectors)
+    const int64_t threads = l.threads == 32 ? 128 : l.threads, lanes = l.threads == 32 ? 4 : 1;
+    const int64_t per_sm = l.threads == 0 ? 1 : (l.vec * l.nv > 16 ? 512 : 1024) / threads;
+    const int64_t want = ceil_div64(rows, lanes), most = info.sm_count * (per_sm > 0 ? per_sm : 1);
+    const unsigned grid = (unsigned)(want < most ? want : most);
+#define CPMK_LN_FORWARD(VEC, NV, BLOCK, MANY, THREADS) \
+    ln_rows_forward_kernel<T, VEC, NV, BLOCK, MANY><<<grid, THREADS, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd)
+#define CPMK_LN_FORWARD_IF(VEC, EACH) \
+    else if (l.vec == VEC && l.threads == 32 && l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, false, false, 128); \
+    else if (l.vec == VEC && l.threads == 32) CPMK_LN_FORWARD(VEC, 2 * EACH, false, false, 128); \
+    else if (l.vec == VEC && l.threads == 1024) CPMK_LN_FORWARD(VEC, 4 * EACH, true, true, 1024); \
+    else if (l.vec == VEC && l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, true, false, l.threads); \
+    else if (l.vec == VEC && l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, true, false, l.threads); \
+    else if (l.vec == VEC) CPMK_LN_FORWARD(VEC, 4 * EACH, true, false, l.threads)
     if (l.threads == 0) ln_rows_forward_wide_kernel<T><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
-    CPMK_LN_FORWARD(kVec, 1);
-    CPMK_LN_FORWARD(kVec, 2);
-    CPMK_LN_FORWARD(kVec, 4);
-    CPMK_LN_FORWARD(1, 4);
-    CPMK_LN_FORWARD(1, 8);
-    CPMK_LN_FORWARD(1, 16);
+    CPMK_LN_FORWARD_IF(kVec, 1);
+    CPMK_LN_FORWARD_IF(1, 4);
+#undef CPMK_LN_FORWARD_IF
 #undef CPMK_LN_FORWARD
     CPMK_LAUNCH_CHECK();
     return CPMK_OK;
 }
 
 template <typename T, bool COLUMNS>
-int32_t backward_rows(int blocks, int32_t rows, int32_t n, const T *dy, const T *x, int rd_mean, const T *w, const float *mean, const float *rstd, T *dx,
-                      float *partial, cudaStream_t stream) {
+int32_t backward_rows(const DeviceInfo &info, int blocks, int32_t rows, int32_t n, const T *dy, const T *x, int rd_mean, const T *w, const float *mean,
+                      const float *rstd, T *dx, float *partial, cudaStream_t stream) {
     constexpr int kVec = 16 / (int)sizeof(T);
-    const Layout l = backward_layout(n, kVec, aligned16(x) && aligned16(dy) && aligned16(w) && aligned16(dx));
+    Layout l = backward_layout(n, kVec, aligned16(x) && aligned16(dy) && aligned16(w) && aligned16(dx));
     const float inv_n = 1.f / (float)n;
-#define CPMK_LN_BACKWARD_WARP(VEC, NV) \
-    else if (l.vec == VEC && l.nv == NV && l.threads == 32) \
-        ln_rows_backward_kernel<T, VEC, NV, false, COLUMNS><<<blocks, 256, COLUMNS ? 2 * n * sizeof(float) : 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, \
-                                                                                                                       rstd, w, dx, partial)
-#define CPMK_LN_BACKWARD_BLOCK(VEC, NV) \
-    else if (l.vec == VEC && l.nv == NV) \
-        ln_rows_backward_kernel<T, VEC, NV, true, COLUMNS><<<blocks, l.threads, 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial)
-    if (l.threads == 0) ln_rows_backward_wide_kernel<T, COLUMNS><<<blocks, kWideThreads, 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial);
-    CPMK_LN_BACKWARD_WARP(kVec, 1);
-    CPMK_LN_BACKWARD_WARP(kVec, 2);
-    CPMK_LN_BACKWARD_WARP(1, 4);
-    CPMK_LN_BACKWARD_WARP(1, 8);
-    CPMK_LN_BACKWARD_BLOCK(kVec, 1);
-    CPMK_LN_BACKWARD_BLOCK(kVec, 2);
-    CPMK_LN_BACKWARD_BLOCK(kVec, 4);
-    CPMK_LN_BACKWARD_BLOCK(1, 4);
-    CPMK_LN_BACKWARD_BLOCK(1, 8);
-    CPMK_LN_BACKWARD_BLOCK(1, 16);
-#undef CPMK_LN_BACKWARD_WARP
-#undef CPMK_LN_BACKWARD_BLOCK
+    const int32_t pitch = column_pitch(n);
+    const int64_t sums = COLUMNS ? 2 * (int64_t)n * (int64_t)sizeof(float) : 0;
+    if (l.threads == 1024 && sums > info.max_smem_optin - 1024) l = {1, 0, 0};   // the kernel's static arrays take half a KiB
+#define CPMK_LN_BACKWARD(VEC, NV, BLOCK, THREADS, SMEM) \
+    ln_rows_backward_kernel<T, VEC, NV, BLOCK, COLUMNS><<<blocks, THREADS, SMEM, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch)
+#define CPMK_LN_BACKWARD_LONG(VEC, NV) \
+    { \
+        if (COLUMNS) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums)); \
+        ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS><<<blocks, 1024, sums, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch); \
+    }
+#define CPMK_LN_BACKWARD_IF(VEC, EACH) \
+    else if (l.vec == VEC && l.threads == 32 && l.nv == EACH) CPMK_LN_BACKWARD(VEC, EACH, false, 256, 8 * sums); \
+    else if (l.vec == VEC && l.threads == 32) CPMK_LN_BACKWARD(VEC, 2 * EACH, false, 256, 8 * sums); \
+    else if (l.vec == VEC && l.threads == 1024) CPMK_LN_BACKWARD_LONG(VEC, 4 * EACH) \
+    else if (l.vec == VEC && l.nv == EACH) CPMK_LN_BACKWARD(VEC, EACH, true, l.threads, 0); \
+    else if (l.vec == VEC) CPMK_LN_BACKWARD(VEC, 2 * EACH, true, l.threads, 0);
+    if (l.threads == 0)
+        ln_rows_backward_wide_kernel<T, COLUMNS><<<blocks, kWideThreads, 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch);
+    CPMK_LN_BACKWARD_IF(kVec, 1)
+    CPMK_LN_BACKWARD_IF(1, 4)
+#undef CPMK_LN_BACKWARD_IF
+#undef CPMK_LN_BACKWARD_LONG
+#undef CPMK_LN_BACKWARD
     CPMK_LAUNCH_CHECK();
     return CPMK_OK;
 }
@@ -427,11 +566,11 @@ int32_t backward(const DeviceInfo &info, int32_t rows, int32_t n, const void *dy
     const T *dy = static_cast<const T *>(dyv), *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     T *dx = static_cast<T *>(dxv);
     const int blocks = backward_blocks(info, rows, n);
-    if (!dw && !db) return backward_rows<T, false>(blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, nullptr, stream);
-    const int32_t rc = backward_rows<T, true>(blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, partial, stream);
+    if (!dw && !db) return backward_rows<T, false>(info, blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, nullptr, stream);
+    const int32_t rc = backward_rows<T, true>(info, blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, partial, stream);
     if (rc) return rc;
-    ln_rows_columns_kernel<T><<<dim3((n + 31) / 32, 2), 1024, 0, stream>>>(blocks, n, partial, static_cast<T *>(dw), static_cast<T *>(db));
-    CPMK_LAUNCH_CHECK();
+    CPMK_CUDA_TRY(launch_after_prior(ln_rows_columns_kernel<T>, dim3((n + 31) / 32, 2), dim3(kColumnThreads), 0, stream, blocks, n, column_pitch(n),
+                                     static_cast<const float *>(partial), static_cast<T *>(dw), static_cast<T *>(db)));
     return CPMK_OK;
 }
 
@@ -444,7 +583,8 @@ extern "C" {
 
 int32_t cpmk_layernorm_rows_forward(int32_t rows, int32_t n, int32_t dtype, const void *x, float eps, int32_t rd_mean, const void *weight,
                                     const void *bias, void *y, void *mean, void *rstd, cpmk_stream_t stream) {
-    const int32_t rc = check_common(rows, n, dtype);
+    DeviceInfo info;
+    const int32_t rc = check_common(&info, rows, n, dtype);
     if (rc) return rc;
     CPMK_REQUIRE(eps >= 0.f, "eps must not be negative");
     if (rows == 0) return CPMK_OK;
@@ -455,26 +595,24 @@ int32_t cpmk_layernorm_rows_forward(int32_t rows, int32_t n, int32_t dtype, cons
                  "misaligned pointer");
     const cudaStream_t s = as_stream(stream);
     float *m = static_cast<float *>(mean), *r = static_cast<float *>(rstd);
-    if (dtype == CPMK_F16) return forward<__half>(rows, n, x, eps, rd_mean != 0, weight, bias, y, m, r, s);
-    if (dtype == CPMK_BF16) return forward<__nv_bfloat16>(rows, n, x, eps, rd_mean != 0, weight, bias, y, m, r, s);
-    return forward<float>(rows, n, x, eps, rd_mean != 0, weight, bias, y, m, r, s);
+    if (dtype == CPMK_F16) return forward<__half>(info, rows, n, x, eps, rd_mean != 0, weight, bias, y, m, r, s);
+    if (dtype == CPMK_BF16) return forward<__nv_bfloat16>(info, rows, n, x, eps, rd_mean != 0, weight, bias, y, m, r, s);
+    return forward<float>(info, rows, n, x, eps, rd_mean != 0, weight, bias, y, m, r, s);
 }
 
 int32_t cpmk_layernorm_rows_backward_scratch(int32_t rows, int32_t n, int64_t *bytes) {
     DeviceInfo info;
-    const int32_t rc = current_device_info(&info);
+    const int32_t rc = check_common(&info, rows, n, CPMK_F16);
     if (rc) return rc;
-    CPMK_REQUIRE(rows >= 0 && n >= 1 && bytes, "bad size: rows=%d n=%d", rows, n);
-    *bytes = (int64_t)backward_blocks(info, rows, n) * 2 * n * (int64_t)sizeof(float);
+    CPMK_REQUIRE(bytes, "null pointer");
+    *bytes = (int64_t)backward_blocks(info, rows, n) * 2 * column_pitch(n) * (int64_t)sizeof(float);
     return CPMK_OK;
 }
 
 int32_t cpmk_layernorm_rows_backward(int32_t rows, int32_t n, int32_t dtype, const void *dy, const void *x, int32_t rd_mean, const void *weight,
                                      const void *mean, const void *rstd, void *dx, void *dweight, void *dbias, void *scratch, cpmk_stream_t stream) {
     DeviceInfo info;
-    int32_t rc = check_common(rows, n, dtype);
-    if (rc) return rc;
-    rc = current_device_info(&info);
+    const int32_t rc = check_common(&info, rows, n, dtype);
     if (rc) return rc;
     if (!dx && !dweight && !dbias) return CPMK_OK;
     const int64_t es = dtype_size(dtype);

@@ -64,6 +64,11 @@ __device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void *src, uint
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+// Kernels launched one behind the other with launch_after_prior: the first lets the second's blocks start; the second waits until the
+// first has finished and its writes are visible.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // L2 eviction priorities for bulk copies: lines fetched with evict_last stay in L2 ahead of everything fetched
 // normally (for data a following pass reads again), lines touched with evict_first are the first to go.
 __device__ __forceinline__ uint64_t l2_policy_evict_last() {

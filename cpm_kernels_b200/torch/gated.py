@@ -7,6 +7,7 @@ import torch
 
 from ..kernels import gated_linear_forward, gated_linear_backward, gated_feed_forward_forward, gated_feed_forward_backward, gated_scratch
 from ..library import cpmk
+from ._launch import address, launch, once
 
 _DTYPES = {torch.float16: cpmk.F16, torch.bfloat16: cpmk.BF16}
 
@@ -21,24 +22,29 @@ def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation
     assert activation in cpmk.ACTIVATIONS
 
 
-def _scratch(tokens: int, k: int, n: int, m: int, device) -> torch.Tensor:
-    return torch.empty((gated_scratch(tokens, k, n, m),), dtype=torch.uint8, device=device)
+def _scratch(tokens: int, k: int, n: int, m: int, device):
+    size = gated_scratch(tokens, k, n, m)
+    return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
 
 
-def _ptr(t) -> int:
-    return t.data_ptr() if t is not None else 0
+def _part(t, i: int) -> int:
+    """Address of t[i] for a contiguous t, without a view of it."""
+    return t.data_ptr() + i * (t.numel() // t.size(0)) * t.element_size()
+
+
+def _launch_linear(x, w_gate, w_up, activation, h, gu, stream):
+    n, k = w_gate.shape
+    tokens = x.numel() // k
+    scratch = _scratch(tokens, k, n, 0, x.device)
+    gated_linear_forward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(),
+                         _part(gu, 0) if gu is not None else 0, _part(gu, 1) if gu is not None else 0, address(scratch), stream)
 
 
 def _linear_forward(x, w_gate, w_up, activation: str, save: bool):
     n, k = w_gate.shape
-    tokens = x.numel() // k
     h = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    gu = torch.empty((2, tokens, n), dtype=x.dtype, device=x.device) if save else None
-    with torch.cuda.device(x.device):
-        scratch = _scratch(tokens, k, n, 0, x.device)
-        gated_linear_forward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-                             h.data_ptr(), _ptr(gu[0]) if save else 0, _ptr(gu[1]) if save else 0, scratch.data_ptr(),
-                             torch.cuda.current_stream().cuda_stream)
+    gu = torch.empty((2, x.numel() // k, n), dtype=x.dtype, device=x.device) if save else None
+    launch(x.get_device(), _launch_linear, x, w_gate, w_up, activation, h, gu)
     return h, gu
 
 
@@ -51,19 +57,16 @@ class OpGatedLinear(torch.autograd.Function):
         ctx.activation = activation
         return h
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, grad_output: torch.Tensor):
         x, w_gate, w_up, gu = ctx.saved_tensors
         dh = grad_output.contiguous()
         n, k = w_gate.shape
-        tokens = x.numel() // k
         dgu = torch.empty_like(gu)
         dx, dw_gate, dw_up = (torch.empty_like(t) if need else None for t, need in zip((x, w_gate, w_up), ctx.needs_input_grad))
-        with torch.cuda.device(x.device):
-            gated_linear_backward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation], dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
-                                  w_up.data_ptr(), gu[0].data_ptr(), gu[1].data_ptr(), dgu[0].data_ptr(), dgu[1].data_ptr(), _ptr(dx), _ptr(dw_gate),
-                                  _ptr(dw_up), torch.cuda.current_stream().cuda_stream)
+        launch(x.get_device(), gated_linear_backward, x.numel() // k, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation], dh.data_ptr(),
+               x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _part(gu, 0), _part(gu, 1), _part(dgu, 0), _part(dgu, 1), address(dx), address(dw_gate),
+               address(dw_up))
         return dx, dw_gate, dw_up, None
 
 
@@ -77,17 +80,22 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     return _linear_forward(x, w_gate, w_up, activation, False)[0]
 
 
-def _block_forward(x, w_gate, w_up, w_down, activation: str, save: bool):
+def _launch_block(x, w_gate, w_up, w_down, activation, hgu, y, stream):
     n, k = w_gate.shape
     m = w_down.size(0)
     tokens = x.numel() // k
-    y = torch.empty((*x.shape[:-1], m), dtype=x.dtype, device=x.device)
-    hgu = torch.empty((3 if save else 1, tokens, n), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        scratch = _scratch(tokens, k, n, m, x.device)
-        gated_feed_forward_forward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-                                   w_down.data_ptr(), hgu[0].data_ptr(), hgu[1].data_ptr() if save else 0, hgu[2].data_ptr() if save else 0,
-                                   y.data_ptr(), scratch.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    scratch = _scratch(tokens, k, n, m, x.device)
+    save = hgu.size(0) == 3
+    gated_feed_forward_forward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                               w_down.data_ptr(), hgu.data_ptr(), _part(hgu, 1) if save else 0, _part(hgu, 2) if save else 0, y.data_ptr(),
+                               address(scratch), stream)
+
+
+def _block_forward(x, w_gate, w_up, w_down, activation: str, save: bool):
+    n, k = w_gate.shape
+    y = torch.empty((*x.shape[:-1], w_down.size(0)), dtype=x.dtype, device=x.device)
+    hgu = torch.empty((3 if save else 1, x.numel() // k, n), dtype=x.dtype, device=x.device)      # h, and g, u for the backward pass
+    launch(x.get_device(), _launch_block, x, w_gate, w_up, w_down, activation, hgu, y)
     return y, hgu
 
 
@@ -100,21 +108,17 @@ class OpGatedFeedForward(torch.autograd.Function):
         ctx.activation = activation
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, grad_output: torch.Tensor):
         x, w_gate, w_up, w_down, hgu = ctx.saved_tensors
         dy = grad_output.contiguous()
         n, k = w_gate.shape
-        m = w_down.size(0)
         tokens = x.numel() // k
         dgu = torch.empty((2, tokens, n), dtype=x.dtype, device=x.device)
         dx, dw_gate, dw_up, dw_down = (torch.empty_like(t) if need else None for t, need in zip((x, w_gate, w_up, w_down), ctx.needs_input_grad))
-        with torch.cuda.device(x.device):
-            gated_feed_forward_backward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation], dy.data_ptr(), x.data_ptr(),
-                                        w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), hgu[1].data_ptr(), hgu[2].data_ptr(),
-                                        hgu[0].data_ptr(), dgu[0].data_ptr(), dgu[1].data_ptr(), _ptr(dx), _ptr(dw_gate), _ptr(dw_up),
-                                        _ptr(dw_down), torch.cuda.current_stream().cuda_stream)
+        launch(x.get_device(), gated_feed_forward_backward, tokens, k, n, w_down.size(0), _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation],
+               dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _part(hgu, 1), _part(hgu, 2), hgu.data_ptr(),
+               _part(dgu, 0), _part(dgu, 1), address(dx), address(dw_gate), address(dw_up), address(dw_down))
         return dx, dw_gate, dw_up, dw_down, None
 
 

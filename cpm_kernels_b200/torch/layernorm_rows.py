@@ -7,20 +7,30 @@ import torch
 
 from ..kernels import layernorm_rows_forward, layernorm_rows_backward, layernorm_rows_backward_scratch
 from ..library import cpmk
+from ._launch import address, launch, once
 
 _DTYPES = {torch.float16: cpmk.F16, torch.bfloat16: cpmk.BF16, torch.float32: cpmk.F32}
 
 
 def _forward(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Optional[torch.Tensor], rd_mean: bool, statistics: bool):
-    n = x.size(-1)
+    """(y, stats): stats holds the rows' means, then their reciprocal deviations, when they are wanted."""
+    n = weight.numel()
     rows = x.numel() // n
     y = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if statistics else None
-    with torch.cuda.device(x.device):
-        layernorm_rows_forward(rows, n, _DTYPES[x.dtype], x.data_ptr(), eps, rd_mean, weight.data_ptr(), bias.data_ptr() if bias is not None else 0,
-                               y.data_ptr(), stats[0].data_ptr() if statistics else 0, stats[1].data_ptr() if statistics else 0,
-                               torch.cuda.current_stream().cuda_stream)
+    stats = torch.empty((2 * rows,), dtype=torch.float32, device=x.device) if statistics else None
+    mean = address(stats)
+    launch(x.get_device(), layernorm_rows_forward, rows, n, _DTYPES[x.dtype], x.data_ptr(), eps, rd_mean, weight.data_ptr(), address(bias), y.data_ptr(),
+           mean, mean + 4 * rows if statistics else 0)
     return y, stats
+
+
+def _launch_backward(rows, n, dtype, dy, x, rd_mean, weight, stats, dx, dweight, dbias, stream):
+    scratch = None
+    if dweight is not None or dbias is not None:
+        scratch = torch.empty((layernorm_rows_backward_scratch(rows, n),), dtype=torch.uint8, device=x.device)
+    mean = stats.data_ptr()
+    layernorm_rows_backward(rows, n, dtype, dy.data_ptr(), x.data_ptr(), rd_mean, weight.data_ptr(), mean, mean + 4 * rows, address(dx), address(dweight),
+                            address(dbias), address(scratch), stream)
 
 
 class OpLayerNormRows(torch.autograd.Function):
@@ -32,21 +42,16 @@ class OpLayerNormRows(torch.autograd.Function):
         ctx.rd_mean = rd_mean
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, grad_output: torch.Tensor):
         x, weight, stats = ctx.saved_tensors
-        dy = grad_output.contiguous()
-        n = x.size(-1)
-        rows = x.numel() // n
-        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-        dweight = torch.empty_like(weight) if ctx.needs_input_grad[2] else None
-        dbias = torch.empty_like(weight) if ctx.needs_input_grad[3] else None
-        with torch.cuda.device(x.device):
-            scratch = torch.empty((layernorm_rows_backward_scratch(rows, n),), dtype=torch.uint8, device=x.device)
-            layernorm_rows_backward(rows, n, _DTYPES[x.dtype], dy.data_ptr(), x.data_ptr(), ctx.rd_mean, weight.data_ptr(), stats[0].data_ptr(),
-                                    stats[1].data_ptr(), dx.data_ptr() if dx is not None else 0, dweight.data_ptr() if dweight is not None else 0,
-                                    dbias.data_ptr() if dbias is not None else 0, scratch.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        n = weight.numel()
+        want_x, _, want_weight, want_bias, _ = ctx.needs_input_grad
+        dx = torch.empty_like(x) if want_x else None
+        dweight = torch.empty_like(weight) if want_weight else None
+        dbias = torch.empty_like(weight) if want_bias else None
+        launch(x.get_device(), _launch_backward, x.numel() // n, n, _DTYPES[x.dtype], grad_output.contiguous(), x, ctx.rd_mean, weight, stats, dx, dweight,
+               dbias)
         return dx, None, dweight, dbias, None
 
 
