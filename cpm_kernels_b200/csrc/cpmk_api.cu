@@ -108,6 +108,33 @@ int32_t get_workspace(cudaStream_t stream, Workspace *ws) {
     return CPMK_OK;
 }
 
+static std::map<int, uint32_t *> g_device_status;
+
+int32_t get_device_status(uint32_t **status) {
+    int dev = 0;
+    CPMK_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(g_mutex);
+    auto it = g_device_status.find(dev);
+    if (it == g_device_status.end()) {
+        void *p = nullptr;
+        CPMK_CUDA_TRY(cudaMalloc(&p, 256));
+        CPMK_CUDA_TRY(cudaMemset(p, 0, 256));
+        it = g_device_status.emplace(dev, static_cast<uint32_t *>(p)).first;
+    }
+    *status = it->second;
+    return CPMK_OK;
+}
+
+// Reads and clears the device's status word (0 when it has none yet).  The caller holds g_mutex and has synchronised.
+static int32_t collect_device_status(int dev, uint32_t *word) {
+    *word = 0;
+    auto it = g_device_status.find(dev);
+    if (it == g_device_status.end()) return CPMK_OK;
+    CPMK_CUDA_TRY(cudaMemcpy(word, it->second, sizeof(*word), cudaMemcpyDeviceToHost));
+    if (*word != 0) CPMK_CUDA_TRY(cudaMemset(it->second, 0, 256));
+    return CPMK_OK;
+}
+
 // Reads the status word of one workspace; when a kernel recorded a failure there, clears the word AND the ticket
 // region: a kernel that gave up a wait leaves without taking its ticket, so the counters it shares with later calls
 // are no longer at zero.  The caller holds g_mutex and has synchronised the work that uses the workspace.
@@ -151,7 +178,10 @@ int32_t cpmk_read_status(uint32_t *status_out) {
         if (rc) return rc;
         if (word != 0 && worst == 0) worst = word;
     }
-    *status_out = worst;
+    uint32_t word = 0;
+    const int32_t rc = cpmk::collect_device_status(dev, &word);
+    if (rc) return rc;
+    *status_out = worst ? worst : word;
     return CPMK_OK;
 }
 
@@ -160,11 +190,15 @@ int32_t cpmk_check_stream(cpmk_stream_t stream) {
     CPMK_CUDA_TRY(cudaGetDevice(&dev));
     CPMK_CUDA_TRY(cudaStreamSynchronize(cpmk::as_stream(stream)));
     std::lock_guard<std::mutex> lock(cpmk::g_mutex);
+    uint32_t word = 0, of_device = 0;
     auto it = cpmk::g_workspaces.find(std::make_pair(dev, cpmk::as_stream(stream)));
-    if (it == cpmk::g_workspaces.end()) return CPMK_OK;          // no kernel with a bounded wait ran on this stream
-    uint32_t word = 0;
-    const int32_t rc = cpmk::collect_status(it->second, &word);
+    if (it != cpmk::g_workspaces.end()) {
+        const int32_t rc = cpmk::collect_status(it->second, &word);
+        if (rc) return rc;
+    }
+    const int32_t rc = cpmk::collect_device_status(dev, &of_device);
     if (rc) return rc;
+    if (word == 0) word = of_device;
     if (word != 0) {
         cpmk::set_error("a kernel on this stream gave up a bounded wait (code 0x%x); its output is incomplete", word);
         return CPMK_EDEVICE;

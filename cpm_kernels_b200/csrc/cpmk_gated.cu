@@ -1,46 +1,14 @@
 // Gated feed-forward block: h = act(x Wg^T) * (x Wu^T), y = h Wd^T, and its backward pass, in fp16 and bf16 with fp32 sums.
 //
 //   backward   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
-#include "cpmk_common.cuh"
-#include "cpmk_types.cuh"
+#include "cpmk_gated.cuh"
 
 namespace cpmk {
 namespace {
 
 // ------------------------------------------------------------------------------------------------
-// the activation
-// ------------------------------------------------------------------------------------------------
-// Both activations are v s(z(v)) with the logistic function s: z = v (silu), z = 2 c (v + 0.044715 v^3), c = sqrt(2 / pi) (gelu:
-// (1 + tanh t) / 2 = s(2 t)).  Derivative: s + v s (1 - s) z'(v).  Beyond |v| = 30 the logistic is 0 or 1 in fp32 (|z| > 1900), so z
-// and z' are taken of the clamped value: the cube cannot overflow and 0 * inf does not arise.
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-
-template <int ACT>
-__device__ __forceinline__ float act_value(float v) {
-    if (ACT == CPMK_ACT_SILU) return v * logistic(v);
-    const float c = fminf(fmaxf(v, -30.f), 30.f);
-    return v * logistic(1.5957691216057308f * fmaf(0.044715f * c * c, c, c));
-}
-
-template <int ACT>
-__device__ __forceinline__ void act_value_slope(float v, float &value, float &slope) {
-    if (ACT == CPMK_ACT_SILU) {
-        const float s = logistic(v);
-        value = v * s;
-        slope = fmaf(value, 1.f - s, s);
-    } else {
-        const float c = fminf(fmaxf(v, -30.f), 30.f), c2 = c * c;
-        const float s = logistic(1.5957691216057308f * fmaf(0.044715f * c2, c, c));
-        value = v * s;
-        slope = fmaf(value * (1.f - s), 1.5957691216057308f * fmaf(3.f * 0.044715f, c2, 1.f), s);
-    }
-}
-
-// ------------------------------------------------------------------------------------------------
 // Generic product: out[r, c] = sum_k P[r, k] Q[c, k] with any strides, 64 x 64 outputs per block of 256 threads, 4 x 4 per thread.
 // ------------------------------------------------------------------------------------------------
-enum { kEpiStore = 0, kEpiGated = 1, kEpiDact = 2 };
-
 struct SimtParams {
     int32_t R, C, K;
     int64_t tiles_c;
@@ -132,12 +100,6 @@ __global__ void __launch_bounds__(256) gated_dact_kernel(int64_t count, const T 
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
-struct Call {
-    DeviceInfo info;
-    int32_t dtype, act;
-    cudaStream_t stream;
-};
-
 template <int EPI>
 int32_t launch_simt(const Call &call, SimtParams prm) {
     prm.tiles_c = ceil_div64(prm.C, kSimtTile);
@@ -156,19 +118,35 @@ int32_t launch_simt(const Call &call, SimtParams prm) {
     return CPMK_OK;
 }
 
-// out (R, C) = P Q^T summed over one or two pairs of operands.  p_t / q_t: the operand is stored (K, rows) instead of (rows, K).
+bool tensor_core_size(int32_t extent) { return extent % 8 == 0; }
+
+// out0 (R, C) = P0 Q0^T (+ P1 Q1^T when `sum`), or out0 = P0 Q0^T and out1 = P1 Q1^T when out1 is given.  p_t / q_t: the operand is stored
+// (K, rows) instead of (rows, K).  The tensor cores' loads and stores want 16-byte rows and addresses; everything else runs generic.
 int32_t product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1, const void *q1,
-                void *out) {
+                bool sum, void *out0, void *out1) {
+    if (tensor_core_size(p_t ? R : K) && tensor_core_size(q_t ? C : K) && tensor_core_size(C) && aligned16(p0) && aligned16(q0) && aligned16(p1) &&
+        aligned16(q1) && aligned16(out0) && aligned16(out1))
+        return tc_product(call, R, C, K, p_t, q_t, p0, q0, p1, q1, sum, out0, out1);
     SimtParams prm = {};
     prm.R = R; prm.C = C; prm.K = K;
     prm.p_rs = p_t ? 1 : K; prm.p_ks = p_t ? R : 1;
     prm.q_rs = q_t ? 1 : K; prm.q_ks = q_t ? C : 1;
-    prm.p[0] = p0; prm.p[1] = p1; prm.q[0] = q0; prm.q[1] = q1;
-    prm.out[0] = out;
+    prm.p[0] = p0; prm.q[0] = q0;
+    if (sum) {
+        prm.p[1] = p1;
+        prm.q[1] = q1;
+    }
+    prm.out[0] = out0;
+    const int32_t rc = launch_simt<kEpiStore>(call, prm);
+    if (rc || !out1) return rc;
+    prm.p[0] = p1; prm.q[0] = q1;
+    prm.out[0] = out1;
     return launch_simt<kEpiStore>(call, prm);
 }
 
 int32_t gated_product(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u) {
+    if (tensor_core_size(k) && tensor_core_size(n) && aligned16(x) && aligned16(wg) && aligned16(wu) && aligned16(h) && aligned16(g) && aligned16(u))
+        return tc_gated(call, tokens, k, n, x, wg, wu, h, g, u);
     SimtParams prm = {};
     prm.R = tokens; prm.C = n; prm.K = k;
     prm.p_rs = k; prm.p_ks = 1; prm.q_rs = k; prm.q_ks = 1;
@@ -180,6 +158,8 @@ int32_t gated_product(const Call &call, int32_t tokens, int32_t k, int32_t n, co
 // dg, du from dh = dy Wd, which is not stored; Wd is (m, n)
 int32_t dact_product(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg,
                      void *du) {
+    if (tensor_core_size(n) && tensor_core_size(m) && aligned16(dy) && aligned16(wd) && aligned16(g) && aligned16(u) && aligned16(dg) && aligned16(du))
+        return tc_dact(call, tokens, n, m, dy, wd, g, u, dg, du);
     SimtParams prm = {};
     prm.R = tokens; prm.C = n; prm.K = m;
     prm.p_rs = m; prm.p_ks = 1; prm.q_rs = 1; prm.q_ks = n;
@@ -225,10 +205,10 @@ int32_t begin(Call *call, int32_t tokens, int32_t k, int32_t n, int32_t m, int32
 int32_t projections_backward(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, const void *dg,
                              const void *du, void *dx, void *dwg, void *dwu) {
     int32_t rc = CPMK_OK;
-    if (dx) rc = product(call, tokens, k, n, false, true, dg, wg, du, wu, dx);
-    if (!rc && dwg) rc = product(call, n, k, tokens, true, true, dg, x, nullptr, nullptr, dwg);
-    if (!rc && dwu) rc = product(call, n, k, tokens, true, true, du, x, nullptr, nullptr, dwu);
-    return rc;
+    if (dx) rc = product(call, tokens, k, n, false, true, dg, wg, du, wu, true, dx, nullptr);
+    if (rc || (!dwg && !dwu)) return rc;
+    if (dwg && dwu) return product(call, n, k, tokens, true, true, dg, x, du, x, false, dwg, dwu);
+    return product(call, n, k, tokens, true, true, dwg ? dg : du, x, nullptr, nullptr, false, dwg ? dwg : dwu, nullptr);
 }
 
 // without tokens the weights' gradients are zero
@@ -300,7 +280,7 @@ int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, in
     CPMK_REQUIRE(aligned16(scratch), "scratch must be 16-byte aligned");
     rc = gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u);
     if (rc) return rc;
-    return product(call, tokens, m, n, false, false, h, w_down, nullptr, nullptr, y);
+    return product(call, tokens, m, n, false, false, h, w_down, nullptr, nullptr, false, y, nullptr);
 }
 
 int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *dy,
@@ -321,7 +301,7 @@ int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, i
         rc = projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up);
         if (rc) return rc;
     }
-    if (dw_down) return product(call, m, n, tokens, true, true, dy, h, nullptr, nullptr, dw_down);
+    if (dw_down) return product(call, m, n, tokens, true, true, dy, h, nullptr, nullptr, false, dw_down, nullptr);
     return CPMK_OK;
 }
 

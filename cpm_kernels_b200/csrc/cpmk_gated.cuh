@@ -1,0 +1,55 @@
+// What the kernel files of the gated feed-forward block share: the activations, one call's constants, and the launchers of the
+// tensor-core kernels.
+#pragma once
+
+#include "cpmk_common.cuh"
+#include "cpmk_types.cuh"
+
+namespace cpmk {
+
+// ------------------------------------------------------------------------------------------------
+// the activation
+// ------------------------------------------------------------------------------------------------
+// Both activations are v s(z(v)) with the logistic function s: z = v (silu), z = 2 c (v + 0.044715 v^3), c = sqrt(2 / pi) (gelu:
+// (1 + tanh t) / 2 = s(2 t)).  Derivative: s + v s (1 - s) z'(v).  Beyond |v| = 30 the logistic is 0 or 1 in fp32 (|z| > 1900), so z
+// and z' are taken of the clamped value: the cube cannot overflow and 0 * inf does not arise.
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float v) {
+    if (ACT == CPMK_ACT_SILU) return v * logistic(v);
+    const float c = fminf(fmaxf(v, -30.f), 30.f);
+    return v * logistic(1.5957691216057308f * fmaf(0.044715f * c * c, c, c));
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_value_slope(float v, float &value, float &slope) {
+    if (ACT == CPMK_ACT_SILU) {
+        const float s = logistic(v);
+        value = v * s;
+        slope = fmaf(value, 1.f - s, s);
+    } else {
+        const float c = fminf(fmaxf(v, -30.f), 30.f), c2 = c * c;
+        const float s = logistic(1.5957691216057308f * fmaf(0.044715f * c2, c, c));
+        value = v * s;
+        slope = fmaf(value * (1.f - s), 1.5957691216057308f * fmaf(3.f * 0.044715f, c2, 1.f), s);
+    }
+}
+
+// What becomes of a finished sum: stored; with its partner (gate and up) through the activation; as dh through the activation's slope.
+enum { kEpiStore = 0, kEpiGated = 1, kEpiDact = 2 };
+
+struct Call {
+    DeviceInfo info;
+    int32_t dtype, act;
+    cudaStream_t stream;
+};
+
+// Tensor-core products on 256 x 256 tiles (cpmk_gated_tc.cu): extents multiples of 8, pointers 16-byte aligned.
+// out0 (R, C) = P0 Q0^T (+ P1 Q1^T when `sum`), or out0 = P0 Q0^T and out1 = P1 Q1^T when out1 is given.  p_t / q_t: stored (K, rows).
+int32_t tc_product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1,
+                   const void *q1, bool sum, void *out0, void *out1);
+int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u);
+int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg, void *du);
+
+}  // namespace cpmk

@@ -26,6 +26,7 @@
 
 #include "cpmk_common.cuh"
 #include "cpmk_ptx.cuh"
+#include "cpmk_tc.cuh"
 
 namespace cpmk {
 namespace {
@@ -79,27 +80,6 @@ struct GemmParams {
     uint32_t per_batch, per_batch_mul, per_batch_shr, tiles_r_mul, tiles_r_shr;
 };
 
-// Division of a 31-bit value by a constant through a multiply-high: q = umulhi(x, mul) >> shr with
-// mul = ceil(2^(31 + ceil(log2 d)) / d), shr = ceil(log2 d) - 1; exact for 0 <= x < 2^31 (d = 1: q = x).
-inline void find_divisor(uint32_t d, uint32_t *mul, uint32_t *shr) {
-    if (d <= 1) {
-        *mul = 0;
-        *shr = 0;
-        return;
-    }
-    uint32_t lg = 0;
-    while ((1ull << lg) < d) ++lg;
-    const uint32_t p = 31 + lg;
-    *mul = (uint32_t)(((1ull << p) + d - 1) / d);
-    *shr = p - 32;
-}
-__host__ __device__ __forceinline__ uint32_t fast_div(uint32_t x, uint32_t d, uint32_t mul, uint32_t shr) {
-#if defined(__CUDA_ARCH__)
-    return d == 1 ? x : (__umulhi(x, mul) >> shr);
-#else
-    return d == 1 ? x : (uint32_t)(((uint64_t)x * mul) >> 32) >> shr;
-#endif
-}
 inline void set_tile_divisors(GemmParams *prm) {
     prm->per_batch = (uint32_t)prm->tiles_r * (uint32_t)prm->tiles_c;
     find_divisor(prm->per_batch, &prm->per_batch_mul, &prm->per_batch_shr);
@@ -112,24 +92,6 @@ __device__ __forceinline__ void tile_coords(const GemmParams &prm, int tile, int
     r_blk = rem - c_blk * prm.tiles_r;
 }
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int32_t c0, int32_t c1, int32_t c2, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-        : "memory");
-}
-
-__device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-
 // D[tmem] (+)= A[smem desc] * B[smem desc]^T, int8 operands, int32 accumulator
 __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -139,62 +101,9 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// arrives on `bar` once all tcgen05.mma issued so far by this thread have completed
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
-          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Shared-memory matrix descriptor of a k-major tile whose rows are 128 bytes, stored with the 128-byte
-// swizzle (what TMA writes with CU_TENSOR_MAP_SWIZZLE_128B): 8-row groups are 1024 bytes apart.
-//   bits [0,14)  start address >> 4        bits [16,30) leading byte offset >> 4 (unused here: 1)
-//   bits [32,46) stride byte offset >> 4   bits [46,48) descriptor version (1 on sm_100)
-//   bits [61,64) layout type (2 = 128-byte swizzle)
-__device__ __forceinline__ uint64_t make_kmajor_sw128_desc(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3ffffu) >> 4);
-    d |= (uint64_t)1u << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1u << 46;
-    d |= (uint64_t)2u << 61;
-    return d;
-}
-
-// Shared-memory matrix descriptor of an MN-major tile (the operand's rows, not k, are contiguous in memory): what
-// TMA writes for a box of 128 elements (one 128-byte swizzle row) by kBK k-rows.  Eight k-rows form a 1024-byte
-// swizzle atom (stride byte offset); a further block of 128 elements along M/N, when an MMA spans more than
-// one, lies `mn_block_bytes` away (leading byte offset).
-__device__ __forceinline__ uint64_t make_mnmajor_sw128_desc(uint32_t smem_addr, uint32_t mn_block_bytes) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3ffffu) >> 4);
-    d |= (uint64_t)((mn_block_bytes >> 4) & 0x3fffu) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1u << 46;
-    d |= (uint64_t)2u << 61;
-    return d;
-}
-
 // Instruction descriptor of tcgen05.mma kind::i8: int32 accumulator (bits 4-5 = 2), signed 8-bit A and B
 // (bits 7-9 = 1, 10-12 = 1), both k-major (bits 15, 16 = 0), N >> 3 at bits 17-22, M >> 4 at bits 24-28.
 constexpr uint32_t kInstrDesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t *>(&h);
-}
 
 // One epilogue warp's share of a finished accumulator: TMEM lanes [32*quarter, 32*quarter+32) = output rows
 // row_base + 32*quarter + lane, all kBN columns from col_base, 32 columns per tcgen05.ld.
@@ -402,40 +311,6 @@ constexpr int kOutStagingBytes = 8 * 2 * kOutStageBytes; // eight epilogue warps
 constexpr int kTc2SmemBytes = kStages2 * kStageBytes2 + kOutStagingBytes + 1024 + kBarrierBytes;
 constexpr uint32_t kInstrDesc2 = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)((2 * kBM) >> 4) << 24);
 
-__device__ __forceinline__ uint32_t cluster_cta_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// shared::cluster address of `addr` (a shared::cta address of this CTA) in the CTA of rank `rank`
-__device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
-    uint32_t out;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
-    return out;
-}
-// Arrive on a barrier of either CTA of the pair.  The arrival only hands a resource back (an accumulator that has been
-// read); nothing written by this thread is published through it, so the default CTA-scope release is enough -- a
-// cluster-scope release made every epilogue warp wait ~1000 cycles per tile for its earlier writes to drain.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// TMA load issued by one CTA of a pair; the completion bytes go to `bar`, a shared::cluster barrier address
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, int32_t c0, int32_t c1, int32_t c2, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t slot, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
 __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -444,45 +319,16 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// the same for fp16 operands with an fp32 accumulator (k = 16 per instruction)
-__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 // Instruction descriptor of kind::f16: fp32 accumulator (bits 4-5 = 1), fp16 A and B (bits 7-9 = 0, 10-12 = 0).
 constexpr uint32_t kInstrDescF16 = (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)((2 * kBM) >> 4) << 24);
 constexpr int kBKf16 = kBK / 2;                        // fp16 elements of k per stage (one 128-byte swizzle row)
 constexpr int kMnBlockF16 = 64 * kBKf16 * 2;           // an MN-major fp16 tile is two blocks of 64 rows x kBKf16 k-rows: 8 KiB each
-
-// arrives on the barrier at offset `bar` in every CTA of `cta_mask` once the MMAs issued so far have completed
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint16_t cta_mask) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"(cta_mask) : "memory");
-}
 
 // Up to eight destinations of the output (this GPU's buffer and, when the output is scattered, its peers').
 constexpr int kMaxDst = 8;
 struct OutMaps {
     CUtensorMap m[kMaxDst];
 };
-
-// TMA store of a staged 32-row x 128-byte tile (128-byte swizzle) to the 3-d output map; out-of-range rows and
-// columns are clipped by the hardware.
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int32_t c0, int32_t c1, int32_t c2) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
 
 // The dequantisation scales one epilogue warp needs for one tile, held in registers: the scale of the lane's output
 // row, and the 128 column scales of the warp's half of the tile spread over the lanes (lane l holds columns
