@@ -31,16 +31,18 @@ constexpr int kPieceBytes = 32 * 128;                  // a warp's staging tile:
 constexpr int kPieces = 2;                             // staging tiles per warp
 constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kPieces * kPieceBytes + 1024 + 256;
 constexpr int kTmemColumns = 512;
-constexpr int kBandRows = 8;                           // row tiles walked together (below)
+constexpr int kBandRows = 16;                          // row tiles walked together (below)
 
 constexpr uint32_t kErrLoad = 0x201, kErrFull = 0x202, kErrAccumulator = 0x203, kErrEpilogue = 0x204;
 
+// p, q: boxes of 128 rows by 64 k where one load can have them; q64: boxes of 64 rows (half tiles).  One load per operand and stage: with
+// two of 64 rows each the gated product took 489 us instead of 459 (4096 x 4096 x 20480).
 struct TcMaps {
-    CUtensorMap p[2], q[2], out[3];
+    CUtensorMap p[2], q[2], q64[2], out[3];
 };
 
-// Tiles are walked in bands of kBandRows row tiles, row by row within a column of the band: the tiles that run at one time then form
-// a block of about 8 x 9, which reads the fewest distinct operand rows.  The tiles left over by whole waves of the pairs are
+// Tiles are walked in bands of kBandRows row tiles, row by row within a column of the band: the band's rows of P stay in L2 while the
+// columns pass by (4096 tokens, gated: bands of 4, 8, 16 rows took 476, 459, 447 us).  The tiles left over by whole waves of the pairs are
 // split into halves of 128 accumulator columns when that makes the last wave shorter (2 x left-over <= pairs).
 struct TcParams {
     int32_t C;                         // row pitch of g and u (kEpiDact)
@@ -48,6 +50,7 @@ struct TcParams {
     int32_t blocks0, blocks;           // k blocks of the first pair of operands, of all
     int32_t tiles_r, tiles_c, per_product;
     int32_t whole, items;              // whole tiles, work items: items - whole halves follow
+    int32_t p_boxes, q_boxes;          // loads per 128 rows of P and Q: 1, or 2 for a transposed operand whose rows are no multiple of 64
     const void *g, *u;
     uint32_t *status;
 };
@@ -238,6 +241,18 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
     }
 }
 
+// Loads the rows of one operand from `row`, k from `k`.  A transposed operand whose rows are a multiple of 64 is mapped as
+// (64 rows, k, blocks of 64 rows), so that a box holds several blocks; others as (rows, k), one block per box (`two`: two boxes).
+template <bool MN>
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, int row, int k, bool two, bool plain, uint32_t bar) {
+    if (!MN) tma_load_3d_pair(dst, map, k, row, 0, bar);
+    else if (!two && !plain) tma_load_3d_pair(dst, map, 0, k, row / 64, bar);
+    else {
+        tma_load_3d_pair(dst, map, row, k, 0, bar);
+        if (two) tma_load_3d_pair(dst + kBlockBytes, map, row + 64, k, 0, bar);
+    }
+}
+
 // P_MN / Q_MN: the operand is stored (k, rows) instead of (rows, k).
 template <bool BF16, bool P_MN, bool Q_MN, int EPI, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -291,19 +306,13 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
                     const bool second = kb >= prm.blocks0;
                     const int k = (second ? kb - prm.blocks0 : kb) * kStageK;
                     const CUtensorMap *pm = &maps.p[second ? 1 : it.product];
-                    const CUtensorMap *qm = &maps.q[EPI == kEpiGated ? (int)rank : second ? 1 : it.product];
+                    const int which = EPI == kEpiGated ? (int)rank : second ? 1 : it.product;
+                    const CUtensorMap *qm = it.half || (Q_MN && prm.q_boxes == 2) ? &maps.q64[which] : &maps.q[which];
                     const uint32_t dst = tiles_base + stage * kStageBytes, q_dst = dst + kPBytes;
                     if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * (kPBytes + (uint32_t)(q_rows / 64) * kBlockBytes));
                     const uint32_t bar = map_to_cta(full_bar + 8 * stage, 0);
-                    if (P_MN) {
-                        tma_load_3d_pair(dst, pm, p_row, k, 0, bar);
-                        tma_load_3d_pair(dst + kBlockBytes, pm, p_row + 64, k, 0, bar);
-                    } else {
-                        tma_load_3d_pair(dst, pm, k, p_row, 0, bar);
-                        tma_load_3d_pair(dst + kBlockBytes, pm, k, p_row + 64, 0, bar);
-                    }
-                    for (int b = 0; b < q_rows; b += 64)
-                        tma_load_3d_pair(q_dst + (uint32_t)(b / 64) * kBlockBytes, qm, Q_MN ? q_row + b : k, Q_MN ? k : q_row + b, 0, bar);
+                    load_rows<P_MN>(dst, pm, p_row, k, P_MN && prm.p_boxes == 2, false, bar);
+                    load_rows<Q_MN>(q_dst, qm, q_row, k, Q_MN && prm.q_boxes == 2 && !it.half, Q_MN && prm.q_boxes == 2, bar);
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -379,12 +388,23 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
-// An operand of 16-bit elements stored (rows, k), or (k, rows) when transposed: boxes of 64 rows by 64 k.
-bool encode_operand(CUtensorMap *map, const void *ptr, int64_t rows, int64_t k, bool transposed) {
+// An operand of 16-bit elements stored (rows, k), or (k, rows) when transposed: boxes of `box_rows` (64 or 128) rows by 64 k.  A transposed
+// operand has 64 rows in a 128-byte swizzle row; as (64 rows, k, blocks of 64 rows) a box can hold two blocks, when there is no partial
+// block (it would reach past the tensor's end); otherwise boxes are 64 rows.
+bool encode_operand(CUtensorMap *map, const void *ptr, int64_t rows, int64_t k, bool transposed, uint32_t box_rows) {
+    if (transposed && rows % 64 == 0) {
+        const uint64_t dims[3] = {64, (uint64_t)k, (uint64_t)(rows / 64)}, strides[2] = {(uint64_t)rows * 2, 128};
+        const uint32_t box[3] = {64, 64, box_rows / 64};
+        return encode_tiled_3d(map, 2, ptr, dims, strides, box, true);
+    }
     const uint64_t inner = (uint64_t)(transposed ? rows : k), outer = (uint64_t)(transposed ? k : rows);
     const uint64_t dims[3] = {inner, outer, 1}, strides[2] = {inner * 2, inner * outer * 2};
-    const uint32_t box[3] = {64, 64, 1};
+    const uint32_t box[3] = {64, transposed ? 64 : box_rows, 1};
     return encode_tiled_3d(map, 2, ptr, dims, strides, box, true);
+}
+int32_t boxes(int64_t rows, bool transposed) { return transposed && rows % 64 ? 2 : 1; }
+bool encode_q(TcMaps *maps, int i, const void *ptr, int64_t rows, int64_t k, bool transposed) {
+    return encode_operand(&maps->q[i], ptr, rows, k, transposed, 128) && encode_operand(&maps->q64[i], ptr, rows, k, transposed, 64);
 }
 // An output (R, C): boxes of 32 rows by 64 columns.
 bool encode_output(CUtensorMap *map, void *ptr, int64_t R, int64_t C) {
@@ -440,8 +460,10 @@ int32_t tc_product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, 
     if (rc) return rc;
     TcMaps maps;
     memset(&maps, 0, sizeof(maps));
-    bool ok = encode_operand(&maps.p[0], p0, R, K, p_t) && encode_operand(&maps.q[0], q0, C, K, q_t) && encode_output(&maps.out[0], out0, R, C);
-    if (ok && p1) ok = encode_operand(&maps.p[1], p1, R, K, p_t) && encode_operand(&maps.q[1], q1, C, K, q_t);
+    bool ok = encode_operand(&maps.p[0], p0, R, K, p_t, 128) && encode_q(&maps, 0, q0, C, K, q_t) && encode_output(&maps.out[0], out0, R, C);
+    if (ok && p1) ok = encode_operand(&maps.p[1], p1, R, K, p_t, 128) && encode_q(&maps, 1, q1, C, K, q_t);
+    prm.p_boxes = boxes(R, p_t);
+    prm.q_boxes = boxes(C, q_t);
     if (ok && out1) ok = encode_output(&maps.out[1], out1, R, C);
     if (!ok) return encode_failed();
     const int64_t products = out1 ? 2 : 1;
@@ -458,8 +480,7 @@ int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const v
     if (rc) return rc;
     TcMaps maps;
     memset(&maps, 0, sizeof(maps));
-    bool ok = encode_operand(&maps.p[0], x, tokens, k, false) && encode_operand(&maps.q[0], wg, n, k, false) &&
-              encode_operand(&maps.q[1], wu, n, k, false) && encode_output(&maps.out[0], h, tokens, n);
+    bool ok = encode_operand(&maps.p[0], x, tokens, k, false, 128) && encode_q(&maps, 0, wg, n, k, false) && encode_q(&maps, 1, wu, n, k, false) && encode_output(&maps.out[0], h, tokens, n);
     if (ok && g) ok = encode_output(&maps.out[1], g, tokens, n) && encode_output(&maps.out[2], u, tokens, n);
     if (!ok) return encode_failed();
     prm.g = g;
@@ -476,9 +497,10 @@ int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const vo
     if (rc) return rc;
     TcMaps maps;
     memset(&maps, 0, sizeof(maps));
-    if (!(encode_operand(&maps.p[0], dy, tokens, m, false) && encode_operand(&maps.q[0], wd, n, m, true) && encode_output(&maps.out[0], dg, tokens, n) &&
+    if (!(encode_operand(&maps.p[0], dy, tokens, m, false, 128) && encode_q(&maps, 0, wd, n, m, true) && encode_output(&maps.out[0], dg, tokens, n) &&
           encode_output(&maps.out[1], du, tokens, n)))
         return encode_failed();
+    prm.q_boxes = boxes(n, true);
     prm.g = g;
     prm.u = u;
     const bool silu = call.act == CPMK_ACT_SILU;
