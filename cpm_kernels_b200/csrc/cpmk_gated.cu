@@ -144,9 +144,16 @@ int32_t product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, boo
     return launch_simt<kEpiStore>(call, prm);
 }
 
-int32_t gated_product(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u) {
-    if (tensor_core_size(k) && tensor_core_size(n) && aligned16(x) && aligned16(wg) && aligned16(wu) && aligned16(h) && aligned16(g) && aligned16(u))
-        return tc_gated(call, tokens, k, n, x, wg, wu, h, g, u);
+bool few_tokens(int32_t tokens) { return tokens <= kFewTokens; }
+
+bool gated_on_tensor_cores(int32_t k, int32_t n, const void *x, const void *wg, const void *wu, const void *h, const void *g, const void *u) {
+    return tensor_core_size(k) && tensor_core_size(n) && aligned16(x) && aligned16(wg) && aligned16(wu) && aligned16(h) && aligned16(g) && aligned16(u);
+}
+
+int32_t gated_product(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u,
+                      void *scratch) {
+    if (gated_on_tensor_cores(k, n, x, wg, wu, h, g, u))
+        return few_tokens(tokens) ? few_gated(call, tokens, k, n, x, wg, wu, h, g, u, scratch) : tc_gated(call, tokens, k, n, x, wg, wu, h, g, u);
     SimtParams prm = {};
     prm.R = tokens; prm.C = n; prm.K = k;
     prm.p_rs = k; prm.p_ks = 1; prm.q_rs = k; prm.q_ks = 1;
@@ -231,7 +238,7 @@ int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int6
     const int32_t rc = current_device_info(&info);
     if (rc) return rc;
     CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 0 && bytes, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
-    *bytes = 0;
+    *bytes = tokens > 0 && few_tokens(tokens) && tensor_core_size(k) && tensor_core_size(n) ? few_scratch(info, tokens, k, n, tensor_core_size(m) ? m : 0) : 0;
     return CPMK_OK;
 }
 
@@ -245,8 +252,9 @@ int32_t cpmk_gated_linear_forward(int32_t tokens, int32_t k, int32_t n, int32_t 
     CPMK_REQUIRE((g == nullptr) == (u == nullptr), "g and u are wanted together or not at all");
     CPMK_REQUIRE(even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(h) && even_address(g) && even_address(u),
                  "tensors must be 2-byte aligned");
-    CPMK_REQUIRE(aligned16(scratch), "scratch must be 16-byte aligned");
-    return gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u);
+    CPMK_REQUIRE(aligned16(scratch) && (scratch || !few_tokens(tokens) || !tensor_core_size(k) || !tensor_core_size(n)),
+                 "scratch of cpmk_gated_scratch bytes, 16-byte aligned, is needed");
+    return gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u, scratch);
 }
 
 int32_t cpmk_gated_linear_backward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *dh, const void *x,
@@ -277,9 +285,12 @@ int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, in
     CPMK_REQUIRE(even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(w_down) && even_address(h) && even_address(g) &&
                      even_address(u) && even_address(y),
                  "tensors must be 2-byte aligned");
-    CPMK_REQUIRE(aligned16(scratch), "scratch must be 16-byte aligned");
-    rc = gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u);
+    CPMK_REQUIRE(aligned16(scratch) && (scratch || !few_tokens(tokens) || !tensor_core_size(k) || !tensor_core_size(n)),
+                 "scratch of cpmk_gated_scratch bytes, 16-byte aligned, is needed");
+    rc = gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u, scratch);
     if (rc) return rc;
+    if (few_tokens(tokens) && tensor_core_size(m) && gated_on_tensor_cores(k, n, x, w_gate, w_up, h, g, u) && aligned16(w_down) && aligned16(y))
+        return few_down(call, tokens, k, n, m, h, w_down, y, scratch);
     return product(call, tokens, m, n, false, false, h, w_down, nullptr, nullptr, false, y, nullptr);
 }
 

@@ -52,4 +52,12 @@ int32_t tc_product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, 
 int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u);
 int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg, void *du);
 
+// Products for few tokens (cpmk_gated_few.cu), the same requirements; few_down follows few_gated of the same call.  few_scratch: bytes
+// for both (m = 0: the first alone).
+constexpr int32_t kFewTokens = 128;
+int64_t few_scratch(const DeviceInfo &info, int32_t tokens, int32_t k, int32_t n, int32_t m);
+int32_t few_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u,
+                  void *scratch);
+int32_t few_down(const Call &call, int32_t tokens, int32_t k, int32_t n, int32_t m, const void *h, const void *wd, void *y, void *scratch);
+
 }  // namespace cpmk
