@@ -123,10 +123,10 @@ bool tensor_core_size(int32_t extent) { return extent % 8 == 0; }
 // out0 (R, C) = P0 Q0^T (+ P1 Q1^T when `sum`), or out0 = P0 Q0^T and out1 = P1 Q1^T when out1 is given.  p_t / q_t: the operand is stored
 // (K, rows) instead of (rows, K).  The tensor cores' loads and stores want 16-byte rows and addresses; everything else runs generic.
 int32_t product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1, const void *q1,
-                bool sum, void *out0, void *out1) {
+                bool sum, void *out0, void *out1, void *scratch) {
     if (tensor_core_size(p_t ? R : K) && tensor_core_size(q_t ? C : K) && tensor_core_size(C) && aligned16(p0) && aligned16(q0) && aligned16(p1) &&
         aligned16(q1) && aligned16(out0) && aligned16(out1))
-        return tc_product(call, R, C, K, p_t, q_t, p0, q0, p1, q1, sum, out0, out1);
+        return tc_product(call, R, C, K, p_t, q_t, p0, q0, p1, q1, sum, out0, out1, scratch);
     SimtParams prm = {};
     prm.R = R; prm.C = C; prm.K = K;
     prm.p_rs = p_t ? 1 : K; prm.p_ks = p_t ? R : 1;
@@ -153,7 +153,7 @@ bool gated_on_tensor_cores(int32_t k, int32_t n, const void *x, const void *wg, 
 int32_t gated_product(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u,
                       void *scratch) {
     if (gated_on_tensor_cores(k, n, x, wg, wu, h, g, u))
-        return few_tokens(tokens) ? few_gated(call, tokens, k, n, x, wg, wu, h, g, u, scratch) : tc_gated(call, tokens, k, n, x, wg, wu, h, g, u);
+        return few_tokens(tokens) ? few_gated(call, tokens, k, n, x, wg, wu, h, g, u, scratch) : tc_gated(call, tokens, k, n, x, wg, wu, h, g, u, scratch);
     SimtParams prm = {};
     prm.R = tokens; prm.C = n; prm.K = k;
     prm.p_rs = k; prm.p_ks = 1; prm.q_rs = k; prm.q_ks = 1;
@@ -164,9 +164,9 @@ int32_t gated_product(const Call &call, int32_t tokens, int32_t k, int32_t n, co
 
 // dg, du from dh = dy Wd, which is not stored; Wd is (m, n)
 int32_t dact_product(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg,
-                     void *du) {
+                     void *du, void *scratch) {
     if (tensor_core_size(n) && tensor_core_size(m) && aligned16(dy) && aligned16(wd) && aligned16(g) && aligned16(u) && aligned16(dg) && aligned16(du))
-        return tc_dact(call, tokens, n, m, dy, wd, g, u, dg, du);
+        return tc_dact(call, tokens, n, m, dy, wd, g, u, dg, du, scratch);
     SimtParams prm = {};
     prm.R = tokens; prm.C = n; prm.K = m;
     prm.p_rs = m; prm.p_ks = 1; prm.q_rs = 1; prm.q_ks = n;
@@ -210,12 +210,12 @@ int32_t begin(Call *call, int32_t tokens, int32_t k, int32_t n, int32_t m, int32
 
 // dx, dWg, dWu from dg, du
 int32_t projections_backward(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, const void *dg,
-                             const void *du, void *dx, void *dwg, void *dwu) {
+                             const void *du, void *dx, void *dwg, void *dwu, void *scratch) {
     int32_t rc = CPMK_OK;
-    if (dx) rc = product(call, tokens, k, n, false, true, dg, wg, du, wu, true, dx, nullptr);
+    if (dx) rc = product(call, tokens, k, n, false, true, dg, wg, du, wu, true, dx, nullptr, scratch);
     if (rc || (!dwg && !dwu)) return rc;
-    if (dwg && dwu) return product(call, n, k, tokens, true, true, dg, x, du, x, false, dwg, dwu);
-    return product(call, n, k, tokens, true, true, dwg ? dg : du, x, nullptr, nullptr, false, dwg ? dwg : dwu, nullptr);
+    if (dwg && dwu) return product(call, n, k, tokens, true, true, dg, x, du, x, false, dwg, dwu, scratch);
+    return product(call, n, k, tokens, true, true, dwg ? dg : du, x, nullptr, nullptr, false, dwg ? dwg : dwu, nullptr, scratch);
 }
 
 // without tokens the weights' gradients are zero
@@ -225,6 +225,17 @@ int32_t clear_gradients(const Call &call, void *dwg, void *dwu, void *dwd, int64
     if (dwd) CPMK_CUDA_TRY(cudaMemsetAsync(dwd, 0, (size_t)mn * 2, call.stream));
     return CPMK_OK;
 }
+
+// scratch is there where the sizes ask for it, and aligned
+int32_t check_scratch(const void *scratch, int32_t (*bytes_of)(int32_t, int32_t, int32_t, int32_t, int64_t *), int32_t tokens, int32_t k, int32_t n, int32_t m) {
+    int64_t bytes = 0;
+    const int32_t rc = bytes_of(tokens, k, n, m, &bytes);
+    if (rc) return rc;
+    CPMK_REQUIRE(aligned16(scratch) && (scratch || !bytes), "scratch of %lld bytes, 16-byte aligned, is needed", (long long)bytes);
+    return CPMK_OK;
+}
+
+int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }
 
 }  // namespace
 }  // namespace cpmk
@@ -238,28 +249,53 @@ int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int6
     const int32_t rc = current_device_info(&info);
     if (rc) return rc;
     CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 0 && bytes, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
-    *bytes = tokens > 0 && few_tokens(tokens) && tensor_core_size(k) && tensor_core_size(n) ? few_scratch(info, tokens, k, n, tensor_core_size(m) ? m : 0) : 0;
+    int64_t need = 0;
+    if (tokens > 0 && tensor_core_size(n)) {
+        const bool down = m > 0 && tensor_core_size(m), first = tensor_core_size(k);
+        // pointers are not known here: room for the few-token pair of products, and for those of the tiles
+        if (few_tokens(tokens) && first) need = few_scratch(info, tokens, k, n, down ? m : 0);
+        if (!few_tokens(tokens) && first) need = tc_gated_scratch(info, tokens, k, n);
+        if (down) need = larger(need, tc_product_scratch(info, tokens, m, n, false, 1));
+    }
+    *bytes = need;
+    return CPMK_OK;
+}
+
+int32_t cpmk_gated_backward_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int64_t *bytes) {
+    DeviceInfo info;
+    const int32_t rc = current_device_info(&info);
+    if (rc) return rc;
+    CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 0 && bytes, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
+    int64_t need = 0;
+    if (tokens > 0 && tensor_core_size(n)) {
+        if (tensor_core_size(k)) {
+            need = larger(need, tc_product_scratch(info, tokens, k, n, true, 1));
+            need = larger(need, larger(tc_product_scratch(info, n, k, tokens, false, 1), tc_product_scratch(info, n, k, tokens, false, 2)));
+        }
+        if (m > 0 && tensor_core_size(m)) need = larger(need, larger(tc_dact_scratch(info, tokens, n, m), tc_product_scratch(info, m, n, tokens, false, 1)));
+    }
+    *bytes = need;
     return CPMK_OK;
 }
 
 int32_t cpmk_gated_linear_forward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *x, const void *w_gate,
                                   const void *w_up, void *h, void *g, void *u, void *scratch, cpmk_stream_t stream) {
     Call call;
-    const int32_t rc = begin(&call, tokens, k, n, 1, dtype, activation, stream);
+    int32_t rc = begin(&call, tokens, k, n, 1, dtype, activation, stream);
     if (rc) return rc;
     if (tokens == 0) return CPMK_OK;
     CPMK_REQUIRE(x && w_gate && w_up && h, "null pointer");
     CPMK_REQUIRE((g == nullptr) == (u == nullptr), "g and u are wanted together or not at all");
     CPMK_REQUIRE(even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(h) && even_address(g) && even_address(u),
                  "tensors must be 2-byte aligned");
-    CPMK_REQUIRE(aligned16(scratch) && (scratch || !few_tokens(tokens) || !tensor_core_size(k) || !tensor_core_size(n)),
-                 "scratch of cpmk_gated_scratch bytes, 16-byte aligned, is needed");
+    rc = check_scratch(scratch, cpmk_gated_scratch, tokens, k, n, 0);
+    if (rc) return rc;
     return gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u, scratch);
 }
 
 int32_t cpmk_gated_linear_backward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *dh, const void *x,
                                    const void *w_gate, const void *w_up, const void *g, const void *u, void *dg, void *du, void *dx, void *dw_gate,
-                                   void *dw_up, cpmk_stream_t stream) {
+                                   void *dw_up, void *scratch, cpmk_stream_t stream) {
     Call call;
     int32_t rc = begin(&call, tokens, k, n, 1, dtype, activation, stream);
     if (rc) return rc;
@@ -268,9 +304,11 @@ int32_t cpmk_gated_linear_backward(int32_t tokens, int32_t k, int32_t n, int32_t
     CPMK_REQUIRE(even_address(dh) && even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(g) && even_address(u) &&
                      even_address(dg) && even_address(du) && even_address(dx) && even_address(dw_gate) && even_address(dw_up),
                  "tensors must be 2-byte aligned");
+    rc = check_scratch(scratch, cpmk_gated_backward_scratch, tokens, k, n, 0);
+    if (rc) return rc;
     rc = dact(call, (int64_t)tokens * n, dh, g, u, dg, du);
     if (rc) return rc;
-    return projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up);
+    return projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up, scratch);
 }
 
 int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *x,
@@ -285,18 +323,19 @@ int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, in
     CPMK_REQUIRE(even_address(x) && even_address(w_gate) && even_address(w_up) && even_address(w_down) && even_address(h) && even_address(g) &&
                      even_address(u) && even_address(y),
                  "tensors must be 2-byte aligned");
-    CPMK_REQUIRE(aligned16(scratch) && (scratch || !few_tokens(tokens) || !tensor_core_size(k) || !tensor_core_size(n)),
-                 "scratch of cpmk_gated_scratch bytes, 16-byte aligned, is needed");
+    rc = check_scratch(scratch, cpmk_gated_scratch, tokens, k, n, m);
+    if (rc) return rc;
     rc = gated_product(call, tokens, k, n, x, w_gate, w_up, h, g, u, scratch);
     if (rc) return rc;
     if (few_tokens(tokens) && tensor_core_size(m) && gated_on_tensor_cores(k, n, x, w_gate, w_up, h, g, u) && aligned16(w_down) && aligned16(y))
         return few_down(call, tokens, k, n, m, h, w_down, y, scratch);
-    return product(call, tokens, m, n, false, false, h, w_down, nullptr, nullptr, false, y, nullptr);
+    return product(call, tokens, m, n, false, false, h, w_down, nullptr, nullptr, false, y, nullptr, scratch);
 }
 
 int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *dy,
                                          const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *g, const void *u,
-                                         const void *h, void *dg, void *du, void *dx, void *dw_gate, void *dw_up, void *dw_down, cpmk_stream_t stream) {
+                                         const void *h, void *dg, void *du, void *dx, void *dw_gate, void *dw_up, void *dw_down, void *scratch,
+                                         cpmk_stream_t stream) {
     Call call;
     int32_t rc = begin(&call, tokens, k, n, m, dtype, activation, stream);
     if (rc) return rc;
@@ -306,13 +345,15 @@ int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, i
                      even_address(u) && even_address(h) && even_address(dg) && even_address(du) && even_address(dx) && even_address(dw_gate) &&
                      even_address(dw_up) && even_address(dw_down),
                  "tensors must be 2-byte aligned");
+    rc = check_scratch(scratch, cpmk_gated_backward_scratch, tokens, k, n, m);
+    if (rc) return rc;
     if (dx || dw_gate || dw_up) {
-        rc = dact_product(call, tokens, n, m, dy, w_down, g, u, dg, du);
+        rc = dact_product(call, tokens, n, m, dy, w_down, g, u, dg, du, scratch);
         if (rc) return rc;
-        rc = projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up);
+        rc = projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up, scratch);
         if (rc) return rc;
     }
-    if (dw_down) return product(call, m, n, tokens, true, true, dy, h, nullptr, nullptr, false, dw_down, nullptr);
+    if (dw_down) return product(call, m, n, tokens, true, true, dy, h, nullptr, nullptr, false, dw_down, nullptr, scratch);
     return CPMK_OK;
 }
 

@@ -35,46 +35,86 @@ constexpr int kBandRows = 16;                          // row tiles walked toget
 
 constexpr uint32_t kErrLoad = 0x201, kErrFull = 0x202, kErrAccumulator = 0x203, kErrEpilogue = 0x204;
 
-// p, q: boxes of 128 rows by 64 k where one load can have them; q64: boxes of 64 rows (half tiles).  One load per operand and stage: with
-// two of 64 rows each the gated product took 489 us instead of 459 (4096 x 4096 x 20480).
+// Boxes of 128 rows by 64 k where one load can have them: with two boxes of 64 rows each the gated product took 489 us instead of 459
+// (4096 x 4096 x 20480).
 struct TcMaps {
-    CUtensorMap p[2], q[2], q64[2], out[3];
+    CUtensorMap p[2], q[2], out[3];
 };
 
-// Tiles are walked in bands of kBandRows row tiles, row by row within a column of the band: the band's rows of P stay in L2 while the
-// columns pass by (4096 tokens, gated: bands of 4, 8, 16 rows took 476, 459, 447 us).  The tiles left over by whole waves of the pairs are
-// split into halves of 128 accumulator columns when that makes the last wave shorter (2 x left-over <= pairs).
+// Whole waves of tiles are walked in bands of kBandRows row tiles, row by row within a column of the band: the band's rows of P stay in
+// L2 while the columns pass by (4096 tokens, gated: bands of 4, 8, 16 rows took 476, 459, 447 us).  The tiles that are left over (all
+// of them, when there are fewer tiles than pairs) would occupy a part of the SMs for the time of a whole tile.  Where that costs more
+// than it takes to join sums (split_pays), their k blocks form one list that is cut into equal pieces, one per pair; a piece leaves
+// fp32 partial sums in scratch, tc_join_kernel adds a tile's pieces in order of k and finishes its outputs.
 struct TcParams {
-    int32_t C;                         // row pitch of g and u (kEpiDact)
-    int32_t R;
+    int32_t R, C;
     int32_t blocks0, blocks;           // k blocks of the first pair of operands, of all
     int32_t tiles_r, tiles_c, per_product;
-    int32_t whole, items;              // whole tiles, work items: items - whole halves follow
+    int32_t whole;                     // tiles done whole; the others are split
+    int32_t split_tiles, split_pairs;  // how many are split, over how many pairs
     int32_t p_boxes, q_boxes;          // loads per 128 rows of P and Q: 1, or 2 for a transposed operand whose rows are no multiple of 64
-    const void *g, *u;
+    const void *g, *u;                 // kEpiDact: read;  kEpiGated: not null when they are wanted
+    float *partial;                    // [split tile + pair][accumulator column][row of the tile]
     uint32_t *status;
 };
 
 struct Item {
     int32_t product, row, col;         // first row; first column of the outputs
-    bool half;
+    int32_t block, count;              // k blocks
+    int32_t slot;                      // where the partial sums go, -1 for a whole tile
 };
 
 template <int EPI>
-__device__ __forceinline__ Item item_of(const TcParams &prm, int i) {
-    Item it;
-    it.half = i >= prm.whole;
-    int tile = it.half ? prm.whole + ((i - prm.whole) >> 1) : i;
+__device__ __forceinline__ void place(const TcParams &prm, int tile, Item &it) {
     it.product = tile / prm.per_product;
     tile -= it.product * prm.per_product;
     const int band = tile / (kBandRows * prm.tiles_c), in_band = tile - band * kBandRows * prm.tiles_c;
     const int rows = min(kBandRows, prm.tiles_r - band * kBandRows);
     const int c = in_band / rows;
     it.row = (band * kBandRows + in_band - c * rows) * kTileR;
-    constexpr int kWidth = EPI == kEpiGated ? kTileC / 2 : kTileC;
-    it.col = c * kWidth + (it.half && ((i - prm.whole) & 1) ? kWidth / 2 : 0);
-    return it;
+    it.col = c * (EPI == kEpiGated ? kTileC / 2 : kTileC);
 }
+
+// Pair p of P owns the units [p units / P, (p + 1) units / P) of the split tiles' k blocks.
+__device__ __forceinline__ int first_unit(const TcParams &prm, int pair) {
+    return (int)((int64_t)pair * prm.split_tiles * prm.blocks / prm.split_pairs);
+}
+__device__ __forceinline__ int owner_of(const TcParams &prm, int unit) {
+    return (int)((((int64_t)unit + 1) * prm.split_pairs - 1) / ((int64_t)prm.split_tiles * prm.blocks));
+}
+
+// A pair's work, in the order in which all its roles go through it.
+template <int EPI>
+struct Walk {
+    const TcParams &prm;
+    int tile, pairs, unit, end, slot;
+    __device__ __forceinline__ Walk(const TcParams &p, int pair, int n) : prm(p), tile(pair), pairs(n) {
+        unit = end = slot = 0;
+        if (pair < prm.split_pairs) {
+            unit = first_unit(prm, pair);
+            end = first_unit(prm, pair + 1);
+            slot = pair + unit / prm.blocks;
+        }
+    }
+    __device__ __forceinline__ bool next(Item &it) {
+        if (tile < prm.whole) {
+            place<EPI>(prm, tile, it);
+            tile += pairs;
+            it.block = 0;
+            it.count = prm.blocks;
+            it.slot = -1;
+            return true;
+        }
+        if (unit >= end) return false;
+        const int t = unit / prm.blocks;
+        place<EPI>(prm, prm.whole + t, it);
+        it.block = unit - t * prm.blocks;
+        it.count = min(end - unit, prm.blocks - it.block);
+        it.slot = slot++;
+        unit += it.count;
+        return true;
+    }
+};
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -88,6 +128,17 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
     if (BF16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v));
     return __half22float2(*reinterpret_cast<__half2 *>(&v));
+}
+
+// dg = dh u act'(g), du = dh act(g) for two neighbouring outputs
+template <bool BF16, int ACT>
+__device__ __forceinline__ void dact_pair(float d0, float d1, uint32_t g, uint32_t u, uint32_t &dg, uint32_t &du) {
+    const float2 g2 = unpack2<BF16>(g), u2 = unpack2<BF16>(u);
+    float a0, s0, a1, s1;
+    act_value_slope<ACT>(g2.x, a0, s0);
+    act_value_slope<ACT>(g2.y, a1, s1);
+    dg = pack2<BF16>(d0 * u2.x * s0, d1 * u2.y * s1);
+    du = pack2<BF16>(d0 * a0, d1 * a1);
 }
 
 // One warp's staging tiles: 32 rows by 64 columns each, 16-byte chunk j of row r at chunk j ^ (r & 7) (no bank conflicts, and what the
@@ -133,26 +184,23 @@ __device__ __forceinline__ void stage_sums(const Staging &st, int piece, uint32_
 template <bool BF16, int EPI, int ACT>
 __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps, const Staging &st, uint32_t tmem, const Item &it, int row, int half) {
     const int lane = (int)st.lane;
-    if (EPI == kEpiStore) {
-        // 128 columns per warp, 64 in a half tile
-        const int columns = it.half ? 64 : 128;
-        const int col = it.col + half * columns;
+    if (EPI == kEpiStore) {                              // 128 columns per warp
+        const int col = it.col + half * 128;
         if (col >= prm.C) return;
         st.acquire();
-        stage_sums<BF16>(st, 0, tmem + half * columns);
-        const bool second = !it.half && col + 64 < prm.C;
-        if (second) stage_sums<BF16>(st, 1, tmem + half * columns + 64);
+        stage_sums<BF16>(st, 0, tmem + half * 128);
+        const bool second = col + 64 < prm.C;
+        if (second) stage_sums<BF16>(st, 1, tmem + half * 128 + 64);
         st.ready();
         if (lane == 0) {
             st.store(0, &maps.out[it.product], col, row);
             if (second) st.store(1, &maps.out[it.product], col + 64, row);
             bulk_commit();
         }
-    } else if (EPI == kEpiGated) {
-        // whole tile: 64 output columns per warp; half tile: 64 in all, for the first half's warps
-        const int up = it.half ? 64 : 128;
+    } else if (EPI == kEpiGated) {                       // 64 output columns per warp: gate sums, and 128 columns on the up sums
+        constexpr int up = 128;
         const int col = it.col + half * 64;
-        if (col >= prm.C || (it.half && half)) return;
+        if (col >= prm.C) return;
         const uint32_t gate_at = tmem + half * 64;
         st.acquire();
 #pragma unroll
@@ -190,9 +238,8 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
             }
         }
     } else {
-        const int pieces = it.half ? 1 : 2;
-        for (int p = 0; p < pieces; ++p) {
-            const int offset = half * 64 * pieces + p * 64;
+        for (int p = 0; p < 2; ++p) {
+            const int offset = half * 128 + p * 64;
             const int col = it.col + offset;
             if (col >= prm.C) return;
             const int64_t at = (int64_t)(row + lane) * prm.C + col;
@@ -219,13 +266,7 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
                     uint32_t dg[4], du[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float2 g2 = unpack2<BF16>(gw[e]), u2 = unpack2<BF16>(uw[e]);
-                        const float d0 = __uint_as_float(v[8 * k + 2 * e]), d1 = __uint_as_float(v[8 * k + 2 * e + 1]);
-                        float a0, s0, a1, s1;
-                        act_value_slope<ACT>(g2.x, a0, s0);
-                        act_value_slope<ACT>(g2.y, a1, s1);
-                        dg[e] = pack2<BF16>(d0 * u2.x * s0, d1 * u2.y * s1);
-                        du[e] = pack2<BF16>(d0 * a0, d1 * a1);
+                        dact_pair<BF16, ACT>(__uint_as_float(v[8 * k + 2 * e]), __uint_as_float(v[8 * k + 2 * e + 1]), gw[e], uw[e], dg[e], du[e]);
                     }
                     st.put(0, 4 * s + k, dg[0], dg[1], dg[2], dg[3]);
                     st.put(1, 4 * s + k, du[0], du[1], du[2], du[3]);
@@ -241,15 +282,27 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
     }
 }
 
-// Loads the rows of one operand from `row`, k from `k`.  A transposed operand whose rows are a multiple of 64 is mapped as
-// (64 rows, k, blocks of 64 rows), so that a box holds several blocks; others as (rows, k), one block per box (`two`: two boxes).
+// A warp's share of a piece's partial sums: its 32 rows, its 128 accumulator columns; a column's 32 rows are 128 bytes.
+__device__ __forceinline__ void store_partial(const TcParams &prm, uint32_t tmem, const Item &it, int tile_row, int half, int lane) {
+    float *to = prm.partial + ((int64_t)it.slot * kTileC + half * 128) * kTileR + tile_row + lane;
+    for (int s = 0; s < 4; ++s, to += 32 * kTileR) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + half * 128 + s * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) __stcg(to + c * kTileR, __uint_as_float(v[c]));
+    }
+}
+
+// Loads the 128 rows of one operand from `row`, k from `k`.  A transposed operand whose rows are a multiple of 64 is mapped as
+// (64 rows, k, blocks of 64 rows), so that a box holds two blocks; others as (rows, k), one block per box.
 template <bool MN>
-__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, int row, int k, bool two, bool plain, uint32_t bar) {
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, int row, int k, int boxes, uint32_t bar) {
     if (!MN) tma_load_3d_pair(dst, map, k, row, 0, bar);
-    else if (!two && !plain) tma_load_3d_pair(dst, map, 0, k, row / 64, bar);
+    else if (boxes == 1) tma_load_3d_pair(dst, map, 0, k, row / 64, bar);
     else {
         tma_load_3d_pair(dst, map, row, k, 0, bar);
-        if (two) tma_load_3d_pair(dst + kBlockBytes, map, row + 64, k, 0, bar);
+        tma_load_3d_pair(dst + kBlockBytes, map, row + 64, k, 0, bar);
     }
 }
 
@@ -270,6 +323,7 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
     const bool leader = rank == 0;
+    if (prm.split_pairs) launch_dependents();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
@@ -296,23 +350,21 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool alive = true;
-            for (int i = pair; alive && i < prm.items; i += pairs) {
-                const Item it = item_of<EPI>(prm, i);
-                const int p_row = it.row + (int)rank * 128, q_rows = it.half ? 64 : 128;
+            Walk<EPI> walk(prm, pair, pairs);
+            Item it;
+            while (alive && walk.next(it)) {
+                const int p_row = it.row + (int)rank * 128;
                 // gated: the same rows of the rank's weight; otherwise the rank's half of the tile's columns
-                const int q_row = EPI == kEpiGated ? it.col : it.col + (int)rank * q_rows;
-                for (int kb = 0; kb < prm.blocks; ++kb) {
+                const int q_row = EPI == kEpiGated ? it.col : it.col + (int)rank * 128;
+                for (int kb = it.block; kb < it.block + it.count; ++kb) {
                     if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, abort_flag, prm.status, kErrLoad)) { alive = false; break; }
                     const bool second = kb >= prm.blocks0;
                     const int k = (second ? kb - prm.blocks0 : kb) * kStageK;
-                    const CUtensorMap *pm = &maps.p[second ? 1 : it.product];
-                    const int which = EPI == kEpiGated ? (int)rank : second ? 1 : it.product;
-                    const CUtensorMap *qm = it.half || (Q_MN && prm.q_boxes == 2) ? &maps.q64[which] : &maps.q[which];
-                    const uint32_t dst = tiles_base + stage * kStageBytes, q_dst = dst + kPBytes;
-                    if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * (kPBytes + (uint32_t)(q_rows / 64) * kBlockBytes));
+                    const uint32_t dst = tiles_base + stage * kStageBytes;
+                    if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * kStageBytes);
                     const uint32_t bar = map_to_cta(full_bar + 8 * stage, 0);
-                    load_rows<P_MN>(dst, pm, p_row, k, P_MN && prm.p_boxes == 2, false, bar);
-                    load_rows<Q_MN>(q_dst, qm, q_row, k, Q_MN && prm.q_boxes == 2 && !it.half, Q_MN && prm.q_boxes == 2, bar);
+                    load_rows<P_MN>(dst, &maps.p[second ? 1 : it.product], p_row, k, prm.p_boxes, bar);
+                    load_rows<Q_MN>(dst + kPBytes, &maps.q[EPI == kEpiGated ? (int)rank : second ? 1 : it.product], q_row, k, prm.q_boxes, bar);
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -326,13 +378,14 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
             // N / 8 at bits 17-22, M / 16 at bits 24-28
             constexpr uint32_t kType = BF16 ? 1u : 0u;
             constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | (P_MN ? (1u << 15) : 0u) | (Q_MN ? (1u << 16) : 0u) |
-                                       ((uint32_t)(kTileR >> 4) << 24);
-            for (int i = pair; alive && i < prm.items; i += pairs) {
-                const uint32_t desc = kDesc | ((uint32_t)((i >= prm.whole ? 128 : 256) >> 3) << 17);
+                                       ((uint32_t)(kTileC >> 3) << 17) | ((uint32_t)(kTileR >> 4) << 24);
+            Walk<EPI> walk(prm, pair, pairs);
+            Item it;
+            while (alive && walk.next(it)) {
                 if (!mbar_wait(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_flag, prm.status, kErrAccumulator)) break;
                 tcgen05_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * kTileC;
-                for (int kb = 0; kb < prm.blocks; ++kb) {
+                for (int kb = 0; kb < it.count; ++kb) {
                     if (!mbar_wait(full_bar + 8 * stage, phase, abort_flag, prm.status, kErrFull)) { alive = false; break; }
                     tcgen05_fence_after();
                     const uint32_t src = tiles_base + stage * kStageBytes;
@@ -340,7 +393,7 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
                     const uint64_t qd = Q_MN ? make_mnmajor_sw128_desc(src + kPBytes, kBlockBytes) : make_kmajor_sw128_desc(src + kPBytes);
 #pragma unroll
                     for (int j = 0; j < kStageK / 16; ++j)                               // 16 of k: 32 bytes of a row, or 16 rows of 128 bytes
-                        umma_f16_pair(d_tmem, pd + (uint64_t)((P_MN ? 128 : 2) * j), qd + (uint64_t)((Q_MN ? 128 : 2) * j), desc, (kb | j) != 0 ? 1u : 0u);
+                        umma_f16_pair(d_tmem, pd + (uint64_t)((P_MN ? 128 : 2) * j), qd + (uint64_t)((Q_MN ? 128 : 2) * j), kDesc, (kb | j) != 0 ? 1u : 0u);
                     umma_commit_pair(empty_bar + 8 * stage, 3);
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -355,13 +408,17 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const Staging st = {staging_base + (uint32_t)(warp - 2) * kPieces * kPieceBytes, (uint32_t)lane};
         uint32_t acc = 0, acc_phase = 0;
-        for (int i = pair; i < prm.items; i += pairs) {
-            const Item it = item_of<EPI>(prm, i);
+        Walk<EPI> walk(prm, pair, pairs);
+        Item it;
+        while (walk.next(it)) {
             if (!mbar_wait(acc_full_bar + 8 * acc, acc_phase, abort_flag, prm.status, kErrEpilogue)) break;
             tcgen05_fence_after();
-            const int row = it.row + (int)rank * 128 + quarter * 32;
-            if (row < prm.R)
-                epilogue<BF16, EPI, ACT>(prm, maps, st, tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTileC, it, row, half);
+            const int tile_row = (int)rank * 128 + quarter * 32, row = it.row + tile_row;
+            const uint32_t tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTileC;
+            if (row < prm.R) {
+                if (it.slot >= 0) store_partial(prm, tmem, it, tile_row, half, lane);
+                else epilogue<BF16, EPI, ACT>(prm, maps, st, tmem, it, row, half);
+            }
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(acc_empty_bar + 8 * acc, 0));
@@ -385,27 +442,87 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
     }
 }
 
+// Finishes the split tiles.  A block has 32 rows by 64 outputs of a tile: a warp 32 rows of 8 neighbouring outputs, so that it reads 128
+// bytes per column and piece, and a thread writes 16 bytes.
+constexpr int kJoinColumns = 8, kJoinBlockColumns = 64;
+
+template <bool BF16, int EPI, int ACT>
+__global__ void __launch_bounds__(256) tc_join_kernel(const TcParams prm, void *out0, void *out1, void *out2) {
+    constexpr int kWidth = EPI == kEpiGated ? kTileC / 2 : kTileC, kAcross = kWidth / kJoinBlockColumns, kPerTile = kAcross * (kTileR / 32);
+    const int t = blockIdx.x / kPerTile, part = blockIdx.x - t * kPerTile;
+    Item it;
+    place<EPI>(prm, prm.whole + t, it);
+    const int tile_row = part / kAcross * 32 + (threadIdx.x & 31), tile_col = part % kAcross * kJoinBlockColumns + (threadIdx.x >> 5) * kJoinColumns;
+    const int row = it.row + tile_row, col = it.col + tile_col;
+    const int first = owner_of(prm, t * prm.blocks), last = owner_of(prm, (t + 1) * prm.blocks - 1);
+    wait_for_prior_grid();
+    if (row >= prm.R || col >= prm.C) return;
+    float a[kJoinColumns], b[EPI == kEpiGated ? kJoinColumns : 1];
+#pragma unroll
+    for (int c = 0; c < kJoinColumns; ++c) a[c] = b[EPI == kEpiGated ? c : 0] = 0.f;
+    const float *at = prm.partial + ((int64_t)(first + t) * kTileC + tile_col) * kTileR + tile_row;
+#pragma unroll 2
+    for (int p = first; p <= last; ++p, at += kTileC * kTileR) {
+#pragma unroll
+        for (int c = 0; c < kJoinColumns; ++c) {
+            a[c] += __ldcg(at + c * kTileR);
+            if (EPI == kEpiGated) b[EPI == kEpiGated ? c : 0] += __ldcg(at + (128 + c) * kTileR);
+        }
+    }
+    const int64_t to = (int64_t)row * prm.C + col;
+    uint32_t o[3][kJoinColumns / 2];
+    if (EPI == kEpiDact) {
+#pragma unroll
+        for (int k = 0; k < kJoinColumns / 8; ++k) {
+            if (col + 8 * k >= prm.C) break;
+            const uint4 g4 = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(prm.g) + to + 8 * k));
+            const uint4 u4 = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(prm.u) + to + 8 * k));
+            const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dact_pair<BF16, ACT>(a[8 * k + 2 * e], a[8 * k + 2 * e + 1], gw[e], uw[e], o[0][4 * k + e], o[1][4 * k + e]);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < kJoinColumns; c += 2) {
+            if (EPI == kEpiGated) {
+                constexpr int kOne = EPI == kEpiGated ? 1 : 0;
+                o[0][c / 2] = pack2<BF16>(act_value<ACT>(a[c]) * b[c * kOne], act_value<ACT>(a[c + 1]) * b[(c + 1) * kOne]);
+                o[1][c / 2] = pack2<BF16>(a[c], a[c + 1]);
+                o[2][c / 2] = pack2<BF16>(b[c * kOne], b[(c + 1) * kOne]);
+            } else {
+                o[0][c / 2] = pack2<BF16>(a[c], a[c + 1]);
+            }
+        }
+    }
+    void *out[3] = {EPI == kEpiStore && it.product ? out1 : out0, EPI == kEpiStore ? nullptr : out1, out2};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        if ((EPI == kEpiStore && k) || (EPI == kEpiDact && k == 2) || !out[k]) break;
+        uint4 *p = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out[k]) + to);
+#pragma unroll
+        for (int c = 0; c < kJoinColumns / 8; ++c)
+            if (col + 8 * c < prm.C) p[c] = make_uint4(o[k][4 * c], o[k][4 * c + 1], o[k][4 * c + 2], o[k][4 * c + 3]);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
-// An operand of 16-bit elements stored (rows, k), or (k, rows) when transposed: boxes of `box_rows` (64 or 128) rows by 64 k.  A transposed
-// operand has 64 rows in a 128-byte swizzle row; as (64 rows, k, blocks of 64 rows) a box can hold two blocks, when there is no partial
-// block (it would reach past the tensor's end); otherwise boxes are 64 rows.
-bool encode_operand(CUtensorMap *map, const void *ptr, int64_t rows, int64_t k, bool transposed, uint32_t box_rows) {
+// An operand of 16-bit elements stored (rows, k), or (k, rows) when transposed: boxes of 128 rows by 64 k.  A transposed operand has 64
+// rows in a 128-byte swizzle row; as (64 rows, k, blocks of 64 rows) a box can hold two blocks, when there is no partial block (it
+// would reach past the tensor's end); otherwise boxes are 64 rows.
+bool encode_operand(CUtensorMap *map, const void *ptr, int64_t rows, int64_t k, bool transposed) {
     if (transposed && rows % 64 == 0) {
         const uint64_t dims[3] = {64, (uint64_t)k, (uint64_t)(rows / 64)}, strides[2] = {(uint64_t)rows * 2, 128};
-        const uint32_t box[3] = {64, 64, box_rows / 64};
+        const uint32_t box[3] = {64, 64, 2};
         return encode_tiled_3d(map, 2, ptr, dims, strides, box, true);
     }
     const uint64_t inner = (uint64_t)(transposed ? rows : k), outer = (uint64_t)(transposed ? k : rows);
     const uint64_t dims[3] = {inner, outer, 1}, strides[2] = {inner * 2, inner * outer * 2};
-    const uint32_t box[3] = {64, transposed ? 64 : box_rows, 1};
+    const uint32_t box[3] = {64, transposed ? 64u : 128u, 1};
     return encode_tiled_3d(map, 2, ptr, dims, strides, box, true);
 }
 int32_t boxes(int64_t rows, bool transposed) { return transposed && rows % 64 ? 2 : 1; }
-bool encode_q(TcMaps *maps, int i, const void *ptr, int64_t rows, int64_t k, bool transposed) {
-    return encode_operand(&maps->q[i], ptr, rows, k, transposed, 128) && encode_operand(&maps->q64[i], ptr, rows, k, transposed, 64);
-}
 // An output (R, C): boxes of 32 rows by 64 columns.
 bool encode_output(CUtensorMap *map, void *ptr, int64_t R, int64_t C) {
     const uint64_t dims[3] = {(uint64_t)C, (uint64_t)R, 1}, strides[2] = {(uint64_t)C * 2, (uint64_t)R * (uint64_t)C * 2};
@@ -413,35 +530,61 @@ bool encode_output(CUtensorMap *map, void *ptr, int64_t R, int64_t C) {
     return encode_tiled_3d(map, 2, ptr, dims, strides, box, true);
 }
 
+struct Plan {
+    int64_t tiles_r, tiles_c, blocks0, blocks, whole, split_tiles, split_pairs, bytes;
+};
+// K1: the second pair's k when its product is added (0: none); width: outputs per tile along C.
+Plan plan_of(const DeviceInfo &info, int64_t R, int64_t C, int64_t K0, int64_t K1, int64_t width, int64_t products) {
+    Plan p;
+    p.tiles_r = ceil_div64(R, kTileR);
+    p.tiles_c = ceil_div64(C, width);
+    p.blocks0 = ceil_div64(K0, kStageK);
+    p.blocks = p.blocks0 + ceil_div64(K1, kStageK);
+    const int64_t pairs = info.sm_count / 2, total = p.tiles_r * p.tiles_c * products, left = total % pairs;
+    // at least eight k blocks per piece; a k block takes a pair 0.3 us, a piece's sums 1/12 us to write and read back, a join 3 us
+    const int64_t most = left * p.blocks / 8, split = most < pairs ? most : pairs;
+    const bool pays = left > 0 && split > left && 0.3 * p.blocks > 0.3 * left * p.blocks / split + (left + split) / 12.0 + 3.0;
+    p.whole = pays ? total - left : total;
+    p.split_tiles = pays ? left : 0;
+    p.split_pairs = pays ? split : 0;
+    p.bytes = pays ? (left + split) * kTileR * kTileC * (int64_t)sizeof(float) : 0;
+    return p;
+}
+
 template <bool BF16, bool P_MN, bool Q_MN, int EPI, int ACT>
-int32_t launch(const Call &call, const TcMaps &maps, TcParams prm, int64_t products) {
+int32_t launch(const Call &call, const TcMaps &maps, TcParams prm, const Plan &plan, void *out0, void *out1, void *out2) {
     auto kernel = gated_tc_kernel<BF16, P_MN, Q_MN, EPI, ACT>;
     CPMK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    CPMK_REQUIRE(plan.whole + plan.split_tiles < (int64_t(1) << 30) && plan.split_tiles * plan.blocks < (int64_t(1) << 30), "too many output tiles");
     const int64_t pairs = call.info.sm_count / 2;        // advisory: a pair that is not resident at launch starts when another retires
-    const int64_t per_product = (int64_t)prm.tiles_r * prm.tiles_c, total = per_product * products;
-    CPMK_REQUIRE(total < (int64_t(1) << 30), "too many output tiles");
-    const int64_t left = total % pairs;
-    const bool split = left > 0 && 2 * left <= pairs;
-    prm.per_product = (int32_t)per_product;
-    prm.whole = (int32_t)(split ? total - left : total);
-    prm.items = (int32_t)(split ? total + left : total);
-    const unsigned grid = (unsigned)(2 * (prm.items < pairs ? prm.items : pairs));
-    kernel<<<grid, kThreads, kSmemBytes, call.stream>>>(maps, prm);
+    const int64_t used = plan.whole < pairs ? (plan.whole > plan.split_pairs ? plan.whole : plan.split_pairs) : pairs;
+    kernel<<<(unsigned)(2 * used), kThreads, kSmemBytes, call.stream>>>(maps, prm);
     CPMK_LAUNCH_CHECK();
+    if (!plan.split_tiles) return CPMK_OK;
+    const int64_t parts = (EPI == kEpiGated ? kTileC / 2 : kTileC) / kJoinBlockColumns * (kTileR / 32);
+    CPMK_CUDA_TRY(launch_after_prior(tc_join_kernel<BF16, EPI, ACT>, dim3((unsigned)(plan.split_tiles * parts)), dim3(256), 0, call.stream, prm, out0, out1,
+                                     out2));
     return CPMK_OK;
 }
 
-int32_t prepare(TcParams *prm, int64_t R, int64_t C, int64_t K0, int64_t K1, int64_t width) {
+int32_t prepare(TcParams *prm, const Plan &plan, int64_t R, int64_t C, void *scratch) {
     uint32_t *status;
     const int32_t rc = get_device_status(&status);
     if (rc) return rc;
+    CPMK_REQUIRE(scratch || !plan.bytes, "scratch is needed");
     memset(prm, 0, sizeof(*prm));
     prm->R = (int32_t)R;
     prm->C = (int32_t)C;
-    prm->blocks0 = (int32_t)ceil_div64(K0, kStageK);
-    prm->blocks = prm->blocks0 + (int32_t)ceil_div64(K1, kStageK);
-    prm->tiles_r = (int32_t)ceil_div64(R, kTileR);
-    prm->tiles_c = (int32_t)ceil_div64(C, width);
+    prm->blocks0 = (int32_t)plan.blocks0;
+    prm->blocks = (int32_t)plan.blocks;
+    prm->tiles_r = (int32_t)plan.tiles_r;
+    prm->tiles_c = (int32_t)plan.tiles_c;
+    prm->per_product = (int32_t)(plan.tiles_r * plan.tiles_c);
+    prm->whole = (int32_t)plan.whole;
+    prm->split_tiles = (int32_t)plan.split_tiles;
+    prm->split_pairs = (int32_t)plan.split_pairs;
+    prm->p_boxes = prm->q_boxes = 1;
+    prm->partial = static_cast<float *>(scratch);
     prm->status = status;
     return CPMK_OK;
 }
@@ -453,60 +596,78 @@ int32_t encode_failed() {
 
 }  // namespace
 
+int64_t tc_product_scratch(const DeviceInfo &info, int32_t R, int32_t C, int32_t K, bool sum, int32_t products) {
+    return plan_of(info, R, C, K, sum ? K : 0, kTileC, products).bytes;
+}
+int64_t tc_gated_scratch(const DeviceInfo &info, int32_t tokens, int32_t k, int32_t n) { return plan_of(info, tokens, n, k, 0, kTileC / 2, 1).bytes; }
+int64_t tc_dact_scratch(const DeviceInfo &info, int32_t tokens, int32_t n, int32_t m) { return plan_of(info, tokens, n, m, 0, kTileC, 1).bytes; }
+
 int32_t tc_product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1,
-                   const void *q1, bool sum, void *out0, void *out1) {
+                   const void *q1, bool sum, void *out0, void *out1, void *scratch) {
+    const Plan plan = plan_of(call.info, R, C, K, sum ? K : 0, kTileC, out1 ? 2 : 1);
     TcParams prm;
-    const int32_t rc = prepare(&prm, R, C, K, sum ? K : 0, kTileC);
+    const int32_t rc = prepare(&prm, plan, R, C, scratch);
     if (rc) return rc;
-    TcMaps maps;
-    memset(&maps, 0, sizeof(maps));
-    bool ok = encode_operand(&maps.p[0], p0, R, K, p_t, 128) && encode_q(&maps, 0, q0, C, K, q_t) && encode_output(&maps.out[0], out0, R, C);
-    if (ok && p1) ok = encode_operand(&maps.p[1], p1, R, K, p_t, 128) && encode_q(&maps, 1, q1, C, K, q_t);
     prm.p_boxes = boxes(R, p_t);
     prm.q_boxes = boxes(C, q_t);
+    TcMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    bool ok = encode_operand(&maps.p[0], p0, R, K, p_t) && encode_operand(&maps.q[0], q0, C, K, q_t) && encode_output(&maps.out[0], out0, R, C);
+    if (ok && p1) ok = encode_operand(&maps.p[1], p1, R, K, p_t) && encode_operand(&maps.q[1], q1, C, K, q_t);
     if (ok && out1) ok = encode_output(&maps.out[1], out1, R, C);
     if (!ok) return encode_failed();
-    const int64_t products = out1 ? 2 : 1;
     const bool bf16 = call.dtype == CPMK_BF16;
-    if (!p_t && !q_t) return bf16 ? launch<true, false, false, kEpiStore, 0>(call, maps, prm, products) : launch<false, false, false, kEpiStore, 0>(call, maps, prm, products);
-    if (!p_t) return bf16 ? launch<true, false, true, kEpiStore, 0>(call, maps, prm, products) : launch<false, false, true, kEpiStore, 0>(call, maps, prm, products);
+#define CPMK_TC_STORE(P, Q) \
+    return bf16 ? launch<true, P, Q, kEpiStore, 0>(call, maps, prm, plan, out0, out1, nullptr) : launch<false, P, Q, kEpiStore, 0>(call, maps, prm, plan, out0, out1, nullptr)
+    if (!p_t && !q_t) CPMK_TC_STORE(false, false);
+    if (!p_t) CPMK_TC_STORE(false, true);
     CPMK_REQUIRE(q_t, "operand order not built");
-    return bf16 ? launch<true, true, true, kEpiStore, 0>(call, maps, prm, products) : launch<false, true, true, kEpiStore, 0>(call, maps, prm, products);
+    CPMK_TC_STORE(true, true);
+#undef CPMK_TC_STORE
 }
 
-int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u) {
+int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u,
+                 void *scratch) {
+    const Plan plan = plan_of(call.info, tokens, n, k, 0, kTileC / 2, 1);
     TcParams prm;
-    const int32_t rc = prepare(&prm, tokens, n, k, 0, kTileC / 2);
+    const int32_t rc = prepare(&prm, plan, tokens, n, scratch);
     if (rc) return rc;
-    TcMaps maps;
-    memset(&maps, 0, sizeof(maps));
-    bool ok = encode_operand(&maps.p[0], x, tokens, k, false, 128) && encode_q(&maps, 0, wg, n, k, false) && encode_q(&maps, 1, wu, n, k, false) && encode_output(&maps.out[0], h, tokens, n);
-    if (ok && g) ok = encode_output(&maps.out[1], g, tokens, n) && encode_output(&maps.out[2], u, tokens, n);
-    if (!ok) return encode_failed();
     prm.g = g;
     prm.u = u;
-    const bool silu = call.act == CPMK_ACT_SILU;
-    if (call.dtype == CPMK_BF16)
-        return silu ? launch<true, false, false, kEpiGated, CPMK_ACT_SILU>(call, maps, prm, 1) : launch<true, false, false, kEpiGated, CPMK_ACT_GELU>(call, maps, prm, 1);
-    return silu ? launch<false, false, false, kEpiGated, CPMK_ACT_SILU>(call, maps, prm, 1) : launch<false, false, false, kEpiGated, CPMK_ACT_GELU>(call, maps, prm, 1);
-}
-
-int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg, void *du) {
-    TcParams prm;
-    const int32_t rc = prepare(&prm, tokens, n, m, 0, kTileC);
-    if (rc) return rc;
     TcMaps maps;
     memset(&maps, 0, sizeof(maps));
-    if (!(encode_operand(&maps.p[0], dy, tokens, m, false, 128) && encode_q(&maps, 0, wd, n, m, true) && encode_output(&maps.out[0], dg, tokens, n) &&
-          encode_output(&maps.out[1], du, tokens, n)))
-        return encode_failed();
+    bool ok = encode_operand(&maps.p[0], x, tokens, k, false) && encode_operand(&maps.q[0], wg, n, k, false) &&
+              encode_operand(&maps.q[1], wu, n, k, false) && encode_output(&maps.out[0], h, tokens, n);
+    if (ok && g) ok = encode_output(&maps.out[1], g, tokens, n) && encode_output(&maps.out[2], u, tokens, n);
+    if (!ok) return encode_failed();
+#define CPMK_TC_GATED(BF16, ACT) return launch<BF16, false, false, kEpiGated, ACT>(call, maps, prm, plan, h, g, u)
+    if (call.dtype == CPMK_BF16 && call.act == CPMK_ACT_SILU) CPMK_TC_GATED(true, CPMK_ACT_SILU);
+    if (call.dtype == CPMK_BF16) CPMK_TC_GATED(true, CPMK_ACT_GELU);
+    if (call.act == CPMK_ACT_SILU) CPMK_TC_GATED(false, CPMK_ACT_SILU);
+    CPMK_TC_GATED(false, CPMK_ACT_GELU);
+#undef CPMK_TC_GATED
+}
+
+int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg, void *du,
+                void *scratch) {
+    const Plan plan = plan_of(call.info, tokens, n, m, 0, kTileC, 1);
+    TcParams prm;
+    const int32_t rc = prepare(&prm, plan, tokens, n, scratch);
+    if (rc) return rc;
     prm.q_boxes = boxes(n, true);
     prm.g = g;
     prm.u = u;
-    const bool silu = call.act == CPMK_ACT_SILU;
-    if (call.dtype == CPMK_BF16)
-        return silu ? launch<true, false, true, kEpiDact, CPMK_ACT_SILU>(call, maps, prm, 1) : launch<true, false, true, kEpiDact, CPMK_ACT_GELU>(call, maps, prm, 1);
-    return silu ? launch<false, false, true, kEpiDact, CPMK_ACT_SILU>(call, maps, prm, 1) : launch<false, false, true, kEpiDact, CPMK_ACT_GELU>(call, maps, prm, 1);
+    TcMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    if (!(encode_operand(&maps.p[0], dy, tokens, m, false) && encode_operand(&maps.q[0], wd, n, m, true) && encode_output(&maps.out[0], dg, tokens, n) &&
+          encode_output(&maps.out[1], du, tokens, n)))
+        return encode_failed();
+#define CPMK_TC_DACT(BF16, ACT) return launch<BF16, false, true, kEpiDact, ACT>(call, maps, prm, plan, dg, du, nullptr)
+    if (call.dtype == CPMK_BF16 && call.act == CPMK_ACT_SILU) CPMK_TC_DACT(true, CPMK_ACT_SILU);
+    if (call.dtype == CPMK_BF16) CPMK_TC_DACT(true, CPMK_ACT_GELU);
+    if (call.act == CPMK_ACT_SILU) CPMK_TC_DACT(false, CPMK_ACT_SILU);
+    CPMK_TC_DACT(false, CPMK_ACT_GELU);
+#undef CPMK_TC_DACT
 }
 
 }  // namespace cpmk

@@ -11,4 +11,4 @@ from .gemv import (gemv_fp16, gemv_fp16_light, gemv_fp16_transpose, gemv_fp16_tr
                    gemv_broadcast_mat_fp16, gemv_broadcast_mat_fp16_light, gemv_calc_scale, gemv_round,
                    gemv_broadcast_mat_int8)
 from .layernorm_rows import layernorm_rows_forward, layernorm_rows_backward, layernorm_rows_backward_scratch
-from .gated import (gated_linear_forward, gated_linear_backward, gated_feed_forward_forward, gated_feed_forward_backward, gated_scratch)
+from .gated import (gated_linear_forward, gated_linear_backward, gated_feed_forward_forward, gated_feed_forward_backward, gated_scratch, gated_backward_scratch)

@@ -13,6 +13,13 @@ def gated_scratch(tokens: int, k: int, n: int, m: int = 0) -> int:
     return out.value
 
 
+def gated_backward_scratch(tokens: int, k: int, n: int, m: int = 0) -> int:
+    """The same for the two backward launchers."""
+    out = ctypes.c_int64(0)
+    cpmk.call("cpmk_gated_backward_scratch", tokens, k, n, m, ctypes.byref(out))
+    return out.value
+
+
 def gated_linear_forward(tokens: int, k: int, n: int, dtype: int, activation: int,
                          x: DevicePointer,         # (tokens, k)
                          w_gate: DevicePointer,    # (n, k)
@@ -36,10 +43,11 @@ def gated_linear_backward(tokens: int, k: int, n: int, dtype: int, activation: i
                           dx: DevicePointer,        # (tokens, k), written, or 0
                           dw_gate: DevicePointer,   # (n, k), written, or 0
                           dw_up: DevicePointer,     # (n, k), written, or 0
+                          scratch: DevicePointer,   # gated_backward_scratch(tokens, k, n) bytes
                           stream: CUDAStream):
     assert tokens >= 0 and k >= 1 and n >= 1
     cpmk.call("cpmk_gated_linear_backward", tokens, k, n, dtype, activation, dh, x, w_gate, w_up, g, u, dg, du, dx or None, dw_gate or None,
-              dw_up or None, stream_arg(stream))
+              dw_up or None, scratch or None, stream_arg(stream))
 
 
 def gated_feed_forward_forward(tokens: int, k: int, n: int, m: int, dtype: int, activation: int,
@@ -64,7 +72,8 @@ def gated_feed_forward_backward(tokens: int, k: int, n: int, m: int, dtype: int,
                                 dg: DevicePointer, du: DevicePointer,    # (tokens, n), written when dx, dw_gate or dw_up is wanted
                                 dx: DevicePointer, dw_gate: DevicePointer, dw_up: DevicePointer,
                                 dw_down: DevicePointer,   # (m, n), written, or 0
+                                scratch: DevicePointer,   # gated_backward_scratch(tokens, k, n, m) bytes
                                 stream: CUDAStream):
     assert tokens >= 0 and k >= 1 and n >= 1 and m >= 1
     cpmk.call("cpmk_gated_feed_forward_backward", tokens, k, n, m, dtype, activation, dy, x, w_gate, w_up, w_down, g, u, h or None, dg, du, dx or None,
-              dw_gate or None, dw_up or None, dw_down or None, stream_arg(stream))
+              dw_gate or None, dw_up or None, dw_down or None, scratch or None, stream_arg(stream))

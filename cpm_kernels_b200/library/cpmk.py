@@ -67,10 +67,11 @@ SIGNATURES = {
     "cpmk_layernorm_rows_backward_scratch": [_i, _i, POINTER(ctypes.c_int64)],
     "cpmk_layernorm_rows_backward": [_i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p],
     "cpmk_gated_scratch": [_i, _i, _i, _i, POINTER(ctypes.c_int64)],
+    "cpmk_gated_backward_scratch": [_i, _i, _i, _i, POINTER(ctypes.c_int64)],
     "cpmk_gated_linear_forward": [_i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p],
-    "cpmk_gated_linear_backward": [_i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+    "cpmk_gated_linear_backward": [_i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
     "cpmk_gated_feed_forward_forward": [_i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
-    "cpmk_gated_feed_forward_backward": [_i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+    "cpmk_gated_feed_forward_backward": [_i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
 }
 
 # codes of the `dtype` and `activation` arguments

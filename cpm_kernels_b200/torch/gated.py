@@ -5,7 +5,7 @@ with both projections, the activation and the product in one pass, and the activ
 before it on the way back.  fp16 and bf16, fp32 sums."""
 import torch
 
-from ..kernels import gated_linear_forward, gated_linear_backward, gated_feed_forward_forward, gated_feed_forward_backward, gated_scratch
+from ..kernels import gated_linear_forward, gated_linear_backward, gated_feed_forward_forward, gated_feed_forward_backward, gated_scratch, gated_backward_scratch
 from ..library import cpmk
 from ._launch import address, launch, once
 
@@ -22,8 +22,7 @@ def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation
     assert activation in cpmk.ACTIVATIONS
 
 
-def _scratch(tokens: int, k: int, n: int, m: int, device):
-    size = gated_scratch(tokens, k, n, m)
+def _scratch(size: int, device):
     return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
 
 
@@ -35,7 +34,7 @@ def _part(t, i: int) -> int:
 def _launch_linear(x, w_gate, w_up, activation, h, gu, stream):
     n, k = w_gate.shape
     tokens = x.numel() // k
-    scratch = _scratch(tokens, k, n, 0, x.device)
+    scratch = _scratch(gated_scratch(tokens, k, n), x.device)
     gated_linear_forward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(),
                          _part(gu, 0) if gu is not None else 0, _part(gu, 1) if gu is not None else 0, address(scratch), stream)
 
@@ -46,6 +45,14 @@ def _linear_forward(x, w_gate, w_up, activation: str, save: bool):
     gu = torch.empty((2, x.numel() // k, n), dtype=x.dtype, device=x.device) if save else None
     launch(x.get_device(), _launch_linear, x, w_gate, w_up, activation, h, gu)
     return h, gu
+
+
+def _launch_linear_backward(x, w_gate, w_up, activation, gu, dh, dgu, dx, dw_gate, dw_up, stream):
+    n, k = w_gate.shape
+    tokens = x.numel() // k
+    scratch = _scratch(gated_backward_scratch(tokens, k, n), x.device)
+    gated_linear_backward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                          _part(gu, 0), _part(gu, 1), _part(dgu, 0), _part(dgu, 1), address(dx), address(dw_gate), address(dw_up), address(scratch), stream)
 
 
 class OpGatedLinear(torch.autograd.Function):
@@ -60,13 +67,9 @@ class OpGatedLinear(torch.autograd.Function):
     @once
     def backward(ctx, grad_output: torch.Tensor):
         x, w_gate, w_up, gu = ctx.saved_tensors
-        dh = grad_output.contiguous()
-        n, k = w_gate.shape
         dgu = torch.empty_like(gu)
         dx, dw_gate, dw_up = (torch.empty_like(t) if need else None for t, need in zip((x, w_gate, w_up), ctx.needs_input_grad))
-        launch(x.get_device(), gated_linear_backward, x.numel() // k, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation], dh.data_ptr(),
-               x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _part(gu, 0), _part(gu, 1), _part(dgu, 0), _part(dgu, 1), address(dx), address(dw_gate),
-               address(dw_up))
+        launch(x.get_device(), _launch_linear_backward, x, w_gate, w_up, ctx.activation, gu, grad_output.contiguous(), dgu, dx, dw_gate, dw_up)
         return dx, dw_gate, dw_up, None
 
 
@@ -84,7 +87,7 @@ def _launch_block(x, w_gate, w_up, w_down, activation, hgu, y, stream):
     n, k = w_gate.shape
     m = w_down.size(0)
     tokens = x.numel() // k
-    scratch = _scratch(tokens, k, n, m, x.device)
+    scratch = _scratch(gated_scratch(tokens, k, n, m), x.device)
     save = hgu.size(0) == 3
     gated_feed_forward_forward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
                                w_down.data_ptr(), hgu.data_ptr(), _part(hgu, 1) if save else 0, _part(hgu, 2) if save else 0, y.data_ptr(),
@@ -99,6 +102,17 @@ def _block_forward(x, w_gate, w_up, w_down, activation: str, save: bool):
     return y, hgu
 
 
+def _launch_block_backward(x, w_gate, w_up, w_down, activation, hgu, dy, dx, dw_gate, dw_up, dw_down, stream):
+    n, k = w_gate.shape
+    m = w_down.size(0)
+    tokens = x.numel() // k
+    dgu = torch.empty((2, tokens, n), dtype=x.dtype, device=x.device)
+    scratch = _scratch(gated_backward_scratch(tokens, k, n, m), x.device)
+    gated_feed_forward_backward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+                                w_up.data_ptr(), w_down.data_ptr(), _part(hgu, 1), _part(hgu, 2), hgu.data_ptr(), _part(dgu, 0), _part(dgu, 1),
+                                address(dx), address(dw_gate), address(dw_up), address(dw_down), address(scratch), stream)
+
+
 class OpGatedFeedForward(torch.autograd.Function):
 
     @staticmethod
@@ -111,14 +125,8 @@ class OpGatedFeedForward(torch.autograd.Function):
     @once
     def backward(ctx, grad_output: torch.Tensor):
         x, w_gate, w_up, w_down, hgu = ctx.saved_tensors
-        dy = grad_output.contiguous()
-        n, k = w_gate.shape
-        tokens = x.numel() // k
-        dgu = torch.empty((2, tokens, n), dtype=x.dtype, device=x.device)
         dx, dw_gate, dw_up, dw_down = (torch.empty_like(t) if need else None for t, need in zip((x, w_gate, w_up, w_down), ctx.needs_input_grad))
-        launch(x.get_device(), gated_feed_forward_backward, tokens, k, n, w_down.size(0), _DTYPES[x.dtype], cpmk.ACTIVATIONS[ctx.activation],
-               dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _part(hgu, 1), _part(hgu, 2), hgu.data_ptr(),
-               _part(dgu, 0), _part(dgu, 1), address(dx), address(dw_gate), address(dw_up), address(dw_down))
+        launch(x.get_device(), _launch_block_backward, x, w_gate, w_up, w_down, ctx.activation, hgu, grad_output.contiguous(), dx, dw_gate, dw_up, dw_down)
         return dx, dw_gate, dw_up, dw_down, None
 
 

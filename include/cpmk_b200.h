@@ -346,6 +346,9 @@ int32_t cpmk_layernorm_rows_backward(int32_t rows, int32_t n, int32_t dtype, con
  * current device (0: none).  `scratch` (16-byte aligned) is the caller's and not kept; calls that overlap need scratch of their own. */
 int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int64_t *bytes);
 
+/* The same for cpmk_gated_linear_backward (m = 0) and cpmk_gated_feed_forward_backward. */
+int32_t cpmk_gated_backward_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int64_t *bytes);
+
 /* h = act(x w_gate^T) * (x w_up^T): both projections, the activation and the product in one pass; the activation is applied to the
  * fp32 sums.  x (tokens, k); w_gate, w_up (n, k); h (tokens, n).  g, u: (tokens, n), the two projections rounded to `dtype`, written
  * for the backward pass, or both NULL.  The two linears, the gelu and the elementwise product of a gated block, which the reference's
@@ -358,7 +361,7 @@ int32_t cpmk_gated_linear_forward(int32_t tokens, int32_t k, int32_t n, int32_t 
  * dx, dw_gate, dw_up may be NULL. */
 int32_t cpmk_gated_linear_backward(int32_t tokens, int32_t k, int32_t n, int32_t dtype, int32_t activation, const void *dh, const void *x,
                                    const void *w_gate, const void *w_up, const void *g, const void *u, void *dg, void *du, void *dx, void *dw_gate,
-                                   void *dw_up, cpmk_stream_t stream);
+                                   void *dw_up, void *scratch, cpmk_stream_t stream);
 
 /* y = h w_down^T after cpmk_gated_linear_forward: x (tokens, k), w_gate and w_up (n, k), w_down (m, n), y (tokens, m).  h (tokens, n)
  * is written as well (the backward pass reads it). */
@@ -371,7 +374,8 @@ int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, in
  * as cpmk_gated_linear_backward. */
 int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *dy,
                                          const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *g, const void *u,
-                                         const void *h, void *dg, void *du, void *dx, void *dw_gate, void *dw_up, void *dw_down, cpmk_stream_t stream);
+                                         const void *h, void *dg, void *du, void *dx, void *dw_gate, void *dw_up, void *dw_down, void *scratch,
+                                         cpmk_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -25,8 +25,8 @@ def test_launchers_check_sizes():
     with pytest.raises(AssertionError):
         ck.gated_linear_forward(1, 0, 8, cpmk.F16, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     with pytest.raises(AssertionError):
-        ck.gated_linear_backward(1, 8, 0, cpmk.F16, 0, *([0] * 11), 0)
+        ck.gated_linear_backward(1, 8, 0, cpmk.F16, 0, *([0] * 12), 0)
     with pytest.raises(AssertionError):
         ck.gated_feed_forward_forward(1, 8, 8, 0, cpmk.F16, 0, *([0] * 9), 0)
     with pytest.raises(AssertionError):
-        ck.gated_feed_forward_backward(-1, 8, 8, 8, cpmk.F16, 0, *([0] * 14), 0)
+        ck.gated_feed_forward_backward(-1, 8, 8, 8, cpmk.F16, 0, *([0] * 15), 0)

@@ -253,12 +253,12 @@ def test_nothing_is_written_outside_the_outputs(tokens, k, n, m):
     h, g, u, dg, du = (guard(tokens * n) for _ in range(5))
     y, dx, dwg, dwu, dwd = guard(tokens * m), guard(tokens * k), guard(n * k), guard(n * k), guard(m * n)
     at = lambda t: t.data_ptr() + 2 * pad
-    need = ck.gated_scratch(tokens, k, n, m)
+    need = max(ck.gated_scratch(tokens, k, n, m), ck.gated_backward_scratch(tokens, k, n, m))
     scratch = torch.full((need + 256,), 77, dtype=torch.uint8, device="cuda")
     p = lambda t: t.data_ptr()
     ck.gated_feed_forward_forward(tokens, k, n, m, cpmk.F16, 0, p(x), p(wg), p(wu), p(wd), at(h), at(g), at(u), at(y), p(scratch), s)
     ck.gated_feed_forward_backward(tokens, k, n, m, cpmk.F16, 0, p(dy), p(x), p(wg), p(wu), p(wd), at(g), at(u), at(h), at(dg), at(du), at(dx), at(dwg),
-                                   at(dwu), at(dwd), s)
+                                   at(dwu), at(dwd), p(scratch), s)
     for t in (h, g, u, dg, du, y, dx, dwg, dwu, dwd):
         assert (t[:pad] == 7).all() and (t[-pad:] == 7).all()
     assert (scratch[need:] == 77).all()
