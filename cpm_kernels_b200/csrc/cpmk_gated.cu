@@ -199,6 +199,8 @@ bool even_address(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 1u) 
 int32_t begin(Call *call, int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t act, cpmk_stream_t stream) {
     const int32_t rc = current_device_info(&call->info);
     if (rc) return rc;
+    // a thread whose first CUDA call this is (autograd's) has no context yet, and encoding a tensor map fails without one
+    CPMK_CUDA_TRY(cudaSetDevice(call->info.device));
     CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 1, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
     CPMK_REQUIRE(dtype == CPMK_F16 || dtype == CPMK_BF16, "the gated block takes fp16 and bf16 (dtype %d)", dtype);
     CPMK_REQUIRE(act == CPMK_ACT_GELU || act == CPMK_ACT_SILU, "unknown activation %d", act);

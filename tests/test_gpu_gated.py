@@ -236,6 +236,21 @@ def test_some_gradients_only(tokens, k, n, m):
             assert torch.equal(v, full[i])
 
 
+@pytest.mark.parametrize("tokens", [4, 300])
+def test_a_thread_that_has_not_used_the_device(tokens):
+    """The first CUDA call of a thread: no context is current on it, and PyTorch serves the outputs from its cache."""
+    import threading
+    x, wg, wu, wd, _, _ = make(tokens, 64, 64, 64, torch.half, 14)
+    want = ct.gated_feed_forward(x, wg, wu, wd)
+    torch.cuda.synchronize()
+    got = []
+    thread = threading.Thread(target=lambda: got.append(ct.gated_feed_forward(x, wg, wu, wd)))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1 and torch.equal(got[0], want)
+
+
 def test_the_same_tensor_as_both_weights():
     x, wg, _, _, _, dh = make(40, 64, 64, 64, torch.half, 7)
     a, b = wg.clone().requires_grad_(), wg.clone().requires_grad_()
