@@ -9,8 +9,8 @@ def round_up(x: int, m: int) -> int:
     return (x + m - 1) // m * m
 
 
-def stream_arg(stream) -> ctypes.c_void_p:
+def stream_arg(stream):
     """Accept an int, None or a ctypes pointer for the stream, as the reference's callers pass them."""
-    if isinstance(stream, ctypes.c_void_p):
-        return stream
+    if isinstance(stream, (int, ctypes.c_void_p)):
+        return stream                       # the bound functions take an address as it is
     return ctypes.c_void_p(stream or 0)

@@ -31,7 +31,7 @@ def gated_linear_forward(tokens: int, k: int, n: int, dtype: int, activation: in
                          stream: CUDAStream):
     """h = act(x w_gate^T) * (x w_up^T)."""
     assert tokens >= 0 and k >= 1 and n >= 1
-    cpmk.call("cpmk_gated_linear_forward", tokens, k, n, dtype, activation, x, w_gate, w_up, h, g or None, u or None, scratch or None,
+    cpmk.call("cpmk_gated_linear_forward", tokens, k, n, dtype, activation, x, w_gate, w_up, h, g, u, scratch,
               stream_arg(stream))
 
 
@@ -46,8 +46,8 @@ def gated_linear_backward(tokens: int, k: int, n: int, dtype: int, activation: i
                           scratch: DevicePointer,   # gated_backward_scratch(tokens, k, n) bytes
                           stream: CUDAStream):
     assert tokens >= 0 and k >= 1 and n >= 1
-    cpmk.call("cpmk_gated_linear_backward", tokens, k, n, dtype, activation, dh, x, w_gate, w_up, g, u, dg, du, dx or None, dw_gate or None,
-              dw_up or None, scratch or None, stream_arg(stream))
+    cpmk.call("cpmk_gated_linear_backward", tokens, k, n, dtype, activation, dh, x, w_gate, w_up, g, u, dg, du, dx, dw_gate,
+              dw_up, scratch, stream_arg(stream))
 
 
 def gated_feed_forward_forward(tokens: int, k: int, n: int, m: int, dtype: int, activation: int,
@@ -60,8 +60,8 @@ def gated_feed_forward_forward(tokens: int, k: int, n: int, m: int, dtype: int, 
                                stream: CUDAStream):
     """h as gated_linear_forward, y = h w_down^T."""
     assert tokens >= 0 and k >= 1 and n >= 1 and m >= 1
-    cpmk.call("cpmk_gated_feed_forward_forward", tokens, k, n, m, dtype, activation, x, w_gate, w_up, w_down, h, g or None, u or None, y,
-              scratch or None, stream_arg(stream))
+    cpmk.call("cpmk_gated_feed_forward_forward", tokens, k, n, m, dtype, activation, x, w_gate, w_up, w_down, h, g, u, y,
+              scratch, stream_arg(stream))
 
 
 def gated_feed_forward_backward(tokens: int, k: int, n: int, m: int, dtype: int, activation: int,
@@ -75,5 +75,5 @@ def gated_feed_forward_backward(tokens: int, k: int, n: int, m: int, dtype: int,
                                 scratch: DevicePointer,   # gated_backward_scratch(tokens, k, n, m) bytes
                                 stream: CUDAStream):
     assert tokens >= 0 and k >= 1 and n >= 1 and m >= 1
-    cpmk.call("cpmk_gated_feed_forward_backward", tokens, k, n, m, dtype, activation, dy, x, w_gate, w_up, w_down, g, u, h or None, dg, du, dx or None,
-              dw_gate or None, dw_up or None, dw_down or None, scratch or None, stream_arg(stream))
+    cpmk.call("cpmk_gated_feed_forward_backward", tokens, k, n, m, dtype, activation, dy, x, w_gate, w_up, w_down, g, u, h, dg, du, dx,
+              dw_gate, dw_up, dw_down, scratch, stream_arg(stream))

@@ -17,8 +17,7 @@ def layernorm_rows_forward(rows: int, n: int, dtype: int,
                            stream: CUDAStream):
     """y = (x - mean) * rstd * weight + bias per row; ``rd_mean`` False: mean = 0 (the RMS form)."""
     assert rows >= 0 and n >= 1
-    cpmk.call("cpmk_layernorm_rows_forward", rows, n, dtype, x, float(eps), int(bool(rd_mean)), weight, bias or None, y, mean or None, rstd or None,
-              stream_arg(stream))
+    cpmk.call("cpmk_layernorm_rows_forward", rows, n, dtype, x, eps, 1 if rd_mean else 0, weight, bias, y, mean, rstd, stream_arg(stream))
 
 
 def layernorm_rows_backward_scratch(rows: int, n: int) -> int:
@@ -40,5 +39,5 @@ def layernorm_rows_backward(rows: int, n: int, dtype: int,
                             scratch: DevicePointer,    # layernorm_rows_backward_scratch(rows, n) bytes
                             stream: CUDAStream):
     assert rows >= 0 and n >= 1
-    cpmk.call("cpmk_layernorm_rows_backward", rows, n, dtype, dy, x, int(bool(rd_mean)), weight, mean, rstd, dx or None, dweight or None, dbias or None,
-              scratch or None, stream_arg(stream))
+    cpmk.call("cpmk_layernorm_rows_backward", rows, n, dtype, dy, x, 1 if rd_mean else 0, weight, mean, rstd, dx, dweight, dbias, scratch,
+              stream_arg(stream))

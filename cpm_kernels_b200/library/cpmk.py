@@ -101,7 +101,9 @@ def check_status(status: int, what: str) -> None:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point; raise RuntimeError on failure."""
-    check_status(getattr(lib, name)(*args), name)
+    status = getattr(lib, name)(*args)
+    if status != OK:
+        check_status(status, name)
 
 
 def check_device() -> int:

@@ -13,36 +13,32 @@ _DTYPES = {torch.float16: cpmk.F16, torch.bfloat16: cpmk.BF16}
 
 
 def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str) -> None:
-    assert x.is_cuda and x.is_contiguous() and x.ndim >= 1 and x.dtype in _DTYPES
-    assert x.size(-1) >= 1 and x.numel() // x.size(-1) < 2 ** 31
-    for w in (w_gate, w_up):
-        assert w.is_cuda and w.device == x.device and w.is_contiguous() and w.ndim == 2 and w.dtype == x.dtype
-        assert w.size(0) >= 1 and w.size(1) == x.size(-1)
-    assert w_gate.size(0) == w_up.size(0)
+    dtype, device = x.dtype, x.device
+    assert x.is_cuda and x.is_contiguous() and x.ndim >= 1 and dtype in _DTYPES
+    k, n = x.size(-1), w_gate.size(0)
+    assert k >= 1 and n >= 1 and x.numel() // k < 2 ** 31
+    assert w_gate.device == device and w_gate.dtype == dtype and w_gate.shape == (n, k) and w_gate.is_contiguous()
+    assert w_up.device == device and w_up.dtype == dtype and w_up.shape == (n, k) and w_up.is_contiguous()
     assert activation in cpmk.ACTIVATIONS
 
 
-def _scratch(size: int, device):
-    return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
-
-
-def _part(t, i: int) -> int:
-    """Address of t[i] for a contiguous t, without a view of it."""
-    return t.data_ptr() + i * (t.numel() // t.size(0)) * t.element_size()
+def _scratch(size: int, x: torch.Tensor):
+    return x.new_empty(size, dtype=torch.uint8) if size else None
 
 
 def _launch_linear(x, w_gate, w_up, activation, h, gu, stream):
     n, k = w_gate.shape
     tokens = x.numel() // k
-    scratch = _scratch(gated_scratch(tokens, k, n), x.device)
+    scratch = _scratch(gated_scratch(tokens, k, n), x)
+    g = address(gu)
     gated_linear_forward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(),
-                         _part(gu, 0) if gu is not None else 0, _part(gu, 1) if gu is not None else 0, address(scratch), stream)
+                         g, g + 2 * tokens * n if g else 0, address(scratch), stream)
 
 
 def _linear_forward(x, w_gate, w_up, activation: str, save: bool):
     n, k = w_gate.shape
-    h = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    gu = torch.empty((2, x.numel() // k, n), dtype=x.dtype, device=x.device) if save else None
+    h = x.new_empty((*x.shape[:-1], n))
+    gu = x.new_empty((2, x.numel() // k, n)) if save else None
     launch(x.get_device(), _launch_linear, x, w_gate, w_up, activation, h, gu)
     return h, gu
 
@@ -50,9 +46,10 @@ def _linear_forward(x, w_gate, w_up, activation: str, save: bool):
 def _launch_linear_backward(x, w_gate, w_up, activation, gu, dh, dgu, dx, dw_gate, dw_up, stream):
     n, k = w_gate.shape
     tokens = x.numel() // k
-    scratch = _scratch(gated_backward_scratch(tokens, k, n), x.device)
+    scratch = _scratch(gated_backward_scratch(tokens, k, n), x)
+    g, dg, each = gu.data_ptr(), dgu.data_ptr(), 2 * tokens * n
     gated_linear_backward(tokens, k, n, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-                          _part(gu, 0), _part(gu, 1), _part(dgu, 0), _part(dgu, 1), address(dx), address(dw_gate), address(dw_up), address(scratch), stream)
+                          g, g + each, dg, dg + each, address(dx), address(dw_gate), address(dw_up), address(scratch), stream)
 
 
 class OpGatedLinear(torch.autograd.Function):
@@ -87,17 +84,18 @@ def _launch_block(x, w_gate, w_up, w_down, activation, hgu, y, stream):
     n, k = w_gate.shape
     m = w_down.size(0)
     tokens = x.numel() // k
-    scratch = _scratch(gated_scratch(tokens, k, n, m), x.device)
+    scratch = _scratch(gated_scratch(tokens, k, n, m), x)
+    h, each = hgu.data_ptr(), 2 * tokens * n
     save = hgu.size(0) == 3
     gated_feed_forward_forward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-                               w_down.data_ptr(), hgu.data_ptr(), _part(hgu, 1) if save else 0, _part(hgu, 2) if save else 0, y.data_ptr(),
+                               w_down.data_ptr(), h, h + each if save else 0, h + 2 * each if save else 0, y.data_ptr(),
                                address(scratch), stream)
 
 
 def _block_forward(x, w_gate, w_up, w_down, activation: str, save: bool):
     n, k = w_gate.shape
-    y = torch.empty((*x.shape[:-1], w_down.size(0)), dtype=x.dtype, device=x.device)
-    hgu = torch.empty((3 if save else 1, x.numel() // k, n), dtype=x.dtype, device=x.device)      # h, and g, u for the backward pass
+    y = x.new_empty((*x.shape[:-1], w_down.size(0)))
+    hgu = x.new_empty((3 if save else 1, x.numel() // k, n))      # h, and g, u for the backward pass
     launch(x.get_device(), _launch_block, x, w_gate, w_up, w_down, activation, hgu, y)
     return y, hgu
 
@@ -106,10 +104,11 @@ def _launch_block_backward(x, w_gate, w_up, w_down, activation, hgu, dy, dx, dw_
     n, k = w_gate.shape
     m = w_down.size(0)
     tokens = x.numel() // k
-    dgu = torch.empty((2, tokens, n), dtype=x.dtype, device=x.device)
-    scratch = _scratch(gated_backward_scratch(tokens, k, n, m), x.device)
+    dgu = x.new_empty((2, tokens, n))
+    scratch = _scratch(gated_backward_scratch(tokens, k, n, m), x)
+    h, dg, each = hgu.data_ptr(), dgu.data_ptr(), 2 * tokens * n
     gated_feed_forward_backward(tokens, k, n, m, _DTYPES[x.dtype], cpmk.ACTIVATIONS[activation], dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
-                                w_up.data_ptr(), w_down.data_ptr(), _part(hgu, 1), _part(hgu, 2), hgu.data_ptr(), _part(dgu, 0), _part(dgu, 1),
+                                w_up.data_ptr(), w_down.data_ptr(), h + each, h + 2 * each, h, dg, dg + each,
                                 address(dx), address(dw_gate), address(dw_up), address(dw_down), address(scratch), stream)
 
 
@@ -135,7 +134,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     The hidden activations between the two are rounded to the tensors' type.  Differentiable (once) in x and the three weights; a call
     that is differentiated keeps the two projections and the hidden activations."""
     _check(x, w_gate, w_up, activation)
-    assert w_down.is_cuda and w_down.device == x.device and w_down.is_contiguous() and w_down.ndim == 2 and w_down.dtype == x.dtype
+    assert w_down.device == x.device and w_down.dtype == x.dtype and w_down.ndim == 2 and w_down.is_contiguous()
     assert w_down.size(0) >= 1 and w_down.size(1) == w_gate.size(0)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         return OpGatedFeedForward.apply(x, w_gate, w_up, w_down, activation)

@@ -17,7 +17,7 @@ def _forward(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Optional[t
     n = weight.numel()
     rows = x.numel() // n
     y = torch.empty_like(x)
-    stats = torch.empty((2 * rows,), dtype=torch.float32, device=x.device) if statistics else None
+    stats = x.new_empty(2 * rows, dtype=torch.float32) if statistics else None
     mean = address(stats)
     launch(x.get_device(), layernorm_rows_forward, rows, n, _DTYPES[x.dtype], x.data_ptr(), eps, rd_mean, weight.data_ptr(), address(bias), y.data_ptr(),
            mean, mean + 4 * rows if statistics else 0)
@@ -27,7 +27,7 @@ def _forward(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Optional[t
 def _launch_backward(rows, n, dtype, dy, x, rd_mean, weight, stats, dx, dweight, dbias, stream):
     scratch = None
     if dweight is not None or dbias is not None:
-        scratch = torch.empty((layernorm_rows_backward_scratch(rows, n),), dtype=torch.uint8, device=x.device)
+        scratch = x.new_empty(layernorm_rows_backward_scratch(rows, n), dtype=torch.uint8)
     mean = stats.data_ptr()
     layernorm_rows_backward(rows, n, dtype, dy.data_ptr(), x.data_ptr(), rd_mean, weight.data_ptr(), mean, mean + 4 * rows, address(dx), address(dweight),
                             address(dbias), address(scratch), stream)
@@ -59,12 +59,13 @@ def layernorm_rows(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Opti
     """Layer norm of ``x`` (..., n) over its last axis, times ``weight`` (n), plus ``bias`` (n) if given; ``rd_mean`` False leaves the
     mean in (the RMS form).  fp16, bf16 or fp32, the same type for all three; statistics in fp32.  Differentiable in x, weight and bias
     (once).  Any n >= 1 and any number of rows, none included."""
-    assert x.is_cuda and x.is_contiguous() and x.ndim >= 1 and x.dtype in _DTYPES
-    assert x.size(-1) >= 1 and x.numel() // x.size(-1) < 2 ** 31
+    dtype, device = x.dtype, x.device
+    assert x.is_cuda and x.is_contiguous() and x.ndim >= 1 and dtype in _DTYPES
+    n = x.size(-1)
+    assert n >= 1 and x.numel() // n < 2 ** 31
     assert eps >= 0
-    for v in (weight, bias):
-        if v is not None:
-            assert v.is_cuda and v.device == x.device and v.is_contiguous() and v.ndim == 1 and v.dtype == x.dtype and v.numel() == x.size(-1)
+    assert weight.device == device and weight.dtype == dtype and weight.shape == (n,) and weight.is_contiguous()
+    assert bias is None or (bias.device == device and bias.dtype == dtype and bias.shape == (n,) and bias.is_contiguous())
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return OpLayerNormRows.apply(x, eps, weight, bias, rd_mean)
     return _forward(x, eps, weight, bias, rd_mean, False)[0]
