@@ -71,6 +71,27 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     volatile uint32_t *abort_flag = tmem_slot + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     launch_dependents();
+    const int64_t u0 = first_unit(blockIdx.x, gridDim.x, prm.units), u1 = first_unit((int64_t)blockIdx.x + 1, gridDim.x, prm.units);
+    const int32_t count = (int32_t)(u1 - u0);
+    const int32_t tile0 = (int32_t)(u0 / prm.blocks), block0 = (int32_t)(u0 - (int64_t)tile0 * prm.blocks);
+    const int32_t ahead = min(prm.stages, count);
+    int tile = tile0, block = block0;                    // the producer's next
+    auto load_weights = [&](uint32_t stage) {
+        const uint32_t dst = ring + stage * (uint32_t)prm.stage_bytes, bar = full_bar + 8 * stage;
+        mbar_expect_tx(bar, (uint32_t)prm.stage_bytes);
+        if (GATED) {
+            tma_load_3d(dst, &maps.w[0], block * kStageK, tile * 64, 0, bar);
+            tma_load_3d(dst + kWeightBytes / 2, &maps.w[1], block * kStageK, tile * 64, 0, bar);
+        } else {
+            tma_load_3d(dst, &maps.w[0], block * kStageK, tile * kRows, 0, bar);
+        }
+    };
+    auto load_x = [&](uint32_t stage, int x_block) {
+        tma_load_3d(ring + stage * (uint32_t)prm.stage_bytes + kWeightBytes, &maps.x, x_block * kStageK, 0, 0, full_bar + 8 * stage);
+    };
+    auto advance = [&]() {
+        if (++block == prm.blocks) { block = 0; ++tile; }
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < prm.stages; ++s) {
             mbar_init(full_bar + 8 * s, 1);
@@ -83,50 +104,32 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // the first ring's worth of weights is requested before anything else is set up, and before x is there
+        for (int i = 0; i < ahead; ++i) {
+            load_weights((uint32_t)i);
+            advance();
+        }
     }
     if (warp == 1) tmem_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), (uint32_t)prm.tmem_columns);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int64_t u0 = first_unit(blockIdx.x, gridDim.x, prm.units), u1 = first_unit((int64_t)blockIdx.x + 1, gridDim.x, prm.units);
-    const int32_t count = (int32_t)(u1 - u0);
-    const int32_t tile0 = (int32_t)(u0 / prm.blocks), block0 = (int32_t)(u0 - (int64_t)tile0 * prm.blocks);
 
     if (warp == 0) {
         if (lane == 0) {
-            // the weights of the first ring's worth are requested before x is there
-            auto weights = [&](uint32_t stage, int tile, int block) {
-                const uint32_t dst = ring + stage * (uint32_t)prm.stage_bytes, bar = full_bar + 8 * stage;
-                mbar_expect_tx(bar, (uint32_t)prm.stage_bytes);
-                if (GATED) {
-                    tma_load_3d(dst, &maps.w[0], block * kStageK, tile * 64, 0, bar);
-                    tma_load_3d(dst + kWeightBytes / 2, &maps.w[1], block * kStageK, tile * 64, 0, bar);
-                } else {
-                    tma_load_3d(dst, &maps.w[0], block * kStageK, tile * kRows, 0, bar);
-                }
-            };
-            auto tokens = [&](uint32_t stage, int block) {
-                tma_load_3d(ring + stage * (uint32_t)prm.stage_bytes + kWeightBytes, &maps.x, block * kStageK, 0, 0, full_bar + 8 * stage);
-            };
-            const int ahead = min(prm.stages, count);
-            int tile = tile0, block = block0;
-            for (int i = 0; i < ahead; ++i) {
-                weights((uint32_t)i, tile, block);
-                if (++block == prm.blocks) { block = 0; ++tile; }
-            }
             if (prm.after_prior) wait_for_prior_grid();
             int x_block = block0;
             for (int i = 0; i < ahead; ++i) {
-                tokens((uint32_t)i, x_block);
+                load_x((uint32_t)i, x_block);
                 if (++x_block == prm.blocks) x_block = 0;
             }
             uint32_t stage = 0, phase = 0;               // of the next wait for an empty stage
             for (int i = ahead; i < count; ++i) {
                 if (!mbar_wait(empty_bar + 8 * stage, phase, abort_flag, prm.status, kErrLoad)) break;
-                weights(stage, tile, block);
-                tokens(stage, block);
-                if (++block == prm.blocks) { block = 0; ++tile; }
+                load_weights(stage);
+                load_x(stage, block);
+                advance();
                 if (++stage == (uint32_t)prm.stages) { stage = 0; phase ^= 1u; }
             }
         }
