@@ -120,27 +120,44 @@ int32_t launch_simt(const Call &call, SimtParams prm) {
 
 bool tensor_core_size(int32_t extent) { return extent % 8 == 0; }
 
-// out0 (R, C) = P0 Q0^T (+ P1 Q1^T when `sum`), or out0 = P0 Q0^T and out1 = P1 Q1^T when out1 is given.  p_t / q_t: the operand is stored
-// (K, rows) instead of (rows, K).  The tensor cores' loads and stores want 16-byte rows and addresses; everything else runs generic.
-int32_t product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1, const void *q1,
-                bool sum, void *out0, void *out1, void *scratch) {
-    if (tensor_core_size(p_t ? R : K) && tensor_core_size(q_t ? C : K) && tensor_core_size(C) && aligned16(p0) && aligned16(q0) && aligned16(p1) &&
-        aligned16(q1) && aligned16(out0) && aligned16(out1))
-        return tc_product(call, R, C, K, p_t, q_t, p0, q0, p1, q1, sum, out0, out1, scratch);
+// The tensor cores' loads and stores want 16-byte rows and addresses; everything else runs generic.
+bool on_tensor_cores(const Product &p, int32_t K, bool transposed) {
+    return tensor_core_size(transposed ? p.R : K) && tensor_core_size(p.C) && aligned16(p.p) && aligned16(p.q) && aligned16(p.out);
+}
+
+// Up to three products out (R, C) = P Q^T of the same K; operands stored (rows, K), or (K, rows) when `transposed`.
+int32_t products_of(const Call &call, int32_t K, bool transposed, const Product *products, int count, void *scratch) {
+    bool all = true;
+    for (int i = 0; i < count; ++i) all = all && on_tensor_cores(products[i], K, transposed);
+    if (all) return tc_products(call, K, transposed, products, count, scratch);
+    for (int i = 0; i < count; ++i) {
+        const Product &p = products[i];
+        int32_t rc;
+        if (on_tensor_cores(p, K, transposed)) {
+            rc = tc_products(call, K, transposed, &p, 1, scratch);
+        } else {
+            SimtParams prm = {};
+            prm.R = p.R; prm.C = p.C; prm.K = K;
+            prm.p_rs = transposed ? 1 : K; prm.p_ks = transposed ? p.R : 1;
+            prm.q_rs = transposed ? 1 : K; prm.q_ks = transposed ? p.C : 1;
+            prm.p[0] = p.p; prm.q[0] = p.q;
+            prm.out[0] = p.out;
+            rc = launch_simt<kEpiStore>(call, prm);
+        }
+        if (rc) return rc;
+    }
+    return CPMK_OK;
+}
+
+// out (R, C) = P0 Q0^T + P1 Q1^T, P stored (R, K), Q stored (K, C)
+int32_t sum_of(const Call &call, int32_t R, int32_t C, int32_t K, const void *p0, const void *q0, const void *p1, const void *q1, void *out, void *scratch) {
+    if (tensor_core_size(K) && tensor_core_size(C) && aligned16(p0) && aligned16(q0) && aligned16(p1) && aligned16(q1) && aligned16(out))
+        return tc_sum(call, R, C, K, p0, q0, p1, q1, out, scratch);
     SimtParams prm = {};
     prm.R = R; prm.C = C; prm.K = K;
-    prm.p_rs = p_t ? 1 : K; prm.p_ks = p_t ? R : 1;
-    prm.q_rs = q_t ? 1 : K; prm.q_ks = q_t ? C : 1;
-    prm.p[0] = p0; prm.q[0] = q0;
-    if (sum) {
-        prm.p[1] = p1;
-        prm.q[1] = q1;
-    }
-    prm.out[0] = out0;
-    const int32_t rc = launch_simt<kEpiStore>(call, prm);
-    if (rc || !out1) return rc;
-    prm.p[0] = p1; prm.q[0] = q1;
-    prm.out[0] = out1;
+    prm.p_rs = K; prm.p_ks = 1; prm.q_rs = 1; prm.q_ks = C;
+    prm.p[0] = p0; prm.p[1] = p1; prm.q[0] = q0; prm.q[1] = q1;
+    prm.out[0] = out;
     return launch_simt<kEpiStore>(call, prm);
 }
 
@@ -210,14 +227,19 @@ int32_t begin(Call *call, int32_t tokens, int32_t k, int32_t n, int32_t m, int32
     return CPMK_OK;
 }
 
-// dx, dWg, dWu from dg, du
-int32_t projections_backward(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, const void *dg,
-                             const void *du, void *dx, void *dwg, void *dwu, void *scratch) {
-    int32_t rc = CPMK_OK;
-    if (dx) rc = product(call, tokens, k, n, false, true, dg, wg, du, wu, true, dx, nullptr, scratch);
-    if (rc || (!dwg && !dwu)) return rc;
-    if (dwg && dwu) return product(call, n, k, tokens, true, true, dg, x, du, x, false, dwg, dwu, scratch);
-    return product(call, n, k, tokens, true, true, dwg ? dg : du, x, nullptr, nullptr, false, dwg ? dwg : dwu, nullptr, scratch);
+// dx, dWg, dWu from dg, du, and dWd from dy, h
+int32_t gradients(const Call &call, int32_t tokens, int32_t k, int32_t n, int32_t m, const void *x, const void *wg, const void *wu, const void *dg,
+                  const void *du, const void *dy, const void *h, void *dx, void *dwg, void *dwu, void *dwd, void *scratch) {
+    if (dx) {
+        const int32_t rc = sum_of(call, tokens, k, n, dg, wg, du, wu, dx, scratch);
+        if (rc) return rc;
+    }
+    Product wanted[3];
+    int count = 0;
+    if (dwg) wanted[count++] = {n, k, dg, x, dwg};
+    if (dwu) wanted[count++] = {n, k, du, x, dwu};
+    if (dwd) wanted[count++] = {m, n, dy, h, dwd};
+    return count ? products_of(call, tokens, true, wanted, count, scratch) : CPMK_OK;
 }
 
 // without tokens the weights' gradients are zero
@@ -257,7 +279,8 @@ int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int6
         // pointers are not known here: room for the few-token pair of products, and for those of the tiles
         if (few_tokens(tokens) && first) need = few_scratch(info, tokens, k, n, down ? m : 0);
         if (!few_tokens(tokens) && first) need = tc_gated_scratch(info, tokens, k, n);
-        if (down) need = larger(need, tc_product_scratch(info, tokens, m, n, false, 1));
+        const Product y = {tokens, m, nullptr, nullptr, nullptr};
+        if (down) need = larger(need, tc_products_scratch(info, n, &y, 1));
     }
     *bytes = need;
     return CPMK_OK;
@@ -270,11 +293,15 @@ int32_t cpmk_gated_backward_scratch(int32_t tokens, int32_t k, int32_t n, int32_
     CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 0 && bytes, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
     int64_t need = 0;
     if (tokens > 0 && tensor_core_size(n)) {
-        if (tensor_core_size(k)) {
-            need = larger(need, tc_product_scratch(info, tokens, k, n, true, 1));
-            need = larger(need, larger(tc_product_scratch(info, n, k, tokens, false, 1), tc_product_scratch(info, n, k, tokens, false, 2)));
-        }
-        if (m > 0 && tensor_core_size(m)) need = larger(need, larger(tc_dact_scratch(info, tokens, n, m), tc_product_scratch(info, m, n, tokens, false, 1)));
+        const bool down = m > 0 && tensor_core_size(m);
+        if (tensor_core_size(k)) need = larger(need, tc_sum_scratch(info, tokens, k, n));
+        if (down) need = larger(need, tc_dact_scratch(info, tokens, n, m));
+        // the weights' gradients that are wanted are not known here: any of them, alone or together
+        const Product up = {n, k, nullptr, nullptr, nullptr}, last = {m, n, nullptr, nullptr, nullptr};
+        const Product ups[3] = {up, up, last}, one[2] = {up, last};
+        for (int count = 1; tensor_core_size(k) && count <= (down ? 3 : 2); ++count) need = larger(need, tc_products_scratch(info, tokens, ups, count));
+        if (down && tensor_core_size(k)) need = larger(need, tc_products_scratch(info, tokens, one, 2));
+        if (down) need = larger(need, tc_products_scratch(info, tokens, &last, 1));
     }
     *bytes = need;
     return CPMK_OK;
@@ -310,7 +337,7 @@ int32_t cpmk_gated_linear_backward(int32_t tokens, int32_t k, int32_t n, int32_t
     if (rc) return rc;
     rc = dact(call, (int64_t)tokens * n, dh, g, u, dg, du);
     if (rc) return rc;
-    return projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up, scratch);
+    return gradients(call, tokens, k, n, 0, x, w_gate, w_up, dg, du, nullptr, nullptr, dx, dw_gate, dw_up, nullptr, scratch);
 }
 
 int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *x,
@@ -331,7 +358,8 @@ int32_t cpmk_gated_feed_forward_forward(int32_t tokens, int32_t k, int32_t n, in
     if (rc) return rc;
     if (few_tokens(tokens) && tensor_core_size(m) && gated_on_tensor_cores(k, n, x, w_gate, w_up, h, g, u) && aligned16(w_down) && aligned16(y))
         return few_down(call, tokens, k, n, m, h, w_down, y, scratch);
-    return product(call, tokens, m, n, false, false, h, w_down, nullptr, nullptr, false, y, nullptr, scratch);
+    const Product down = {tokens, m, h, w_down, y};
+    return products_of(call, n, false, &down, 1, scratch);
 }
 
 int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t activation, const void *dy,
@@ -352,11 +380,8 @@ int32_t cpmk_gated_feed_forward_backward(int32_t tokens, int32_t k, int32_t n, i
     if (dx || dw_gate || dw_up) {
         rc = dact_product(call, tokens, n, m, dy, w_down, g, u, dg, du, scratch);
         if (rc) return rc;
-        rc = projections_backward(call, tokens, k, n, x, w_gate, w_up, dg, du, dx, dw_gate, dw_up, scratch);
-        if (rc) return rc;
     }
-    if (dw_down) return product(call, m, n, tokens, true, true, dy, h, nullptr, nullptr, false, dw_down, nullptr, scratch);
-    return CPMK_OK;
+    return gradients(call, tokens, k, n, m, x, w_gate, w_up, dg, du, dy, h, dx, dw_gate, dw_up, dw_down, scratch);
 }
 
 }  // extern "C"

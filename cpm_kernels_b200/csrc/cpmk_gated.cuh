@@ -47,14 +47,21 @@ struct Call {
 
 // Tensor-core products on 256 x 256 tiles (cpmk_gated_tc.cu): extents multiples of 8, pointers 16-byte aligned, scratch as many bytes as
 // the _scratch function of the product says.
-// out0 (R, C) = P0 Q0^T (+ P1 Q1^T when `sum`), or out0 = P0 Q0^T and out1 = P1 Q1^T when out1 is given.  p_t / q_t: stored (K, rows).
-int32_t tc_product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1,
-                   const void *q1, bool sum, void *out0, void *out1, void *scratch);
+// tc_products: up to three products out (R, C) = P Q^T of the same K in one launch, operands stored (rows, K), or (K, rows) when
+// `transposed`.  tc_sum: out = P0 Q0^T + P1 Q1^T with P stored (R, K), Q stored (K, C).
+struct Product {
+    int32_t R, C;
+    const void *p, *q;
+    void *out;
+};
+int32_t tc_products(const Call &call, int32_t K, bool transposed, const Product *products, int count, void *scratch);
+int32_t tc_sum(const Call &call, int32_t R, int32_t C, int32_t K, const void *p0, const void *q0, const void *p1, const void *q1, void *out, void *scratch);
 int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u,
                  void *scratch);
 int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg, void *du,
                 void *scratch);
-int64_t tc_product_scratch(const DeviceInfo &info, int32_t R, int32_t C, int32_t K, bool sum, int32_t products);
+int64_t tc_products_scratch(const DeviceInfo &info, int32_t K, const Product *products, int count);
+int64_t tc_sum_scratch(const DeviceInfo &info, int32_t R, int32_t C, int32_t K);
 int64_t tc_gated_scratch(const DeviceInfo &info, int32_t tokens, int32_t k, int32_t n);
 int64_t tc_dact_scratch(const DeviceInfo &info, int32_t tokens, int32_t n, int32_t m);
 

@@ -6,7 +6,7 @@
 //               x is staged once for both and the activation and the product need no exchange.  256 x 128 outputs per tile.
 //   kEpiDact    dh = dy Wd stays in tensor memory; the epilogue reads g and u and stores dg = dh u act'(g) and du = dh act(g).
 //   kEpiStore   plain products: h Wd^T; dg Wg + du Wu (one accumulator, k runs through the first pair of operands, then the second);
-//               dg^T x and du^T x (two products of the same sizes in one launch), dy^T h.
+//               dg^T x, du^T x and dy^T h (three products in one launch).
 //
 // Bound by the tensor cores from a few hundred tokens on.  Roles per CTA as in the int8 GEMM: warp 0 issues TMA loads, warp 1 owns the
 // tensor memory and (in the leading CTA) issues the MMAs, warps 2-9 drain accumulators; two accumulators, so the epilogue of one tile
@@ -38,7 +38,7 @@ constexpr uint32_t kErrLoad = 0x201, kErrFull = 0x202, kErrAccumulator = 0x203, 
 // Boxes of 128 rows by 64 k where one load can have them: with two boxes of 64 rows each the gated product took 489 us instead of 459
 // (4096 x 4096 x 20480).
 struct TcMaps {
-    CUtensorMap p[2], q[2], out[3];
+    CUtensorMap p[3], q[3], out[3];
 };
 
 // Whole waves of tiles are walked in bands of kBandRows row tiles, row by row within a column of the band: the band's rows of P stay in
@@ -47,12 +47,13 @@ struct TcMaps {
 // than it takes to join sums (split_pays), their k blocks form one list that is cut into equal pieces, one per pair; a piece leaves
 // fp32 partial sums in scratch, tc_join_kernel adds a tile's pieces in order of k and finishes its outputs.
 struct TcParams {
-    int32_t R, C;
-    int32_t blocks0, blocks;           // k blocks of the first pair of operands, of all
-    int32_t tiles_r, tiles_c, per_product;
+    // up to three products of the same k in one launch (kEpiStore): the weights' gradients
+    int32_t R[3], C[3], tiles_r[3], tiles_c[3], first_tile[3];
+    int32_t p_boxes[3], q_boxes[3];    // loads per 128 rows of P and Q: 1, or 2 for a transposed operand whose rows are no multiple of 64
+    int32_t products;
+    int32_t blocks0, blocks;           // k blocks of the first pair of operands, of all (two pairs: one product)
     int32_t whole;                     // tiles done whole; the others are split
     int32_t split_tiles, split_pairs;  // how many are split, over how many pairs
-    int32_t p_boxes, q_boxes;          // loads per 128 rows of P and Q: 1, or 2 for a transposed operand whose rows are no multiple of 64
     const void *g, *u;                 // kEpiDact: read;  kEpiGated: not null when they are wanted
     float *partial;                    // [split tile + pair][accumulator column][row of the tile]
     uint32_t *status;
@@ -62,17 +63,26 @@ struct Item {
     int32_t product, row, col;         // first row; first column of the outputs
     int32_t block, count;              // k blocks
     int32_t slot;                      // where the partial sums go, -1 for a whole tile
+    int32_t R, C, p_boxes, q_boxes;    // the product's
 };
 
 template <int EPI>
 __device__ __forceinline__ void place(const TcParams &prm, int tile, Item &it) {
-    it.product = tile / prm.per_product;
-    tile -= it.product * prm.per_product;
-    const int band = tile / (kBandRows * prm.tiles_c), in_band = tile - band * kBandRows * prm.tiles_c;
-    const int rows = min(kBandRows, prm.tiles_r - band * kBandRows);
-    const int c = in_band / rows;
-    it.row = (band * kBandRows + in_band - c * rows) * kTileR;
-    it.col = c * (EPI == kEpiGated ? kTileC / 2 : kTileC);
+    // selected by comparisons, not by index, so that the parameters stay in the constant bank (indexed, dy^T h took 267 us, not 218)
+    const bool b = EPI == kEpiStore && prm.products > 1 && tile >= prm.first_tile[1], c = EPI == kEpiStore && prm.products > 2 && tile >= prm.first_tile[2];
+    auto of = [&](const int32_t (&v)[3]) { return c ? v[2] : b ? v[1] : v[0]; };
+    it.product = c ? 2 : b ? 1 : 0;
+    it.R = of(prm.R);
+    it.C = of(prm.C);
+    it.p_boxes = of(prm.p_boxes);
+    it.q_boxes = of(prm.q_boxes);
+    const int tiles_r = of(prm.tiles_r), tiles_c = of(prm.tiles_c);
+    tile -= of(prm.first_tile);
+    const int band = tile / (kBandRows * tiles_c), in_band = tile - band * kBandRows * tiles_c;
+    const int rows = min(kBandRows, tiles_r - band * kBandRows);
+    const int col = in_band / rows;
+    it.row = (band * kBandRows + in_band - col * rows) * kTileR;
+    it.col = col * (EPI == kEpiGated ? kTileC / 2 : kTileC);
 }
 
 // Pair p of P owns the units [p units / P, (p + 1) units / P) of the split tiles' k blocks.
@@ -183,13 +193,13 @@ __device__ __forceinline__ void stage_sums(const Staging &st, int piece, uint32_
 // A warp's share of a finished accumulator: 32 rows from `row`, and the columns of its half.
 template <bool BF16, int EPI, int ACT>
 __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps, const Staging &st, uint32_t tmem, const Item &it, int row, int half) {
-    const int lane = (int)st.lane;
+    const int lane = (int)st.lane, C = it.C;
     if (EPI == kEpiStore) {                              // 128 columns per warp
         const int col = it.col + half * 128;
-        if (col >= prm.C) return;
+        if (col >= C) return;
         st.acquire();
         stage_sums<BF16>(st, 0, tmem + half * 128);
-        const bool second = col + 64 < prm.C;
+        const bool second = col + 64 < C;
         if (second) stage_sums<BF16>(st, 1, tmem + half * 128 + 64);
         st.ready();
         if (lane == 0) {
@@ -200,7 +210,7 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
     } else if (EPI == kEpiGated) {                       // 64 output columns per warp: gate sums, and 128 columns on the up sums
         constexpr int up = 128;
         const int col = it.col + half * 64;
-        if (col >= prm.C) return;
+        if (col >= C) return;
         const uint32_t gate_at = tmem + half * 64;
         st.acquire();
 #pragma unroll
@@ -241,9 +251,9 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
         for (int p = 0; p < 2; ++p) {
             const int offset = half * 128 + p * 64;
             const int col = it.col + offset;
-            if (col >= prm.C) return;
-            const int64_t at = (int64_t)(row + lane) * prm.C + col;
-            const bool in_row = row + lane < prm.R;
+            if (col >= C) return;
+            const int64_t at = (int64_t)(row + lane) * C + col;
+            const bool in_row = row + lane < it.R;
             const uint16_t *g_at = static_cast<const uint16_t *>(prm.g) + at, *u_at = static_cast<const uint16_t *>(prm.u) + at;
             st.acquire();
 #pragma unroll
@@ -253,7 +263,7 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {            // C is a multiple of 8: the eight columns are in or out together
                     g4[k] = u4[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (in_row && col + s * 32 + k * 8 < prm.C) {
+                    if (in_row && col + s * 32 + k * 8 < C) {
                         g4[k] = __ldg(reinterpret_cast<const uint4 *>(g_at + s * 32 + k * 8));
                         u4[k] = __ldg(reinterpret_cast<const uint4 *>(u_at + s * 32 + k * 8));
                     }
@@ -294,17 +304,21 @@ __device__ __forceinline__ void store_partial(const TcParams &prm, uint32_t tmem
     }
 }
 
-// Loads the 128 rows of one operand from `row`, k from `k`.  A transposed operand whose rows are a multiple of 64 is mapped as
-// (64 rows, k, blocks of 64 rows), so that a box holds two blocks; others as (rows, k), one block per box.
+// Where one operand's 128 rows of a stage come from.  A transposed operand whose rows are a multiple of 64 is mapped as (64 rows, k,
+// blocks of 64 rows), so that a box holds two blocks; others as (rows, k), one block per box.  Everything but k is worked out once per
+// tile: the loads are issued by one thread, which has 512 cycles for a stage.
 template <bool MN>
-__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, int row, int k, int boxes, uint32_t bar) {
-    if (!MN) tma_load_3d_pair(dst, map, k, row, 0, bar);
-    else if (boxes == 1) tma_load_3d_pair(dst, map, 0, k, row / 64, bar);
-    else {
-        tma_load_3d_pair(dst, map, row, k, 0, bar);
-        tma_load_3d_pair(dst + kBlockBytes, map, row + 64, k, 0, bar);
+struct Source {
+    const CUtensorMap *map;
+    int32_t row, block;
+    bool two;
+    __device__ __forceinline__ Source(const CUtensorMap *m, int first_row, int boxes)
+        : map(m), row(MN && boxes == 1 ? 0 : first_row), block(MN && boxes == 1 ? first_row / 64 : 0), two(MN && boxes == 2) {}
+    __device__ __forceinline__ void load(uint32_t dst, int k, uint32_t bar) const {
+        tma_load_3d_pair(dst, map, MN ? row : k, MN ? k : row, block, bar);
+        if (MN && two) tma_load_3d_pair(dst + kBlockBytes, map, row + 64, k, 0, bar);
     }
-}
+};
 
 // P_MN / Q_MN: the operand is stored (k, rows) instead of (rows, k).
 template <bool BF16, bool P_MN, bool Q_MN, int EPI, int ACT>
@@ -350,23 +364,31 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool alive = true;
+            const uint32_t leader_bar = map_to_cta(full_bar, 0);
+            // k blocks [begin, end) of one pair of operands
+            auto stream = [&](const Source<P_MN> &p, const Source<Q_MN> &q, int begin, int end) {
+                for (int kb = begin; kb < end; ++kb) {
+                    if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, abort_flag, prm.status, kErrLoad)) return false;
+                    const uint32_t dst = tiles_base + stage * kStageBytes;
+                    if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * kStageBytes);
+                    p.load(dst, kb * kStageK, leader_bar + 8 * stage);
+                    q.load(dst + kPBytes, kb * kStageK, leader_bar + 8 * stage);
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+                return true;
+            };
             Walk<EPI> walk(prm, pair, pairs);
             Item it;
             while (alive && walk.next(it)) {
                 const int p_row = it.row + (int)rank * 128;
                 // gated: the same rows of the rank's weight; otherwise the rank's half of the tile's columns
                 const int q_row = EPI == kEpiGated ? it.col : it.col + (int)rank * 128;
-                for (int kb = it.block; kb < it.block + it.count; ++kb) {
-                    if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, abort_flag, prm.status, kErrLoad)) { alive = false; break; }
-                    const bool second = kb >= prm.blocks0;
-                    const int k = (second ? kb - prm.blocks0 : kb) * kStageK;
-                    const uint32_t dst = tiles_base + stage * kStageBytes;
-                    if (leader) mbar_expect_tx(full_bar + 8 * stage, 2 * kStageBytes);
-                    const uint32_t bar = map_to_cta(full_bar + 8 * stage, 0);
-                    load_rows<P_MN>(dst, &maps.p[second ? 1 : it.product], p_row, k, prm.p_boxes, bar);
-                    load_rows<Q_MN>(dst + kPBytes, &maps.q[EPI == kEpiGated ? (int)rank : second ? 1 : it.product], q_row, k, prm.q_boxes, bar);
-                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
-                }
+                const int end = it.block + it.count;
+                alive = stream(Source<P_MN>(&maps.p[it.product], p_row, it.p_boxes),
+                               Source<Q_MN>(&maps.q[EPI == kEpiGated ? (int)rank : it.product], q_row, it.q_boxes), it.block, min(end, prm.blocks0));
+                if (EPI == kEpiStore && alive && end > prm.blocks0)
+                    alive = stream(Source<P_MN>(&maps.p[1], p_row, it.p_boxes), Source<Q_MN>(&maps.q[1], q_row, it.q_boxes),
+                                   max(it.block - prm.blocks0, 0), end - prm.blocks0);
             }
         }
     } else if (warp == 1) {
@@ -415,7 +437,7 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
             tcgen05_fence_after();
             const int tile_row = (int)rank * 128 + quarter * 32, row = it.row + tile_row;
             const uint32_t tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTileC;
-            if (row < prm.R) {
+            if (row < it.R) {
                 if (it.slot >= 0) store_partial(prm, tmem, it, tile_row, half, lane);
                 else epilogue<BF16, EPI, ACT>(prm, maps, st, tmem, it, row, half);
             }
@@ -456,7 +478,8 @@ __global__ void __launch_bounds__(256) tc_join_kernel(const TcParams prm, void *
     const int row = it.row + tile_row, col = it.col + tile_col;
     const int first = owner_of(prm, t * prm.blocks), last = owner_of(prm, (t + 1) * prm.blocks - 1);
     wait_for_prior_grid();
-    if (row >= prm.R || col >= prm.C) return;
+    const int C = it.C;
+    if (row >= it.R || col >= C) return;
     float a[kJoinColumns], b[EPI == kEpiGated ? kJoinColumns : 1];
 #pragma unroll
     for (int c = 0; c < kJoinColumns; ++c) a[c] = b[EPI == kEpiGated ? c : 0] = 0.f;
@@ -469,12 +492,12 @@ __global__ void __launch_bounds__(256) tc_join_kernel(const TcParams prm, void *
             if (EPI == kEpiGated) b[EPI == kEpiGated ? c : 0] += __ldcg(at + (128 + c) * kTileR);
         }
     }
-    const int64_t to = (int64_t)row * prm.C + col;
+    const int64_t to = (int64_t)row * C + col;
     uint32_t o[3][kJoinColumns / 2];
     if (EPI == kEpiDact) {
 #pragma unroll
         for (int k = 0; k < kJoinColumns / 8; ++k) {
-            if (col + 8 * k >= prm.C) break;
+            if (col + 8 * k >= C) break;
             const uint4 g4 = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(prm.g) + to + 8 * k));
             const uint4 u4 = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(prm.u) + to + 8 * k));
             const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
@@ -494,14 +517,14 @@ __global__ void __launch_bounds__(256) tc_join_kernel(const TcParams prm, void *
             }
         }
     }
-    void *out[3] = {EPI == kEpiStore && it.product ? out1 : out0, EPI == kEpiStore ? nullptr : out1, out2};
+    void *out[3] = {EPI != kEpiStore || it.product == 0 ? out0 : it.product == 1 ? out1 : out2, EPI == kEpiStore ? nullptr : out1, out2};
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         if ((EPI == kEpiStore && k) || (EPI == kEpiDact && k == 2) || !out[k]) break;
         uint4 *p = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out[k]) + to);
 #pragma unroll
         for (int c = 0; c < kJoinColumns / 8; ++c)
-            if (col + 8 * c < prm.C) p[c] = make_uint4(o[k][4 * c], o[k][4 * c + 1], o[k][4 * c + 2], o[k][4 * c + 3]);
+            if (col + 8 * c < C) p[c] = make_uint4(o[k][4 * c], o[k][4 * c + 1], o[k][4 * c + 2], o[k][4 * c + 3]);
     }
 }
 
@@ -531,16 +554,15 @@ bool encode_output(CUtensorMap *map, void *ptr, int64_t R, int64_t C) {
 }
 
 struct Plan {
-    int64_t tiles_r, tiles_c, blocks0, blocks, whole, split_tiles, split_pairs, bytes;
+    int64_t blocks0, blocks, total, whole, split_tiles, split_pairs, bytes;
 };
-// K1: the second pair's k when its product is added (0: none); width: outputs per tile along C.
-Plan plan_of(const DeviceInfo &info, int64_t R, int64_t C, int64_t K0, int64_t K1, int64_t width, int64_t products) {
+// `total` tiles; K1: the second pair's k when its product is added (0: none).
+Plan plan_of(const DeviceInfo &info, int64_t total, int64_t K0, int64_t K1) {
     Plan p;
-    p.tiles_r = ceil_div64(R, kTileR);
-    p.tiles_c = ceil_div64(C, width);
     p.blocks0 = ceil_div64(K0, kStageK);
     p.blocks = p.blocks0 + ceil_div64(K1, kStageK);
-    const int64_t pairs = info.sm_count / 2, total = p.tiles_r * p.tiles_c * products, left = total % pairs;
+    p.total = total;
+    const int64_t pairs = info.sm_count / 2, left = total % pairs;
     // at least eight k blocks per piece; a k block takes a pair 0.3 us, a piece's sums 1/12 us to write and read back, a join 3 us
     const int64_t most = left * p.blocks / 8, split = most < pairs ? most : pairs;
     const bool pays = left > 0 && split > left && 0.3 * p.blocks > 0.3 * left * p.blocks / split + (left + split) / 12.0 + 3.0;
@@ -550,6 +572,8 @@ Plan plan_of(const DeviceInfo &info, int64_t R, int64_t C, int64_t K0, int64_t K
     p.bytes = pays ? (left + split) * kTileR * kTileC * (int64_t)sizeof(float) : 0;
     return p;
 }
+// Tiles of an (R, C) result; width: outputs per tile along C.
+int64_t tiles_of(int64_t R, int64_t C, int64_t width) { return ceil_div64(R, kTileR) * ceil_div64(C, width); }
 
 template <bool BF16, bool P_MN, bool Q_MN, int EPI, int ACT>
 int32_t launch(const Call &call, const TcMaps &maps, TcParams prm, const Plan &plan, void *out0, void *out1, void *out2) {
@@ -567,26 +591,30 @@ int32_t launch(const Call &call, const TcMaps &maps, TcParams prm, const Plan &p
     return CPMK_OK;
 }
 
-int32_t prepare(TcParams *prm, const Plan &plan, int64_t R, int64_t C, void *scratch) {
+int32_t prepare(TcParams *prm, const Plan &plan, void *scratch) {
     uint32_t *status;
     const int32_t rc = get_device_status(&status);
     if (rc) return rc;
     CPMK_REQUIRE(scratch || !plan.bytes, "scratch is needed");
     memset(prm, 0, sizeof(*prm));
-    prm->R = (int32_t)R;
-    prm->C = (int32_t)C;
     prm->blocks0 = (int32_t)plan.blocks0;
     prm->blocks = (int32_t)plan.blocks;
-    prm->tiles_r = (int32_t)plan.tiles_r;
-    prm->tiles_c = (int32_t)plan.tiles_c;
-    prm->per_product = (int32_t)(plan.tiles_r * plan.tiles_c);
     prm->whole = (int32_t)plan.whole;
     prm->split_tiles = (int32_t)plan.split_tiles;
     prm->split_pairs = (int32_t)plan.split_pairs;
-    prm->p_boxes = prm->q_boxes = 1;
     prm->partial = static_cast<float *>(scratch);
     prm->status = status;
     return CPMK_OK;
+}
+void add_product(TcParams *prm, int64_t R, int64_t C, int64_t width, bool p_t, bool q_t) {
+    const int i = prm->products++;
+    prm->R[i] = (int32_t)R;
+    prm->C[i] = (int32_t)C;
+    prm->tiles_r[i] = (int32_t)ceil_div64(R, kTileR);
+    prm->tiles_c[i] = (int32_t)ceil_div64(C, width);
+    prm->first_tile[i] = i ? prm->first_tile[i - 1] + prm->tiles_r[i - 1] * prm->tiles_c[i - 1] : 0;
+    prm->p_boxes[i] = boxes(R, p_t);
+    prm->q_boxes[i] = boxes(C, q_t);
 }
 
 int32_t encode_failed() {
@@ -596,42 +624,65 @@ int32_t encode_failed() {
 
 }  // namespace
 
-int64_t tc_product_scratch(const DeviceInfo &info, int32_t R, int32_t C, int32_t K, bool sum, int32_t products) {
-    return plan_of(info, R, C, K, sum ? K : 0, kTileC, products).bytes;
+int64_t tc_products_scratch(const DeviceInfo &info, int32_t K, const Product *products, int count) {
+    int64_t total = 0;
+    for (int i = 0; i < count; ++i) total += tiles_of(products[i].R, products[i].C, kTileC);
+    return plan_of(info, total, K, 0).bytes;
 }
-int64_t tc_gated_scratch(const DeviceInfo &info, int32_t tokens, int32_t k, int32_t n) { return plan_of(info, tokens, n, k, 0, kTileC / 2, 1).bytes; }
-int64_t tc_dact_scratch(const DeviceInfo &info, int32_t tokens, int32_t n, int32_t m) { return plan_of(info, tokens, n, m, 0, kTileC, 1).bytes; }
+int64_t tc_sum_scratch(const DeviceInfo &info, int32_t R, int32_t C, int32_t K) { return plan_of(info, tiles_of(R, C, kTileC), K, K).bytes; }
+int64_t tc_gated_scratch(const DeviceInfo &info, int32_t tokens, int32_t k, int32_t n) {
+    return plan_of(info, tiles_of(tokens, n, kTileC / 2), k, 0).bytes;
+}
+int64_t tc_dact_scratch(const DeviceInfo &info, int32_t tokens, int32_t n, int32_t m) { return plan_of(info, tiles_of(tokens, n, kTileC), m, 0).bytes; }
 
-int32_t tc_product(const Call &call, int32_t R, int32_t C, int32_t K, bool p_t, bool q_t, const void *p0, const void *q0, const void *p1,
-                   const void *q1, bool sum, void *out0, void *out1, void *scratch) {
-    const Plan plan = plan_of(call.info, R, C, K, sum ? K : 0, kTileC, out1 ? 2 : 1);
+int32_t tc_products(const Call &call, int32_t K, bool transposed, const Product *products, int count, void *scratch) {
+    int64_t total = 0;
+    for (int i = 0; i < count; ++i) total += tiles_of(products[i].R, products[i].C, kTileC);
+    const Plan plan = plan_of(call.info, total, K, 0);
     TcParams prm;
-    const int32_t rc = prepare(&prm, plan, R, C, scratch);
+    const int32_t rc = prepare(&prm, plan, scratch);
     if (rc) return rc;
-    prm.p_boxes = boxes(R, p_t);
-    prm.q_boxes = boxes(C, q_t);
     TcMaps maps;
     memset(&maps, 0, sizeof(maps));
-    bool ok = encode_operand(&maps.p[0], p0, R, K, p_t) && encode_operand(&maps.q[0], q0, C, K, q_t) && encode_output(&maps.out[0], out0, R, C);
-    if (ok && p1) ok = encode_operand(&maps.p[1], p1, R, K, p_t) && encode_operand(&maps.q[1], q1, C, K, q_t);
-    if (ok && out1) ok = encode_output(&maps.out[1], out1, R, C);
-    if (!ok) return encode_failed();
-    const bool bf16 = call.dtype == CPMK_BF16;
-#define CPMK_TC_STORE(P, Q) \
-    return bf16 ? launch<true, P, Q, kEpiStore, 0>(call, maps, prm, plan, out0, out1, nullptr) : launch<false, P, Q, kEpiStore, 0>(call, maps, prm, plan, out0, out1, nullptr)
-    if (!p_t && !q_t) CPMK_TC_STORE(false, false);
-    if (!p_t) CPMK_TC_STORE(false, true);
-    CPMK_REQUIRE(q_t, "operand order not built");
-    CPMK_TC_STORE(true, true);
+    void *out[3] = {nullptr, nullptr, nullptr};
+    for (int i = 0; i < count; ++i) {
+        const Product &p = products[i];
+        add_product(&prm, p.R, p.C, kTileC, transposed, transposed);
+        if (!(encode_operand(&maps.p[i], p.p, p.R, K, transposed) && encode_operand(&maps.q[i], p.q, p.C, K, transposed) &&
+              encode_output(&maps.out[i], p.out, p.R, p.C)))
+            return encode_failed();
+        out[i] = p.out;
+    }
+#define CPMK_TC_STORE(BF16, MN) return launch<BF16, MN, MN, kEpiStore, 0>(call, maps, prm, plan, out[0], out[1], out[2])
+    if (call.dtype == CPMK_BF16 && transposed) CPMK_TC_STORE(true, true);
+    if (call.dtype == CPMK_BF16) CPMK_TC_STORE(true, false);
+    if (transposed) CPMK_TC_STORE(false, true);
+    CPMK_TC_STORE(false, false);
 #undef CPMK_TC_STORE
+}
+
+int32_t tc_sum(const Call &call, int32_t R, int32_t C, int32_t K, const void *p0, const void *q0, const void *p1, const void *q1, void *out, void *scratch) {
+    const Plan plan = plan_of(call.info, tiles_of(R, C, kTileC), K, K);
+    TcParams prm;
+    const int32_t rc = prepare(&prm, plan, scratch);
+    if (rc) return rc;
+    add_product(&prm, R, C, kTileC, false, true);
+    TcMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    if (!(encode_operand(&maps.p[0], p0, R, K, false) && encode_operand(&maps.q[0], q0, C, K, true) && encode_operand(&maps.p[1], p1, R, K, false) &&
+          encode_operand(&maps.q[1], q1, C, K, true) && encode_output(&maps.out[0], out, R, C)))
+        return encode_failed();
+    return call.dtype == CPMK_BF16 ? launch<true, false, true, kEpiStore, 0>(call, maps, prm, plan, out, nullptr, nullptr)
+                                   : launch<false, false, true, kEpiStore, 0>(call, maps, prm, plan, out, nullptr, nullptr);
 }
 
 int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const void *x, const void *wg, const void *wu, void *h, void *g, void *u,
                  void *scratch) {
-    const Plan plan = plan_of(call.info, tokens, n, k, 0, kTileC / 2, 1);
+    const Plan plan = plan_of(call.info, tiles_of(tokens, n, kTileC / 2), k, 0);
     TcParams prm;
-    const int32_t rc = prepare(&prm, plan, tokens, n, scratch);
+    const int32_t rc = prepare(&prm, plan, scratch);
     if (rc) return rc;
+    add_product(&prm, tokens, n, kTileC / 2, false, false);
     prm.g = g;
     prm.u = u;
     TcMaps maps;
@@ -650,11 +701,11 @@ int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const v
 
 int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const void *dy, const void *wd, const void *g, const void *u, void *dg, void *du,
                 void *scratch) {
-    const Plan plan = plan_of(call.info, tokens, n, m, 0, kTileC, 1);
+    const Plan plan = plan_of(call.info, tiles_of(tokens, n, kTileC), m, 0);
     TcParams prm;
-    const int32_t rc = prepare(&prm, plan, tokens, n, scratch);
+    const int32_t rc = prepare(&prm, plan, scratch);
     if (rc) return rc;
-    prm.q_boxes = boxes(n, true);
+    add_product(&prm, tokens, n, kTileC, false, true);
     prm.g = g;
     prm.u = u;
     TcMaps maps;
