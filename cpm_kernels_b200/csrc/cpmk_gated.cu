@@ -70,30 +70,47 @@ __global__ void __launch_bounds__(256) gated_simt_kernel(const SimtParams prm) {
             if (EPI == kEpiStore) {
                 static_cast<T *>(prm.out[0])[at] = from_f32<T>(acc[i][j]);
             } else if (EPI == kEpiGated) {
-                static_cast<T *>(prm.out[0])[at] = from_f32<T>(act_value<ACT>(acc[i][j]) * acc2[i][j]);
+                static_cast<T *>(prm.out[0])[at] = from_f32<T>(both(act_value2<ACT>(f2(acc[i][j]))).x * acc2[i][j]);
                 if (prm.out[1]) {
                     static_cast<T *>(prm.out[1])[at] = from_f32<T>(acc[i][j]);
                     static_cast<T *>(prm.out[2])[at] = from_f32<T>(acc2[i][j]);
                 }
             } else {
-                float value, slope;
-                act_value_slope<ACT>(to_f32(static_cast<const T *>(prm.in[0])[at]), value, slope);
-                static_cast<T *>(prm.out[0])[at] = from_f32<T>(acc[i][j] * to_f32(static_cast<const T *>(prm.in[1])[at]) * slope);
-                static_cast<T *>(prm.out[1])[at] = from_f32<T>(acc[i][j] * value);
+                F2 value, slope;
+                act2<ACT, true>(f2(to_f32(static_cast<const T *>(prm.in[0])[at])), value, slope);
+                static_cast<T *>(prm.out[0])[at] = from_f32<T>(acc[i][j] * to_f32(static_cast<const T *>(prm.in[1])[at]) * both(slope).x);
+                static_cast<T *>(prm.out[1])[at] = from_f32<T>(acc[i][j] * both(value).x);
             }
         }
 }
 
-// dg = dh u act'(g), du = dh act(g) for a dh that lies in memory (the backward pass of the gated linear on its own).
-template <typename T, int ACT>
+// dg = dh u act'(g), du = dh act(g) for a dh that lies in memory (the backward pass of the gated linear on its own): 16 bytes of each
+// tensor per thread where their addresses and the count allow it (VEC = 8), single elements otherwise.
+template <typename T, int ACT, int VEC>
 __global__ void __launch_bounds__(256) gated_dact_kernel(int64_t count, const T *__restrict__ dh, const T *__restrict__ g, const T *__restrict__ u,
                                                          T *__restrict__ dg, T *__restrict__ du) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const float d = to_f32(dh[i]);
-        float value, slope;
-        act_value_slope<ACT>(to_f32(g[i]), value, slope);
-        dg[i] = from_f32<T>(d * to_f32(u[i]) * slope);
-        du[i] = from_f32<T>(d * value);
+    struct alignas(VEC * sizeof(T)) Vector {
+        T v[VEC];
+    };
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC; i < count; i += (int64_t)gridDim.x * 256 * VEC) {
+        const Vector d = *reinterpret_cast<const Vector *>(dh + i), vg = *reinterpret_cast<const Vector *>(g + i), vu = *reinterpret_cast<const Vector *>(u + i);
+        Vector og, ou;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) {
+            constexpr int kNext = VEC > 1 ? 1 : 0;
+            const F2 d2 = f2(to_f32(d.v[e]), to_f32(d.v[e + kNext]));
+            F2 value, slope;
+            act2<ACT, true>(f2(to_f32(vg.v[e]), to_f32(vg.v[e + kNext])), value, slope);
+            const float2 a = both(d2 * f2(to_f32(vu.v[e]), to_f32(vu.v[e + kNext])) * slope), b = both(d2 * value);
+            og.v[e] = from_f32<T>(a.x);
+            ou.v[e] = from_f32<T>(b.x);
+            if (VEC > 1) {
+                og.v[e + kNext] = from_f32<T>(a.y);
+                ou.v[e + kNext] = from_f32<T>(b.y);
+            }
+        }
+        *reinterpret_cast<Vector *>(dg + i) = og;
+        *reinterpret_cast<Vector *>(du + i) = ou;
     }
 }
 
@@ -193,20 +210,20 @@ int32_t dact_product(const Call &call, int32_t tokens, int32_t n, int32_t m, con
     return launch_simt<kEpiDact>(call, prm);
 }
 
+template <typename T, int ACT>
+void launch_dact(const Call &call, int64_t count, const void *dh, const void *g, const void *u, void *dg, void *du) {
+    const bool wide = count % 8 == 0 && aligned16(dh) && aligned16(g) && aligned16(u) && aligned16(dg) && aligned16(du);
+    const int64_t blocks = ceil_div64(count, wide ? 2048 : 256), most = 8 * call.info.sm_count;
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    const T *d = static_cast<const T *>(dh), *a = static_cast<const T *>(g), *b = static_cast<const T *>(u);
+    if (wide) gated_dact_kernel<T, ACT, 8><<<grid, 256, 0, call.stream>>>(count, d, a, b, static_cast<T *>(dg), static_cast<T *>(du));
+    else gated_dact_kernel<T, ACT, 1><<<grid, 256, 0, call.stream>>>(count, d, a, b, static_cast<T *>(dg), static_cast<T *>(du));
+}
+
 int32_t dact(const Call &call, int64_t count, const void *dh, const void *g, const void *u, void *dg, void *du) {
-    const int64_t blocks = ceil_div64(count, 256);
-    const dim3 grid((unsigned)(blocks < 8 * call.info.sm_count ? blocks : 8 * call.info.sm_count));
-#define CPMK_DACT(T, ACT) \
-    gated_dact_kernel<T, ACT><<<grid, 256, 0, call.stream>>>(count, static_cast<const T *>(dh), static_cast<const T *>(g), static_cast<const T *>(u), \
-                                                             static_cast<T *>(dg), static_cast<T *>(du))
-    if (call.dtype == CPMK_F16) {
-        if (call.act == CPMK_ACT_SILU) CPMK_DACT(__half, CPMK_ACT_SILU);
-        else CPMK_DACT(__half, CPMK_ACT_GELU);
-    } else {
-        if (call.act == CPMK_ACT_SILU) CPMK_DACT(__nv_bfloat16, CPMK_ACT_SILU);
-        else CPMK_DACT(__nv_bfloat16, CPMK_ACT_GELU);
-    }
-#undef CPMK_DACT
+    const bool silu = call.act == CPMK_ACT_SILU;
+    if (call.dtype == CPMK_F16) silu ? launch_dact<__half, CPMK_ACT_SILU>(call, count, dh, g, u, dg, du) : launch_dact<__half, CPMK_ACT_GELU>(call, count, dh, g, u, dg, du);
+    else silu ? launch_dact<__nv_bfloat16, CPMK_ACT_SILU>(call, count, dh, g, u, dg, du) : launch_dact<__nv_bfloat16, CPMK_ACT_GELU>(call, count, dh, g, u, dg, du);
     CPMK_LAUNCH_CHECK();
     return CPMK_OK;
 }

@@ -11,29 +11,72 @@ namespace cpmk {
 // the activation
 // ------------------------------------------------------------------------------------------------
 // Both activations are v s(z(v)) with the logistic function s: z = v (silu), z = 2 c (v + 0.044715 v^3), c = sqrt(2 / pi) (gelu:
-// (1 + tanh t) / 2 = s(2 t)).  Derivative: s + v s (1 - s) z'(v).  Beyond |v| = 30 the logistic is 0 or 1 in fp32 (|z| > 1900), so z
+// (1 + tanh t) / 2 = s(2 t)).  Derivative: s + v s (1 - s) z'(v).  Beyond |v| = 30 gelu's logistic is 0 or 1 in fp32 (|z| > 1900), so z
 // and z' are taken of the clamped value: the cube cannot overflow and 0 * inf does not arise.
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-
-template <int ACT>
-__device__ __forceinline__ float act_value(float v) {
-    if (ACT == CPMK_ACT_SILU) return v * logistic(v);
-    const float c = fminf(fmaxf(v, -30.f), 30.f);
-    return v * logistic(1.5957691216057308f * fmaf(0.044715f * c * c, c, c));
+//
+// Two values at a time in packed fp32 arithmetic: the epilogue of a product is bound by the instructions it issues (scalar, the epilogue
+// of dy Wd took 12 us a tile, more than half of what its products take at k = 4096).  s = 1 / (1 + 2^(-z log2 e)) with the hardware's
+// approximate exponential and reciprocal (2^-22 each; the exponential's argument is rounded, 2^-24 of at most 128).
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float2 both(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+// s(z) from -z log2 e
+__device__ __forceinline__ F2 logistic2(F2 minus_z_log2e) {
+    const float2 t = both(minus_z_log2e);
+    float e0, e1, s0, s1;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(t.y));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s0) : "f"(1.f + e0));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s1) : "f"(1.f + e1));
+    return f2(s0, s1);
 }
 
-template <int ACT>
-__device__ __forceinline__ void act_value_slope(float v, float &value, float &slope) {
+constexpr float kLog2e = 1.4426950408889634f, kGeluTwoC = 1.5957691216057308f, kGeluCube = 0.044715f;
+
+// act(v); SLOPE: and act'(v)
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void act2(F2 v, F2 &value, F2 &slope) {
+    F2 s, dz = f2(1.f);
     if (ACT == CPMK_ACT_SILU) {
-        const float s = logistic(v);
-        value = v * s;
-        slope = fmaf(value, 1.f - s, s);
+        s = logistic2(v * f2(-kLog2e));
     } else {
-        const float c = fminf(fmaxf(v, -30.f), 30.f), c2 = c * c;
-        const float s = logistic(1.5957691216057308f * fmaf(0.044715f * c2, c, c));
-        value = v * s;
-        slope = fmaf(value * (1.f - s), 1.5957691216057308f * fmaf(3.f * 0.044715f, c2, 1.f), s);
+        const float2 x = both(v);
+        const F2 c = f2(fminf(fmaxf(x.x, -30.f), 30.f), fminf(fmaxf(x.y, -30.f), 30.f)), c2 = c * c;
+        s = logistic2(c * fma2(c2, f2(-kLog2e * kGeluTwoC * kGeluCube), f2(-kLog2e * kGeluTwoC)));
+        if (SLOPE) dz = fma2(c2, f2(3.f * kGeluTwoC * kGeluCube), f2(kGeluTwoC));
     }
+    value = v * s;
+    if (SLOPE) {
+        const F2 rest = value * fma2(s, f2(-1.f), f2(1.f));          // v s (1 - s)
+        slope = ACT == CPMK_ACT_SILU ? fma2(rest, f2(1.f), s) : fma2(rest, dz, s);
+    }
+}
+template <int ACT>
+__device__ __forceinline__ F2 act_value2(F2 v) {
+    F2 value, slope;
+    act2<ACT, false>(v, value, slope);
+    return value;
 }
 
 // What becomes of a finished sum: stored; with its partner (gate and up) through the activation; as dh through the activation's slope.

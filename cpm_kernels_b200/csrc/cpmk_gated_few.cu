@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(256) few_join_kernel(int32_t tokens, int32_t n
         store4(out + to, a.x, a.y, a.z, a.w);
         return;
     }
-    store4(out + to, act_value<ACT>(a.x) * b.x, act_value<ACT>(a.y) * b.y, act_value<ACT>(a.z) * b.z, act_value<ACT>(a.w) * b.w);
+    const float2 h0 = both(act_value2<ACT>(f2(a.x, a.y)) * f2(b.x, b.y)), h1 = both(act_value2<ACT>(f2(a.z, a.w)) * f2(b.z, b.w));
+    store4(out + to, h0.x, h0.y, h1.x, h1.y);
     if (g_out) {
         store4(g_out + to, a.x, a.y, a.z, a.w);
         store4(u_out + to, b.x, b.y, b.z, b.w);

@@ -135,20 +135,24 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return pack_half2(a, b);
 }
 template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-    if (BF16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v));
-    return __half22float2(*reinterpret_cast<__half2 *>(&v));
+__device__ __forceinline__ uint32_t pack2(F2 v) {
+    const float2 x = both(v);
+    return pack2<BF16>(x.x, x.y);
+}
+template <bool BF16>
+__device__ __forceinline__ F2 unpack2(uint32_t v) {
+    const float2 x = BF16 ? __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v)) : __half22float2(*reinterpret_cast<__half2 *>(&v));
+    return f2(x.x, x.y);
 }
 
 // dg = dh u act'(g), du = dh act(g) for two neighbouring outputs
 template <bool BF16, int ACT>
 __device__ __forceinline__ void dact_pair(float d0, float d1, uint32_t g, uint32_t u, uint32_t &dg, uint32_t &du) {
-    const float2 g2 = unpack2<BF16>(g), u2 = unpack2<BF16>(u);
-    float a0, s0, a1, s1;
-    act_value_slope<ACT>(g2.x, a0, s0);
-    act_value_slope<ACT>(g2.y, a1, s1);
-    dg = pack2<BF16>(d0 * u2.x * s0, d1 * u2.y * s1);
-    du = pack2<BF16>(d0 * a0, d1 * a1);
+    const F2 d = f2(d0, d1);
+    F2 value, slope;
+    act2<ACT, true>(unpack2<BF16>(g), value, slope);
+    dg = pack2<BF16>(d * unpack2<BF16>(u) * slope);
+    du = pack2<BF16>(d * value);
 }
 
 // One warp's staging tiles: 32 rows by 64 columns each, 16-byte chunk j of row r at chunk j ^ (r & 7) (no bank conflicts, and what the
@@ -225,8 +229,8 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 8 * k + 2 * e;
-                    o[e] = pack2<BF16>(act_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]),
-                                       act_value<ACT>(__uint_as_float(g[i + 1])) * __uint_as_float(u[i + 1]));
+                    o[e] = pack2<BF16>(act_value2<ACT>(f2(__uint_as_float(g[i]), __uint_as_float(g[i + 1]))) *
+                                       f2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])));
                 }
                 st.put(0, 4 * s + k, o[0], o[1], o[2], o[3]);
             }
@@ -484,13 +488,24 @@ __global__ void __launch_bounds__(256) tc_join_kernel(const TcParams prm, void *
 #pragma unroll
     for (int c = 0; c < kJoinColumns; ++c) a[c] = b[EPI == kEpiGated ? c : 0] = 0.f;
     const float *at = prm.partial + ((int64_t)(first + t) * kTileC + tile_col) * kTileR + tile_row;
-#pragma unroll 2
-    for (int p = first; p <= last; ++p, at += kTileC * kTileR) {
+    // 32 values in flight per thread: one after the other, a tile of seven pieces took 18 us
+    constexpr int kAhead = EPI == kEpiGated ? 2 : 4;
+    for (int p = first; p <= last; p += kAhead, at += (int64_t)kAhead * kTileC * kTileR) {
+        float v[kAhead][kJoinColumns], w[EPI == kEpiGated ? kAhead : 1][kJoinColumns];
 #pragma unroll
-        for (int c = 0; c < kJoinColumns; ++c) {
-            a[c] += __ldcg(at + c * kTileR);
-            if (EPI == kEpiGated) b[EPI == kEpiGated ? c : 0] += __ldcg(at + (128 + c) * kTileR);
-        }
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int c = 0; c < kJoinColumns; ++c) {
+                v[i][c] = p + i <= last ? __ldcg(at + (int64_t)i * kTileC * kTileR + c * kTileR) : 0.f;
+                if (EPI == kEpiGated) w[EPI == kEpiGated ? i : 0][c] = p + i <= last ? __ldcg(at + (int64_t)i * kTileC * kTileR + (128 + c) * kTileR) : 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int c = 0; c < kJoinColumns; ++c) {
+                a[c] += v[i][c];
+                if (EPI == kEpiGated) b[EPI == kEpiGated ? c : 0] += w[EPI == kEpiGated ? i : 0][c];
+            }
     }
     const int64_t to = (int64_t)row * C + col;
     uint32_t o[3][kJoinColumns / 2];
@@ -509,7 +524,7 @@ __global__ void __launch_bounds__(256) tc_join_kernel(const TcParams prm, void *
         for (int c = 0; c < kJoinColumns; c += 2) {
             if (EPI == kEpiGated) {
                 constexpr int kOne = EPI == kEpiGated ? 1 : 0;
-                o[0][c / 2] = pack2<BF16>(act_value<ACT>(a[c]) * b[c * kOne], act_value<ACT>(a[c + 1]) * b[(c + 1) * kOne]);
+                o[0][c / 2] = pack2<BF16>(act_value2<ACT>(f2(a[c], a[c + 1])) * f2(b[c * kOne], b[(c + 1) * kOne]));
                 o[1][c / 2] = pack2<BF16>(a[c], a[c + 1]);
                 o[2][c / 2] = pack2<BF16>(b[c * kOne], b[(c + 1) * kOne]);
             } else {
