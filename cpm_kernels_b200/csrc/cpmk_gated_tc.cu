@@ -33,12 +33,12 @@ constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kPieces * kP
 constexpr int kTmemColumns = 512;
 constexpr int kBandRows = 16;                          // row tiles walked together (below)
 
-constexpr uint32_t kErrLoad = 0x201, kErrFull = 0x202, kErrAccumulator = 0x203, kErrEpilogue = 0x204;
+constexpr uint32_t kErrLoad = 0x201, kErrFull = 0x202, kErrAccumulator = 0x203, kErrEpilogue = 0x204, kErrInputs = 0x205;
 
 // Boxes of 128 rows by 64 k where one load can have them: with two boxes of 64 rows each the gated product took 489 us instead of 459
 // (4096 x 4096 x 20480).
 struct TcMaps {
-    CUtensorMap p[3], q[3], out[3];
+    CUtensorMap p[3], q[3], out[3], in[2];               // in: g and u (kEpiDact)
 };
 
 // Whole waves of tiles are walked in bands of kBandRows row tiles, row by row within a column of the band: the band's rows of P stay in
@@ -162,6 +162,9 @@ struct Staging {
     __device__ __forceinline__ void put(int piece, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
         st_shared_v4(base + (uint32_t)piece * kPieceBytes + lane * 128u + (((uint32_t)chunk ^ (lane & 7u)) << 4), a, b, c, d);
     }
+    __device__ __forceinline__ uint4 get(int piece, int chunk) const {
+        return ld_shared_v4(base + (uint32_t)piece * kPieceBytes + lane * 128u + (((uint32_t)chunk ^ (lane & 7u)) << 4));
+    }
     // both tiles are free: the stores out of them have read them
     __device__ __forceinline__ void acquire() const {
         if (lane == 0) bulk_wait_read<0>();
@@ -176,31 +179,59 @@ struct Staging {
     }
 };
 
+// The epilogues run in rolled loops of 16 columns: unrolled over a tile they were 60 KB of instructions, which a kernel of one tile per
+// SM fetches as it goes (dy Wd at 201 tokens, k = 512: 19 us, 12 of them the epilogue of its only tile).
+
 // 64 columns of plain sums, from tensor memory column `taddr`
 template <bool BF16>
 __device__ __forceinline__ void stage_sums(const Staging &st, int piece, uint32_t taddr) {
-    uint32_t v[2][32];
-    tmem_ld_32x32b_x32(taddr, v[0]);
-    tmem_ld_32x32b_x32(taddr + 32, v[1]);
-    tmem_ld_wait();
+#pragma unroll 1
+    for (int s = 0; s < 4; ++s) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(taddr + s * 16, v);
+        tmem_ld_wait();
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        for (int k = 0; k < 2; ++k) {
             uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = pack2<BF16>(__uint_as_float(v[s][8 * g + 2 * e]), __uint_as_float(v[s][8 * g + 2 * e + 1]));
-            st.put(piece, 4 * s + g, o[0], o[1], o[2], o[3]);
+            for (int e = 0; e < 4; ++e) o[e] = pack2<BF16>(__uint_as_float(v[8 * k + 2 * e]), __uint_as_float(v[8 * k + 2 * e + 1]));
+            st.put(piece, 2 * s + k, o[0], o[1], o[2], o[3]);
         }
+    }
 }
 
-// A warp's share of a finished accumulator: 32 rows from `row`, and the columns of its half.
+// g and u of a warp's 32 rows by 64 columns, loaded into its two staging tiles, where dg and du replace them.  (Read by each lane from its
+// row in memory, 16 bytes of 32 lines at a time, they kept the SM's load unit busy for 8 thousand cycles a tile.)
+struct DactInputs {
+    uint32_t bar, phase;
+    __device__ __forceinline__ void request(const Staging &st, const TcMaps &maps, int col, int row) const {
+        st.acquire();
+        if (st.lane == 0) {
+            // the tiles were last touched through the generic proxy: order that before the loads that overwrite them
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_expect_tx(bar, 2 * kPieceBytes);
+            tma_load_3d(st.base, &maps.in[0], col, row, 0, bar);
+            tma_load_3d(st.base + kPieceBytes, &maps.in[1], col, row, 0, bar);
+        }
+    }
+    __device__ __forceinline__ bool arrived(const Staging &st, volatile uint32_t *abort_flag, uint32_t *status) {
+        int ok = 1;
+        if (st.lane == 0) ok = mbar_wait(bar, phase, abort_flag, status, kErrInputs) ? 1 : 0;
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        (void)mbar_try_wait(bar, phase);                 // every lane observes the completed phase before it reads the tiles
+        phase ^= 1u;
+        return ok != 0;
+    }
+};
+
+// A warp's share of a finished accumulator: 32 rows from `row`, and the columns of its half.  False: a wait ran out.
 template <bool BF16, int EPI, int ACT>
-__device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps, const Staging &st, uint32_t tmem, const Item &it, int row, int half) {
+__device__ __forceinline__ bool epilogue(const TcParams &prm, const TcMaps &maps, const Staging &st, uint32_t tmem, const Item &it, int row, int half,
+                                         DactInputs &in, volatile uint32_t *abort_flag) {
     const int lane = (int)st.lane, C = it.C;
     if (EPI == kEpiStore) {                              // 128 columns per warp
         const int col = it.col + half * 128;
-        if (col >= C) return;
+        if (col >= C) return true;
         st.acquire();
         stage_sums<BF16>(st, 0, tmem + half * 128);
         const bool second = col + 64 < C;
@@ -214,17 +245,17 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
     } else if (EPI == kEpiGated) {                       // 64 output columns per warp: gate sums, and 128 columns on the up sums
         constexpr int up = 128;
         const int col = it.col + half * 64;
-        if (col >= C) return;
+        if (col >= C) return true;
         const uint32_t gate_at = tmem + half * 64;
         st.acquire();
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            uint32_t g[32], u[32];
-            tmem_ld_32x32b_x32(gate_at + s * 32, g);
-            tmem_ld_32x32b_x32(gate_at + up + s * 32, u);
+#pragma unroll 1
+        for (int s = 0; s < 4; ++s) {
+            uint32_t g[16], u[16];
+            tmem_ld_32x32b_x16(gate_at + s * 16, g);
+            tmem_ld_32x32b_x16(gate_at + up + s * 16, u);
             tmem_ld_wait();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
                 uint32_t o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -232,7 +263,7 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
                     o[e] = pack2<BF16>(act_value2<ACT>(f2(__uint_as_float(g[i]), __uint_as_float(g[i + 1]))) *
                                        f2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])));
                 }
-                st.put(0, 4 * s + k, o[0], o[1], o[2], o[3]);
+                st.put(0, 2 * s + k, o[0], o[1], o[2], o[3]);
             }
         }
         st.ready();
@@ -251,39 +282,29 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
                 bulk_commit();
             }
         }
-    } else {
+    } else {                                             // 128 columns per warp, 64 at a time
+        const int col0 = it.col + half * 128;
+#pragma unroll 1
         for (int p = 0; p < 2; ++p) {
-            const int offset = half * 128 + p * 64;
-            const int col = it.col + offset;
-            if (col >= C) return;
-            const int64_t at = (int64_t)(row + lane) * C + col;
-            const bool in_row = row + lane < it.R;
-            const uint16_t *g_at = static_cast<const uint16_t *>(prm.g) + at, *u_at = static_cast<const uint16_t *>(prm.u) + at;
-            st.acquire();
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                uint32_t v[32];
-                uint4 g4[4], u4[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {            // C is a multiple of 8: the eight columns are in or out together
-                    g4[k] = u4[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (in_row && col + s * 32 + k * 8 < C) {
-                        g4[k] = __ldg(reinterpret_cast<const uint4 *>(g_at + s * 32 + k * 8));
-                        u4[k] = __ldg(reinterpret_cast<const uint4 *>(u_at + s * 32 + k * 8));
-                    }
-                }
-                tmem_ld_32x32b_x32(tmem + offset + s * 32, v);
+            const int col = col0 + p * 64;
+            if (col >= C) break;
+            if (p) in.request(st, maps, col, row);       // the first were requested before the sums were there
+            if (!in.arrived(st, abort_flag, prm.status)) return false;
+#pragma unroll 1
+            for (int s = 0; s < 4; ++s) {
+                uint32_t v[16];
+                tmem_ld_32x32b_x16(tmem + half * 128 + p * 64 + s * 16, v);
+                const uint4 g4[2] = {st.get(0, 2 * s), st.get(0, 2 * s + 1)}, u4[2] = {st.get(1, 2 * s), st.get(1, 2 * s + 1)};
                 tmem_ld_wait();
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < 2; ++k) {
                     const uint32_t gw[4] = {g4[k].x, g4[k].y, g4[k].z, g4[k].w}, uw[4] = {u4[k].x, u4[k].y, u4[k].z, u4[k].w};
                     uint32_t dg[4], du[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int e = 0; e < 4; ++e)
                         dact_pair<BF16, ACT>(__uint_as_float(v[8 * k + 2 * e]), __uint_as_float(v[8 * k + 2 * e + 1]), gw[e], uw[e], dg[e], du[e]);
-                    }
-                    st.put(0, 4 * s + k, dg[0], dg[1], dg[2], dg[3]);
-                    st.put(1, 4 * s + k, du[0], du[1], du[2], du[3]);
+                    st.put(0, 2 * s + k, dg[0], dg[1], dg[2], dg[3]);
+                    st.put(1, 2 * s + k, du[0], du[1], du[2], du[3]);
                 }
             }
             st.ready();
@@ -294,17 +315,19 @@ __device__ __forceinline__ void epilogue(const TcParams &prm, const TcMaps &maps
             }
         }
     }
+    return true;
 }
 
 // A warp's share of a piece's partial sums: its 32 rows, its 128 accumulator columns; a column's 32 rows are 128 bytes.
 __device__ __forceinline__ void store_partial(const TcParams &prm, uint32_t tmem, const Item &it, int tile_row, int half, int lane) {
     float *to = prm.partial + ((int64_t)it.slot * kTileC + half * 128) * kTileR + tile_row + lane;
-    for (int s = 0; s < 4; ++s, to += 32 * kTileR) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem + half * 128 + s * 32, v);
+#pragma unroll 1
+    for (int s = 0; s < 8; ++s, to += 16 * kTileR) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem + half * 128 + s * 16, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 32; ++c) __stcg(to + c * kTileR, __uint_as_float(v[c]));
+        for (int c = 0; c < 16; ++c) __stcg(to + c * kTileR, __uint_as_float(v[c]));
     }
 }
 
@@ -335,7 +358,8 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
     const uint32_t empty_bar = full_bar + 8 * kStages;
     const uint32_t acc_full_bar = empty_bar + 8 * kStages;
     const uint32_t acc_empty_bar = acc_full_bar + 16;                                    // used in the leader only
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_raw + (acc_empty_bar + 16 - smem_u32(smem_raw)));
+    const uint32_t in_bar = acc_empty_bar + 16;                                          // one per epilogue warp
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_raw + (in_bar + 8 * kEpilogueWarps - smem_u32(smem_raw)));
     volatile uint32_t *abort_flag = tmem_slot + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -353,6 +377,7 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
             mbar_init(acc_full_bar + 8 * a, 1);
             mbar_init(acc_empty_bar + 8 * a, 2 * kEpilogueWarps);                        // the epilogue warps of both CTAs
         }
+        for (int w = 0; w < kEpilogueWarps; ++w) mbar_init(in_bar + 8 * w, 1);
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -434,16 +459,18 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const Staging st = {staging_base + (uint32_t)(warp - 2) * kPieces * kPieceBytes, (uint32_t)lane};
         uint32_t acc = 0, acc_phase = 0;
+        DactInputs in = {in_bar + 8 * (uint32_t)(warp - 2), 0u};
         Walk<EPI> walk(prm, pair, pairs);
         Item it;
         while (walk.next(it)) {
+            const int tile_row = (int)rank * 128 + quarter * 32, row = it.row + tile_row;
+            if (EPI == kEpiDact && it.slot < 0 && row < it.R && it.col + half * 128 < it.C) in.request(st, maps, it.col + half * 128, row);
             if (!mbar_wait(acc_full_bar + 8 * acc, acc_phase, abort_flag, prm.status, kErrEpilogue)) break;
             tcgen05_fence_after();
-            const int tile_row = (int)rank * 128 + quarter * 32, row = it.row + tile_row;
             const uint32_t tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTileC;
             if (row < it.R) {
                 if (it.slot >= 0) store_partial(prm, tmem, it, tile_row, half, lane);
-                else epilogue<BF16, EPI, ACT>(prm, maps, st, tmem, it, row, half);
+                else if (!epilogue<BF16, EPI, ACT>(prm, maps, st, tmem, it, row, half, in, abort_flag)) break;
             }
             tcgen05_fence_before();
             __syncwarp();
@@ -561,8 +588,8 @@ bool encode_operand(CUtensorMap *map, const void *ptr, int64_t rows, int64_t k, 
     return encode_tiled_3d(map, 2, ptr, dims, strides, box, true);
 }
 int32_t boxes(int64_t rows, bool transposed) { return transposed && rows % 64 ? 2 : 1; }
-// An output (R, C): boxes of 32 rows by 64 columns.
-bool encode_output(CUtensorMap *map, void *ptr, int64_t R, int64_t C) {
+// An output (or g, u), (R, C): boxes of 32 rows by 64 columns.
+bool encode_output(CUtensorMap *map, const void *ptr, int64_t R, int64_t C) {
     const uint64_t dims[3] = {(uint64_t)C, (uint64_t)R, 1}, strides[2] = {(uint64_t)C * 2, (uint64_t)R * (uint64_t)C * 2};
     const uint32_t box[3] = {64, 32, 1};
     return encode_tiled_3d(map, 2, ptr, dims, strides, box, true);
@@ -726,7 +753,7 @@ int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const vo
     TcMaps maps;
     memset(&maps, 0, sizeof(maps));
     if (!(encode_operand(&maps.p[0], dy, tokens, m, false) && encode_operand(&maps.q[0], wd, n, m, true) && encode_output(&maps.out[0], dg, tokens, n) &&
-          encode_output(&maps.out[1], du, tokens, n)))
+          encode_output(&maps.out[1], du, tokens, n) && encode_output(&maps.in[0], g, tokens, n) && encode_output(&maps.in[1], u, tokens, n)))
         return encode_failed();
 #define CPMK_TC_DACT(BF16, ACT) return launch<BF16, false, true, kEpiDact, ACT>(call, maps, prm, plan, dg, du, nullptr)
     if (call.dtype == CPMK_BF16 && call.act == CPMK_ACT_SILU) CPMK_TC_DACT(true, CPMK_ACT_SILU);
