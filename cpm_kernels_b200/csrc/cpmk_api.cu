@@ -108,30 +108,35 @@ int32_t get_workspace(cudaStream_t stream, Workspace *ws) {
     return CPMK_OK;
 }
 
-static std::map<int, uint32_t *> g_device_status;
+constexpr int kMaxDevices = 64;
+static uint32_t *g_device_status[kMaxDevices];
 
 int32_t get_device_status(uint32_t **status) {
     int dev = 0;
     CPMK_CUDA_TRY(cudaGetDevice(&dev));
+    CPMK_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d is beyond the %d this library keeps a status word for", dev, kMaxDevices);
     std::lock_guard<std::mutex> lock(g_mutex);
-    auto it = g_device_status.find(dev);
-    if (it == g_device_status.end()) {
+    if (!g_device_status[dev]) {
         void *p = nullptr;
         CPMK_CUDA_TRY(cudaMalloc(&p, 256));
-        CPMK_CUDA_TRY(cudaMemset(p, 0, 256));
-        it = g_device_status.emplace(dev, static_cast<uint32_t *>(p)).first;
+        const cudaError_t e = cudaMemset(p, 0, 256);
+        if (e != cudaSuccess) {
+            (void)cudaFree(p);
+            set_error("clearing the device's status word failed: %s", cudaGetErrorString(e));
+            return CPMK_ECUDA;
+        }
+        g_device_status[dev] = static_cast<uint32_t *>(p);
     }
-    *status = it->second;
+    *status = g_device_status[dev];
     return CPMK_OK;
 }
 
 // Reads and clears the device's status word (0 when it has none yet).  The caller holds g_mutex and has synchronised.
 static int32_t collect_device_status(int dev, uint32_t *word) {
     *word = 0;
-    auto it = g_device_status.find(dev);
-    if (it == g_device_status.end()) return CPMK_OK;
-    CPMK_CUDA_TRY(cudaMemcpy(word, it->second, sizeof(*word), cudaMemcpyDeviceToHost));
-    if (*word != 0) CPMK_CUDA_TRY(cudaMemset(it->second, 0, 256));
+    if (dev < 0 || dev >= kMaxDevices || !g_device_status[dev]) return CPMK_OK;
+    CPMK_CUDA_TRY(cudaMemcpy(word, g_device_status[dev], sizeof(*word), cudaMemcpyDeviceToHost));
+    if (*word != 0) CPMK_CUDA_TRY(cudaMemset(g_device_status[dev], 0, 256));
     return CPMK_OK;
 }
 

@@ -230,12 +230,21 @@ int32_t dact(const Call &call, int64_t count, const void *dh, const void *g, con
 
 bool even_address(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 
+// Every extent fits an int with room for a tile beside it.
+int32_t check_sizes(int32_t tokens, int32_t k, int32_t n, int32_t m) {
+    constexpr int32_t kMost = 1 << 30;
+    CPMK_REQUIRE(tokens >= 0 && tokens <= kMost && k >= 1 && k <= kMost && n >= 1 && n <= kMost && m >= 1 && m <= kMost,
+                 "bad size: tokens=%d k=%d n=%d m=%d (at most 2^30)", tokens, k, n, m);
+    return CPMK_OK;
+}
+
 int32_t begin(Call *call, int32_t tokens, int32_t k, int32_t n, int32_t m, int32_t dtype, int32_t act, cpmk_stream_t stream) {
     const int32_t rc = current_device_info(&call->info);
     if (rc) return rc;
     // a thread whose first CUDA call this is (autograd's) has no context yet, and encoding a tensor map fails without one
     CPMK_CUDA_TRY(cudaSetDevice(call->info.device));
-    CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 1, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
+    const int32_t rc_sizes = check_sizes(tokens, k, n, m);
+    if (rc_sizes) return rc_sizes;
     CPMK_REQUIRE(dtype == CPMK_F16 || dtype == CPMK_BF16, "the gated block takes fp16 and bf16 (dtype %d)", dtype);
     CPMK_REQUIRE(act == CPMK_ACT_GELU || act == CPMK_ACT_SILU, "unknown activation %d", act);
     call->dtype = dtype;
@@ -287,9 +296,11 @@ extern "C" {
 
 int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int64_t *bytes) {
     DeviceInfo info;
-    const int32_t rc = current_device_info(&info);
+    int32_t rc = current_device_info(&info);
     if (rc) return rc;
-    CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 0 && bytes, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
+    rc = check_sizes(tokens, k, n, m > 0 ? m : 1);
+    if (rc) return rc;
+    CPMK_REQUIRE(m >= 0 && bytes, "bad arguments: m=%d", m);
     int64_t need = 0;
     if (tokens > 0 && tensor_core_size(n)) {
         const bool down = m > 0 && tensor_core_size(m), first = tensor_core_size(k);
@@ -305,9 +316,11 @@ int32_t cpmk_gated_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int6
 
 int32_t cpmk_gated_backward_scratch(int32_t tokens, int32_t k, int32_t n, int32_t m, int64_t *bytes) {
     DeviceInfo info;
-    const int32_t rc = current_device_info(&info);
+    int32_t rc = current_device_info(&info);
     if (rc) return rc;
-    CPMK_REQUIRE(tokens >= 0 && k >= 1 && n >= 1 && m >= 0 && bytes, "bad size: tokens=%d k=%d n=%d m=%d", tokens, k, n, m);
+    rc = check_sizes(tokens, k, n, m > 0 ? m : 1);
+    if (rc) return rc;
+    CPMK_REQUIRE(m >= 0 && bytes, "bad arguments: m=%d", m);
     int64_t need = 0;
     if (tokens > 0 && tensor_core_size(n)) {
         const bool down = m > 0 && tensor_core_size(m);

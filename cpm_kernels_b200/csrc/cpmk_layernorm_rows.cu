@@ -501,12 +501,12 @@ int backward_blocks(const DeviceInfo &info, int32_t rows, int32_t n) {
     const int64_t blocks = ceil_div64(rows, warps ? 32 : 4), most = (int64_t)info.sm_count * (threads >= 512 ? 1 : 512 / threads);
     return (int)(blocks < most ? blocks : most);
 }
-int32_t column_pitch(int32_t n) { return (n + 31) / 32 * 32; }         // (n < 2^31 - 32: checked)
+int32_t column_pitch(int32_t n) { return (n + 31) / 32 * 32; }
 
 int32_t check_common(DeviceInfo *info, int32_t rows, int32_t n, int32_t dtype) {
     const int32_t rc = current_device_info(info);
     if (rc) return rc;
-    CPMK_REQUIRE(rows >= 0 && n >= 1 && n <= 0x7fffffff - 32, "bad size: rows=%d n=%d", rows, n);
+    CPMK_REQUIRE(rows >= 0 && n >= 1 && n <= (1 << 30), "bad size: rows=%d n=%d (at most 2^30)", rows, n);
     CPMK_REQUIRE(dtype == CPMK_F16 || dtype == CPMK_BF16 || dtype == CPMK_F32, "unknown element type %d", dtype);
     return CPMK_OK;
 }
@@ -552,13 +552,16 @@ int32_t backward_rows(const DeviceInfo &info, int blocks, int32_t rows, int32_t 
     const float inv_n = 1.f / (float)n;
     const int32_t pitch = column_pitch(n);
     const int64_t sums = COLUMNS ? 2 * (int64_t)n * (int64_t)sizeof(float) : 0;
-    const bool fits = sums <= info.max_smem_optin - 1024;                        // the kernels' static arrays take half a KiB
+    // the kernels' static arrays take half a KiB; the attribute is the same for every size, so that two threads' calls cannot undo each
+    // other's
+    const int64_t smem_most = info.max_smem_optin - 1024;
+    const bool fits = sums <= smem_most;
     if (l.threads == 1024 && !fits) l = {1, 0, 0};
 #define CPMK_LN_BACKWARD(VEC, NV, BLOCK, THREADS, SMEM) \
     ln_rows_backward_kernel<T, VEC, NV, BLOCK, COLUMNS><<<blocks, THREADS, SMEM, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch)
 #define CPMK_LN_BACKWARD_LONG(VEC, NV) \
     { \
-        if (COLUMNS) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums)); \
+        if (COLUMNS) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_most)); \
         ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS><<<blocks, 1024, sums, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch); \
     }
 #define CPMK_LN_BACKWARD_IF(VEC, EACH) \
@@ -569,7 +572,7 @@ int32_t backward_rows(const DeviceInfo &info, int blocks, int32_t rows, int32_t 
     else if (l.vec == VEC) CPMK_LN_BACKWARD(VEC, 2 * EACH, true, l.threads, 0);
     if (l.threads == 0) {
         const int in_smem = COLUMNS && fits;
-        if (in_smem) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_wide_kernel<T, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums));
+        if (in_smem) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_wide_kernel<T, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_most));
         ln_rows_backward_wide_kernel<T, COLUMNS><<<blocks, 1024, in_smem ? sums : 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch,
                                                                                               in_smem);
     }

@@ -17,7 +17,7 @@ def layernorm_rows_forward(rows: int, n: int, dtype: int,
                            stream: CUDAStream):
     """y = (x - mean) * rstd * weight + bias per row; ``rd_mean`` False: mean = 0 (the RMS form)."""
     assert rows >= 0 and n >= 1
-    cpmk.call("cpmk_layernorm_rows_forward", rows, n, dtype, x, eps, 1 if rd_mean else 0, weight, bias, y, mean, rstd, stream_arg(stream))
+    cpmk.call("cpmk_layernorm_rows_forward", rows, n, dtype, x, float(eps), 1 if rd_mean else 0, weight, bias, y, mean, rstd, stream_arg(stream))
 
 
 def layernorm_rows_backward_scratch(rows: int, n: int) -> int:

@@ -16,7 +16,7 @@ def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation
     dtype, device = x.dtype, x.device
     assert x.is_cuda and x.is_contiguous() and x.ndim >= 1 and dtype in _DTYPES
     k, n = x.size(-1), w_gate.size(0)
-    assert k >= 1 and n >= 1 and x.numel() // k < 2 ** 31
+    assert k >= 1 and n >= 1 and x.numel() // k <= 2 ** 30
     assert w_gate.device == device and w_gate.dtype == dtype and w_gate.shape == (n, k) and w_gate.is_contiguous()
     assert w_up.device == device and w_up.dtype == dtype and w_up.shape == (n, k) and w_up.is_contiguous()
     assert activation in cpmk.ACTIVATIONS

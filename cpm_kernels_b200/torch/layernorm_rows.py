@@ -62,7 +62,7 @@ def layernorm_rows(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Opti
     dtype, device = x.dtype, x.device
     assert x.is_cuda and x.is_contiguous() and x.ndim >= 1 and dtype in _DTYPES
     n = x.size(-1)
-    assert n >= 1 and x.numel() // n < 2 ** 31
+    assert 1 <= n <= 2 ** 30 and x.numel() // n < 2 ** 31
     assert eps >= 0
     assert weight.device == device and weight.dtype == dtype and weight.shape == (n,) and weight.is_contiguous()
     assert bias is None or (bias.device == device and bias.dtype == dtype and bias.shape == (n,) and bias.is_contiguous())

@@ -30,3 +30,27 @@ def test_launchers_check_sizes():
         ck.gated_feed_forward_forward(1, 8, 8, 0, cpmk.F16, 0, *([0] * 9), 0)
     with pytest.raises(AssertionError):
         ck.gated_feed_forward_backward(-1, 8, 8, 8, cpmk.F16, 0, *([0] * 15), 0)
+
+
+def test_the_launch_follows_the_tensors_device(monkeypatch):
+    """``launch`` makes the tensors' device current for the call when another one is, and hands on that device's stream."""
+    from cpm_kernels_b200.torch import _launch
+    entered = []
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+
+        def __exit__(self, *a):
+            entered.append(None)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(_launch, "_raw_stream", lambda device: 1000 + device)
+    body = lambda *a: (a, list(entered))
+    assert _launch.launch(0, body, 5) == ((5, 1000), [])
+    assert _launch.launch(1, body, 5, 6) == ((5, 6, 1001), [1])
+    assert entered == [1, None]

@@ -354,7 +354,8 @@ def test_refusals():
     h = torch.empty((4, 24), device="cuda", dtype=torch.half)
     for args in ((4, 16, 24, cpmk.F32, 0, p(x), p(wg), p(wu), p(h), 0, 0, 0, s), (4, 16, 24, 0, 5, p(x), p(wg), p(wu), p(h), 0, 0, 0, s),
                  (4, 16, 24, 0, 0, 0, p(wg), p(wu), p(h), 0, 0, 0, s), (4, 16, 24, 0, 0, p(x), p(wg), p(wu), p(h), p(h), 0, 0, s),
-                 (4, 16, 24, 0, 0, p(x) + 1, p(wg), p(wu), p(h), 0, 0, 0, s)):
+                 (4, 16, 24, 0, 0, p(x) + 1, p(wg), p(wu), p(h), 0, 0, 0, s), (2 ** 30 + 1, 16, 24, 0, 0, p(x), p(wg), p(wu), p(h), 0, 0, 0, s),
+                 (4, 16, 24, 0, 0, p(x), p(wg), p(wu), p(h), 0, 0, 0, s), (4, 16, 24, 0, 0, p(x), p(wg), p(wu), p(h), 0, 0, p(x) + 8, s)):
         with pytest.raises(RuntimeError):
             ck.gated_linear_forward(*args)
 

@@ -234,7 +234,8 @@ def test_refusals():
     s = torch.cuda.current_stream().cuda_stream
     for args in ((4, 16, 9, x.data_ptr(), EPS, True, w.data_ptr(), 0, x.data_ptr(), 0, 0, s), (4, 16, 0, 0, EPS, True, w.data_ptr(), 0, x.data_ptr(), 0, 0, s),
                  (4, 16, 0, x.data_ptr() + 1, EPS, True, w.data_ptr(), 0, x.data_ptr(), 0, 0, s),
-                 (4, 16, 0, x.data_ptr(), EPS, True, w.data_ptr(), 0, x.data_ptr(), x.data_ptr(), 0, s)):
+                 (4, 16, 0, x.data_ptr(), EPS, True, w.data_ptr(), 0, x.data_ptr(), x.data_ptr(), 0, s),
+                 (1, 2 ** 30 + 8, 0, x.data_ptr(), EPS, True, w.data_ptr(), 0, x.data_ptr(), 0, 0, s)):
         with pytest.raises(RuntimeError):
             ck.layernorm_rows_forward(*args)
     y = ct.layernorm_rows(x.requires_grad_(), EPS, w)
