@@ -1,5 +1,6 @@
 """Builds ``lib/libcpmk_b200.so`` from ``csrc/*.cu`` and the loadable kernel modules ``lib/gemm.fatbin`` /
-``lib/gemv.fatbin`` from ``csrc/modules/*_module.cu`` with nvcc for sm_100a (cross-compiles without a GPU).
+``lib/gemv.fatbin`` from ``csrc/modules/*_module.cu`` with nvcc for sm_100a (cross-compiles without a GPU), and the autograd module
+``lib/cpmk_torch.so`` from ``csrc/torch/ffn.cpp`` with the host compiler.
 
 Usage: ``python -m cpm_kernels_b200.build [--force] [--verbose]``
 """
@@ -23,6 +24,9 @@ NVCC_FLAGS = [
 ]
 
 
+EXT_PATH = os.path.join(LIB_DIR, "cpmk_torch.so")
+EXT_SOURCE = os.path.join(CSRC, "torch", "ffn.cpp")
+
 MODULES = {"gemm": "gemm_module.cu", "gemv": "gemv_module.cu", "transpose": "transpose_module.cu"}
 MODULE_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-fatbin"]
 
@@ -43,7 +47,29 @@ def _inputs() -> list[str]:
         glob.glob(os.path.join(root, "include", "*.h")) + glob.glob(os.path.join(CSRC, "modules", "*"))
 
 
+def _ext_inputs() -> list[str]:
+    return [EXT_SOURCE] + glob.glob(os.path.join(os.path.dirname(_PKG), "include", "*.h"))
+
+
+def _ext_is_stale() -> bool:
+    return not os.path.exists(EXT_PATH) or any(os.path.getmtime(p) > os.path.getmtime(EXT_PATH) for p in _ext_inputs())
+
+
+def _ext_command() -> list[str]:
+    """The host compiler's command for the autograd module, against the installed PyTorch's headers and libraries."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=cpmk_torch",
+            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] + ["-I" + i for i in include] + \
+        ["-o", EXT_PATH, EXT_SOURCE, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
+
+
 def is_stale() -> bool:
+    if _ext_is_stale():
+        return True
     if not os.path.exists(LIB_PATH) or not all(os.path.exists(module_path(n)) for n in MODULES):
         return True
     built = os.path.getmtime(LIB_PATH)
@@ -56,6 +82,21 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "nvcc")
     os.makedirs(LIB_DIR, exist_ok=True)
+    # the autograd module is compiled beside the library
+    ext_cmd = _ext_command() if force or _ext_is_stale() else None
+    ext = subprocess.Popen(ext_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) if ext_cmd else None
+    try:
+        _compile_cuda(nvcc, verbose)
+    finally:
+        ext_out = ext.communicate()[0] if ext else ""
+    if ext and ext.returncode != 0:
+        raise RuntimeError("%s failed:\n%s\n%s" % (ext_cmd[0], " ".join(ext_cmd), ext_out))
+    # the library is written first, so a stale check against its time stamp also covers the modules
+    os.utime(LIB_PATH, None)
+    return LIB_PATH
+
+
+def _compile_cuda(nvcc: str, verbose: bool) -> None:
     cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB_PATH] + sources()
     proc = subprocess.run(cmd, cwd=CSRC, capture_output=True, text=True)
     if verbose:
@@ -69,9 +110,6 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
             sys.stderr.write(proc.stderr)
         if proc.returncode != 0:
             raise RuntimeError("nvcc failed:\n%s\n%s" % (" ".join(cmd), proc.stderr))
-    # the library is written first, so a stale check against its time stamp also covers the modules
-    os.utime(LIB_PATH, None)
-    return LIB_PATH
 
 
 if __name__ == "__main__":

@@ -32,25 +32,19 @@ def test_launchers_check_sizes():
         ck.gated_feed_forward_backward(-1, 8, 8, 8, cpmk.F16, 0, *([0] * 15), 0)
 
 
-def test_the_launch_follows_the_tensors_device(monkeypatch):
-    """``launch`` makes the tensors' device current for the call when another one is, and hands on that device's stream."""
-    from cpm_kernels_b200.torch import _launch
-    entered = []
+def test_the_autograd_module_is_built_and_takes_every_entry_point(built_library):
+    from cpm_kernels_b200 import build
+    from cpm_kernels_b200.torch import _ext
+    import os
+    assert os.path.getsize(build.EXT_PATH) > 0
+    with pytest.raises(RuntimeError):
+        _ext.ext.bind([0])
+    for name in _ext._ENTRY_POINTS[1:]:
+        assert name in cpmk.SIGNATURES
 
-    class Guard:
-        def __init__(self, device):
-            self.device = device
 
-        def __enter__(self):
-            entered.append(self.device)
-
-        def __exit__(self, *a):
-            entered.append(None)
-
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(torch.cuda, "device", Guard)
-    monkeypatch.setattr(_launch, "_raw_stream", lambda device: 1000 + device)
-    body = lambda *a: (a, list(entered))
-    assert _launch.launch(0, body, 5) == ((5, 1000), [])
-    assert _launch.launch(1, body, 5, 6) == ((5, 6, 1001), [1])
-    assert entered == [1, None]
+def test_a_missing_autograd_module_fails_loudly(monkeypatch, tmp_path):
+    from cpm_kernels_b200.torch import _ext
+    monkeypatch.setattr(_ext, "EXT_PATH", str(tmp_path / "nope.so"))
+    with pytest.raises(RuntimeError, match="no fallback"):
+        _ext._load()
