@@ -128,8 +128,12 @@ def test_gated_feed_forward(tokens, k, n, m, name):
     assert cpmk.read_status() == 0
 
 
+# whole layers; sums that are cut along k: of every product (600 tokens), of left-over tiles behind whole waves (2304), of the three weight
+# gradients together (5000, 3001)
 @pytest.mark.parametrize("tokens,k,n,m,name", [(1, 4096, 10240, 4096, "fp16"), (48, 4096, 10240, 4096, "bf16"), (700, 4096, 1024, 2048, "bf16"),
-                                               (1500, 1024, 4096, 1024, "fp16")])
+                                               (1500, 1024, 4096, 1024, "fp16"), (600, 4096, 512, 4096, "fp16"), (2304, 64, 4096, 2560, "bf16"),
+                                               (5000, 256, 264, 520, "bf16"), (3001, 64, 136, 72, "fp16"), (256, 2048, 1368, 2048, "fp16"),
+                                               (257, 2048, 1368, 2048, "fp16")])
 def test_wide_layers(tokens, k, n, m, name):
     x, wg, wu, wd, dy, _ = make(tokens, k, n, m, TYPES[name], 5)
     ts = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
