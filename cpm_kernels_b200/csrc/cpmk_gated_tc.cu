@@ -44,7 +44,7 @@ struct TcMaps {
 // Whole waves of tiles are walked in bands of kBandRows row tiles, row by row within a column of the band: the band's rows of P stay in
 // L2 while the columns pass by (4096 tokens, gated: bands of 4, 8, 16 rows took 476, 459, 447 us).  The tiles that are left over (all
 // of them, when there are fewer tiles than pairs) would occupy a part of the SMs for the time of a whole tile.  Where that costs more
-// than it takes to join sums (split_pays), their k blocks form one list that is cut into equal pieces, one per pair; a piece leaves
+// than it takes to join sums (plan_of), their k blocks form one list that is cut into equal pieces, one per pair; a piece leaves
 // fp32 partial sums in scratch, tc_join_kernel adds a tile's pieces in order of k and finishes its outputs.
 struct TcParams {
     // up to three products of the same k in one launch (kEpiStore): the weights' gradients

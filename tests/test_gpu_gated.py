@@ -255,6 +255,24 @@ def test_a_thread_that_has_not_used_the_device(tokens):
     assert len(got) == 1 and torch.equal(got[0], want)
 
 
+def test_offsets_beyond_32_bits():
+    """2.2e9 hidden activations: rows at both ends and around the 2^31st element against the same rows among 300 of their own."""
+    tokens, k, n, m = 262_200, 64, 8200, 64
+    x, wg, wu, wd, dy, _ = make(tokens, k, n, m, torch.half, 15)
+    x.requires_grad_()
+    y = ct.gated_feed_forward(x, wg, wu, wd)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    h = ct.gated_linear(x.detach(), wg, wu)
+    for at in (0, 2 ** 31 // n - 150, tokens - 300):
+        part = x.detach()[at:at + 300].clone().requires_grad_()
+        z = ct.gated_feed_forward(part, wg, wu, wd)
+        (dpart,) = torch.autograd.grad(z, part, dy[at:at + 300].clone())
+        # other tiles are cut along k than in the large call: a step of fp16 apart, 2^-8 below 8 and 2^-6 below 32
+        assert torch.equal(ct.gated_linear(part.detach(), wg, wu), h[at:at + 300])
+        assert (z - y[at:at + 300]).abs().max() <= 2.0 ** -8 and (dpart - dx[at:at + 300]).abs().max() <= 2.0 ** -6
+    Exact(x.detach()[-40:], wg, wu, "gelu", wd, dy[-40:]).check(y[-40:], "y", 2)
+
+
 def test_the_same_tensor_as_both_weights():
     x, wg, _, _, _, dh = make(40, 64, 64, 64, torch.half, 7)
     a, b = wg.clone().requires_grad_(), wg.clone().requires_grad_()

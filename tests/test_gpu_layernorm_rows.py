@@ -186,6 +186,24 @@ def test_nothing_is_written_outside_the_outputs(rows, n):
         check(got, v, e, "fp16", what)
 
 
+def test_offsets_beyond_32_bits():
+    """2.2e9 elements per tensor: the rows at both ends and around the 2^31st element against the same rows on their own."""
+    rows, n = 1_050_000, 2056
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.empty((rows, n), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    dy = torch.empty_like(x).normal_(generator=g)
+    w = torch.ones(n, dtype=torch.bfloat16, device="cuda") * 1.5
+    x.requires_grad_()
+    y = ct.layernorm_rows(x, EPS, w)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    middle = 2 ** 31 // n
+    for at in (0, middle - 2, rows - 4):
+        part = x.detach()[at:at + 4].clone().requires_grad_()
+        z = ct.layernorm_rows(part, EPS, w)
+        assert torch.equal(z, y[at:at + 4])
+        assert torch.equal(torch.autograd.grad(z, part, dy[at:at + 4].clone())[0], dx[at:at + 4])
+
+
 def test_same_bits_on_every_run_and_stream():
     x, w, b, dy = make(3000, 1024, torch.bfloat16, 8)
     results = []
