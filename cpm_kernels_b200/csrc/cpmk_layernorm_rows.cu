@@ -17,6 +17,12 @@ namespace {
 //   * G threads share a row, NV 16-byte vectors each (VEC = 16 / element size).  Short rows take one warp (no block-wide step), longer
 //     ones a block.
 //   * the same with single elements (VEC = 1), for rows whose length or address is no multiple of 16 bytes.
+//   * forward, 16-bit rows of 1025 to about 16,000 elements (SHIFT): a row whose length is no multiple of 16 bytes starts anywhere in a
+//     16-byte vector, but rows 8 apart start at the same place of one.  A block takes every 8th (16th, ...) row, so that the shift and the
+//     weights behind a thread's elements stay the same, and reads whole vectors.  Single elements -> shifted vectors: 8192 x 2047
+//     34.2 -> 25.8 us, 4096 x 4095 34.1 -> 23.7, 1027 x 5001 12.8 -> 10.2, 2048 x 12289 61.4 -> 39.8, one row of 5001 5.5 -> 3.5;
+//     but 8192 x 511 12.1 -> 13.2, 2048 x 20001 65 -> 100 (weights gathered per row), fp32 8192 x 1023 18.3 -> 18.1, and the backward
+//     pass, which holds two rows, 4096 x 4095 36.6 -> 40.5.
 //   * rows too long for that: a block walks the row several times (it is in L1 and L2 after the first).
 // load_once, store_once: data that passes through once leaves L2 first, so that the partial sums stay there (16384 x 4096: 79 -> 77 us).
 template <typename T, int VEC> struct Pack;
@@ -37,6 +43,50 @@ template <typename T, int VEC> struct alignas(16) Pack {
     __device__ __forceinline__ void clear() { *reinterpret_cast<uint4 *>(v) = make_uint4(0u, 0u, 0u, 0u); }
 };
 
+// Elements [i, i + VEC) of a row of n.  SHIFT: i may be negative; the vector is read whole, with the neighbouring rows' elements in it,
+// unless it reaches over the end of the tensor (`left` elements behind the row's start), and clean() zeroes what is not the row's before
+// use.  Both handle whole 32-bit words: single 16-bit elements would be taken apart, and so waited for, where they are read.
+template <typename T>
+__device__ __forceinline__ uint32_t word_of(const T *row, int i, int64_t left) {
+    const uint16_t *bits = reinterpret_cast<const uint16_t *>(row);
+    return (i < left ? (uint32_t)bits[i] : 0u) | (i + 1 < left ? (uint32_t)bits[i + 1] << 16 : 0u);
+}
+template <bool SHIFT, typename T, int VEC>
+__device__ __forceinline__ void load_part(Pack<T, VEC> &p, const T *row, int i, int n, int64_t left) {
+    if (i >= n) return;
+    if (!SHIFT || i + VEC <= left) {
+        p.load(row + i);
+    } else if constexpr (SHIFT) {
+        *reinterpret_cast<uint4 *>(p.v) = make_uint4(word_of(row, i, left), word_of(row, i + 2, left), word_of(row, i + 4, left), word_of(row, i + 6, left));
+    }
+}
+__device__ __forceinline__ uint32_t mask_of(int i, int n) {
+    return (i >= 0 && i < n ? 0xffffu : 0u) | (i + 1 >= 0 && i + 1 < n ? 0xffff0000u : 0u);
+}
+template <bool SHIFT, typename T, int VEC>
+__device__ __forceinline__ void clean(Pack<T, VEC> &p, int i, int n) {
+    if constexpr (SHIFT) {
+        if (i >= 0 && i + VEC <= n) return;
+        uint4 *words = reinterpret_cast<uint4 *>(p.v);
+        *words = make_uint4(words->x & mask_of(i, n), words->y & mask_of(i + 2, n), words->z & mask_of(i + 4, n), words->w & mask_of(i + 6, n));
+    }
+}
+template <bool SHIFT, typename T, int VEC>
+__device__ __forceinline__ void store_part(const Pack<T, VEC> &p, T *row, int i, int n) {
+    if (SHIFT ? i >= 0 && i + VEC <= n : i < n) {
+        p.store(row + i);
+    } else if (SHIFT) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (i + e >= 0 && i + e < n) row[i + e] = p.v[e];
+    }
+}
+// the same elements of a vector that every row shares (weight, bias), whatever its alignment
+template <typename T, int VEC>
+__device__ __forceinline__ void gather(Pack<T, VEC> &p, const T *v, int i, int n) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) p.v[e] = i + e >= 0 && i + e < n ? v[i + e] : from_f32<T>(0.f);
+}
 // VEC floats between registers and shared memory (16-byte aligned when VEC > 1)
 template <int VEC>
 __device__ __forceinline__ void load_floats(float (&v)[VEC], const float *p) {
@@ -84,7 +134,7 @@ __device__ __forceinline__ void prefetch_row(const T *row, int32_t n) {
 // ------------------------------------------------------------------------------------------------
 // BLOCK: the whole block shares one row; otherwise each warp has its own.  MANY: more than 512 threads share it; with 64 registers a
 // thread the next row is asked for in L2 instead of in registers.
-template <typename T, int VEC, int NV, bool BLOCK, bool MANY>
+template <typename T, int VEC, int NV, bool BLOCK, bool MANY, bool SHIFT>
 __global__ void __launch_bounds__(MANY ? 1024 : BLOCK ? 512 : 128, MANY ? 1 : VEC * NV > 16 ? 1 : BLOCK ? 2 : 8)
 ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_mean, const T *__restrict__ x, const T *__restrict__ w,
                        const T *__restrict__ b, T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
@@ -92,24 +142,45 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
     const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, stride = (BLOCK ? blockDim.x : 32) * VEC;
     const int64_t first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int64_t step = BLOCK ? gridDim.x : (int64_t)gridDim.x * 4;
+    const int shift = SHIFT ? (int)((first * n) % VEC) : 0;         // where the walker's rows start in a vector
+    // SHIFT: weight and bias are gathered by element, once, and kept in the thread's own slots of shared memory (64 registers hold no more),
+    // with four vectors a thread in registers (of which there are 128 then)
+    static_assert(!SHIFT || (BLOCK && !MANY), "shifted rows are a block's of 512 threads at most");
+    constexpr bool kKeep = SHIFT && NV <= 2, kHold = SHIFT && NV > 2;
+    __shared__ uint4 kept[kKeep ? 2 * NV : 1][kKeep ? 512 : 1];
+    Pack<T, VEC> held[kHold ? 2 * NV : 1];
     Pack<T, VEC> in[NV];
     auto request = [&](int64_t row) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = t * VEC + j * stride;
-            if (i < n) in[j].load(x + row * n + i);
-        }
+        for (int j = 0; j < NV; ++j) load_part<SHIFT>(in[j], x + row * n, t * VEC + j * stride - shift, n, (rows - row) * n);
     };
 #pragma unroll
-    for (int j = 0; j < NV; ++j) in[j].clear();
+    for (int j = 0; j < NV; ++j) {
+        in[j].clear();
+        if constexpr (kKeep) {
+            Pack<T, VEC> pw, pb;
+            gather(pw, w, t * VEC + j * stride - shift, n);
+            if (b) gather(pb, b, t * VEC + j * stride - shift, n);
+            else pb.clear();
+            kept[kKeep ? 2 * j : 0][kKeep ? threadIdx.x : 0] = *reinterpret_cast<const uint4 *>(pw.v);
+            kept[kKeep ? 2 * j + 1 : 0][kKeep ? threadIdx.x : 0] = *reinterpret_cast<const uint4 *>(pb.v);
+        }
+        if constexpr (kHold) {
+            gather(held[2 * j], w, t * VEC + j * stride - shift, n);
+            if (b) gather(held[2 * j + 1], b, t * VEC + j * stride - shift, n);
+            else held[2 * j + 1].clear();
+        }
+    }
     if (first < rows) request(first);
     int parity = 0;
     for (int64_t row = first; row < rows; row += step, parity ^= 1) {
         float v[NV][VEC], mean = 0.f;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            clean<SHIFT>(in[j], t * VEC + j * stride - shift, n);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[j][e] = to_f32(in[j].v[e]);
+        }
         if (row + step < rows) {
             if (MANY) prefetch_row(x + (row + step) * n, n);
             else request(row + step);
@@ -127,8 +198,9 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
+                const int i = t * VEC + j * stride - shift;
                 v[j][e] -= mean;
-                if (t * VEC + j * stride < n) q = fmaf(v[j][e], v[j][e], q);
+                if (SHIFT ? i + e >= 0 && i + e < n : i < n) q = fmaf(v[j][e], v[j][e], q);
             }
         const float rstd = 1.f / sqrtf(row_sum<BLOCK>(q, red[parity][1]) * inv_n + eps);
         if (t == 0 && rstd_out) {
@@ -137,15 +209,23 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int i = t * VEC + j * stride;
+            const int i = t * VEC + j * stride - shift;
             if (i >= n) break;
             Pack<T, VEC> pw, pb, out;
-            pw.load(w + i);                              // out of L1 after the first row
-            if (b) pb.load(b + i);
-            else pb.clear();
+            if constexpr (kKeep) {
+                *reinterpret_cast<uint4 *>(pw.v) = kept[kKeep ? 2 * j : 0][kKeep ? threadIdx.x : 0];
+                *reinterpret_cast<uint4 *>(pb.v) = kept[kKeep ? 2 * j + 1 : 0][kKeep ? threadIdx.x : 0];
+            } else if constexpr (kHold) {
+                pw = held[2 * j];
+                pb = held[2 * j + 1];
+            } else {
+                pw.load(w + i);                          // out of L1 after the first row
+                if (b) pb.load(b + i);
+                else pb.clear();
+            }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf(v[j][e] * rstd, to_f32(pw.v[e]), to_f32(pb.v[e])));
-            out.store(y + row * n + i);
+            store_part<SHIFT>(out, y + row * n, i, n);
         }
         if (MANY && row + step < rows) request(row + step);
     }
@@ -519,26 +599,41 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv), *b = static_cast<const T *>(bv);
     T *y = static_cast<T *>(yv);
     constexpr int kVec = 16 / (int)sizeof(T);
-    const Layout l = forward_layout(n, kVec, aligned16(x) && aligned16(w) && aligned16(b) && aligned16(y));
+    const bool rows_aligned = aligned16(x) && aligned16(y), aligned = rows_aligned && aligned16(w) && aligned16(b);
+    Layout l = forward_layout(n, kVec, aligned);
+    // shifted rows touch up to a vector more at each end; the layout of the next longer row whose length is whole vectors
+    const bool shift = sizeof(T) == 2 && rows_aligned && l.vec == 1 && n > 1024 && n <= 4 * 8 * 512 - 16;
+    if (shift) l = forward_layout((n + 2 * (kVec - 1)) / kVec * kVec, kVec, true);
     const float inv_n = 1.f / (float)n;
     // as many blocks as the SMs hold (launch bounds: 1024 threads of 64 registers, 512 of 128 with four vectors)
     const int64_t threads = l.threads == 32 ? 128 : l.threads, lanes = l.threads == 32 ? 4 : 1;
     const int64_t per_sm = l.threads == 0 ? 1 : (l.vec * l.nv > 16 ? 512 : 1024) / threads;
     const int64_t want = ceil_div64(rows, lanes), most = info.sm_count * (per_sm > 0 ? per_sm : 1);
-    const unsigned grid = (unsigned)(want < most ? want : most);
-#define CPMK_LN_FORWARD(VEC, NV, BLOCK, MANY, THREADS) \
-    ln_rows_forward_kernel<T, VEC, NV, BLOCK, MANY><<<grid, THREADS, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd)
-#define CPMK_LN_FORWARD_IF(VEC, EACH) \
-    else if (l.vec == VEC && l.threads == 32 && l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, false, false, 128); \
-    else if (l.vec == VEC && l.threads == 32) CPMK_LN_FORWARD(VEC, 2 * EACH, false, false, 128); \
-    else if (l.vec == VEC && l.threads == 1024) CPMK_LN_FORWARD(VEC, 4 * EACH, true, true, 1024); \
-    else if (l.vec == VEC && l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, true, false, l.threads); \
-    else if (l.vec == VEC && l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, true, false, l.threads); \
-    else if (l.vec == VEC) CPMK_LN_FORWARD(VEC, 4 * EACH, true, false, l.threads)
-    if (l.threads == 0) ln_rows_forward_wide_kernel<T><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
-    CPMK_LN_FORWARD_IF(kVec, 1);
-    CPMK_LN_FORWARD_IF(1, 4);
-#undef CPMK_LN_FORWARD_IF
+    const unsigned grid = (unsigned)(want <= most ? want : shift ? most / 8 * 8 : most);         // shifted: one row each, or a multiple of 8 walkers
+#define CPMK_LN_FORWARD(VEC, NV, BLOCK, MANY, SHIFT, THREADS) \
+    ln_rows_forward_kernel<T, VEC, NV, BLOCK, MANY, SHIFT><<<grid, THREADS, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd)
+#define CPMK_LN_FORWARD_BLOCK(VEC, EACH, SHIFT) \
+    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, true, false, SHIFT, l.threads); \
+    else if (l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, true, false, SHIFT, l.threads); \
+    else CPMK_LN_FORWARD(VEC, 4 * EACH, true, false, SHIFT, l.threads)
+#define CPMK_LN_FORWARD_WARP(VEC, EACH) \
+    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, false, false, false, 128); \
+    else CPMK_LN_FORWARD(VEC, 2 * EACH, false, false, false, 128)
+    if (l.threads == 0) {
+        ln_rows_forward_wide_kernel<T><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
+    } else if (shift) {
+        if constexpr (sizeof(T) == 2) { CPMK_LN_FORWARD_BLOCK(kVec, 1, true); }
+    } else if (l.vec == kVec) {
+        if (l.threads == 32) { CPMK_LN_FORWARD_WARP(kVec, 1); }
+        else if (l.threads == 1024) CPMK_LN_FORWARD(kVec, 4, true, true, false, 1024);
+        else { CPMK_LN_FORWARD_BLOCK(kVec, 1, false); }
+    } else {
+        if (l.threads == 32) { CPMK_LN_FORWARD_WARP(1, 4); }
+        else if (l.threads == 1024) CPMK_LN_FORWARD(1, 16, true, true, false, 1024);
+        else { CPMK_LN_FORWARD_BLOCK(1, 4, false); }
+    }
+#undef CPMK_LN_FORWARD_BLOCK
+#undef CPMK_LN_FORWARD_WARP
 #undef CPMK_LN_FORWARD
     CPMK_LAUNCH_CHECK();
     return CPMK_OK;
