@@ -8,6 +8,7 @@
 #include "cpmk_common.cuh"
 #include "cpmk_ptx.cuh"
 #include "cpmk_types.cuh"
+#include <algorithm>
 
 namespace cpmk {
 namespace {
@@ -377,9 +378,9 @@ ln_rows_backward_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const
     }
 }
 
-// The same for rows of up to 16384 elements or 4096 vectors whose column sums do not fit the registers: 1024 threads, the block's sums
-// in shared memory (each thread adds to its own columns), the next row asked for in L2.  Per row 16 bytes of shared-memory traffic a
-// column, half of what the SM moves while the row's 6 (16-bit) to 12 (fp32) bytes a column arrive.
+// The same for rows of up to 16384 elements or 4096 vectors that do not fit the registers beside their column sums: 1024 threads, the
+// block's sums in shared memory (each thread adds to its own columns), the next row asked for in L2.  Per row 16 bytes of shared-memory
+// traffic a column, half of what the SM moves while the 12 bytes a column of an fp32 row arrive.
 template <typename T, int VEC, int NV, bool COLUMNS>
 __global__ void __launch_bounds__(1024, 1) ln_rows_backward_long_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const T *__restrict__ dy,
                                                                         const T *__restrict__ x, const float *__restrict__ mean_in,
@@ -467,35 +468,22 @@ __global__ void __launch_bounds__(1024, 1) ln_rows_backward_long_kernel(int32_t 
     }
 }
 
-// Rows too long for registers, any length and alignment: the row is read twice.  The block's sums lie in shared memory (`in_smem`), or in
-// its own rows of `partial` where they do not fit; each thread adds to the columns it owns.
-template <typename T, bool COLUMNS>
+// Rows too long for registers, any length and alignment, dx only: the row is read twice.
+template <typename T>
 __global__ void __launch_bounds__(1024) ln_rows_backward_wide_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const T *__restrict__ dy,
                                                                      const T *__restrict__ x, const float *__restrict__ mean_in,
-                                                                     const float *__restrict__ rstd_in, const T *__restrict__ w, T *__restrict__ dx,
-                                                                     float *__restrict__ partial, int32_t pitch, int in_smem) {
+                                                                     const float *__restrict__ rstd_in, const T *__restrict__ w, T *__restrict__ dx) {
     __shared__ float red[2][32];
-    extern __shared__ float columns[];                   // 2 n, or nothing
-    if (COLUMNS) launch_dependents();
-    float *global = COLUMNS ? partial + (int64_t)blockIdx.x * 2 * pitch : nullptr;
-    float *sums = in_smem ? columns : global;
-    const int second = in_smem ? n : pitch;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * n, *dyr = dy + row * n;
         const float mean = mean_in[row], rstd = rstd_in[row];
-        const bool first = row == blockIdx.x;
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll 4
         for (int i = threadIdx.x; i < n; i += 1024) {
-            const float d = to_f32(dyr[i]), g = d * to_f32(w[i]), xh = (to_f32(xr[i]) - mean) * rstd;
+            const float g = to_f32(dyr[i]) * to_f32(w[i]);
             s1 += g;
-            s2 = fmaf(g, xh, s2);
-            if (COLUMNS) {
-                sums[i] = first ? d * xh : fmaf(d, xh, sums[i]);
-                sums[second + i] = first ? d : sums[second + i] + d;
-            }
+            s2 = fmaf(g, (to_f32(xr[i]) - mean) * rstd, s2);
         }
-        if (!dx) continue;
         const float c1 = row_sum<true>(s1, red[0]) * (rd_mean ? inv_n : 0.f);
         const float c2 = row_sum<true>(s2, red[1]) * inv_n;
 #pragma unroll 4
@@ -504,11 +492,59 @@ __global__ void __launch_bounds__(1024) ln_rows_backward_wide_kernel(int32_t row
             dx[row * n + i] = from_f32<T>(rstd * (g - c1 - xh * c2));
         }
     }
-    if (!COLUMNS || !in_smem) return;
-    for (int i = threadIdx.x; i < n; i += 1024) {        // the columns this thread added to
-        global[i] = columns[i];
-        global[pitch + i] = columns[n + i];
+}
+
+// The sums of dw and db alone, where a row's sums find no room beside the row: x and dy are read once more, but without a step that waits
+// for a whole row.  A thread has one vector's columns and adds every gridDim.y-th row to them; the block's sums go to row blockIdx.y of
+// `partial`.  2048 x 16384 bf16 24.5 us with the kernel that joins them (84 % of the copy rate; 27.9 without load_once, 29.3 with two rows
+// on their way).
+constexpr int kStripThreads = 128;
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kStripThreads, 8) ln_rows_strip_kernel(int32_t rows, int32_t n, const T *__restrict__ dy, const T *__restrict__ x,
+                                                                         const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+                                                                         float *__restrict__ partial, int32_t pitch) {
+    constexpr int kAhead = VEC == 1 ? 8 : 4;             // rows on their way at a time
+    launch_dependents();
+    const int64_t i = ((int64_t)blockIdx.x * kStripThreads + threadIdx.x) * VEC;
+    if (i >= n) return;
+    float sw[VEC], sb[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sw[e] = sb[e] = 0.f;
+    const int64_t step = (int64_t)gridDim.y;
+    int64_t row = blockIdx.y;
+    const T *xr = x + row * n + i, *dr = dy + row * n + i;
+    auto take = [&](const Pack<T, VEC> &px, const Pack<T, VEC> &pd, float m, float r) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float d = to_f32(pd.v[e]);
+            sw[e] = fmaf(d, (to_f32(px.v[e]) - m) * r, sw[e]);
+            sb[e] += d;
+        }
+    };
+    for (; row + (kAhead - 1) * step < rows; row += kAhead * step) {
+        Pack<T, VEC> px[kAhead], pd[kAhead];
+        float m[kAhead], r[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            px[a].load_once(xr + a * step * n);
+            pd[a].load_once(dr + a * step * n);
+            m[a] = mean_in[row + a * step];
+            r[a] = rstd_in[row + a * step];
+        }
+        xr += kAhead * step * n;
+        dr += kAhead * step * n;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) take(px[a], pd[a], m[a], r[a]);
     }
+    for (; row < rows; row += step, xr += step * n, dr += step * n) {
+        Pack<T, VEC> px, pd;
+        px.load_once(xr);
+        pd.load_once(dr);
+        take(px, pd, mean_in[row], rstd_in[row]);
+    }
+    float *mine = partial + (int64_t)blockIdx.y * 2 * pitch + i;
+    store_floats<VEC>(mine, sw);
+    store_floats<VEC>(mine + pitch, sb);
 }
 
 // dw and db: the sums of the blocks' partial rows.  A block has 32 columns: 8 threads of four columns, 64 lanes of rows, the lanes
@@ -639,25 +675,31 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
     return CPMK_OK;
 }
 
+// Whether dw and db take a pass of their own.  Beside a row in shared memory (one pass) -> pass of their own, bf16 or fp16: 2048 x 16384
+// 73.7 -> 68.7 us, 2048 x 8200 47.9 -> 46.2, 20 x 16384 24.0 -> 15.9; the rows move half the bytes of their sums there.  fp32 rows and single
+// elements keep to one pass (2048 x 8192 fp32 43.0 against 61, 2048 x 12289 bf16 63.5 against 88).
+template <typename T>
+constexpr bool kSumsBesideVectors = sizeof(T) == 4;
+template <typename T>
+bool strips_for(const Layout &l) { return l.threads == 0 || (l.threads == 1024 && l.vec > 1 && !kSumsBesideVectors<T>); }
+constexpr int kMostSums = 2 * 16384 * (int)sizeof(float);        // in shared memory: of a row that 1024 threads take
+
 template <typename T, bool COLUMNS>
-int32_t backward_rows(const DeviceInfo &info, int blocks, int32_t rows, int32_t n, const T *dy, const T *x, int rd_mean, const T *w, const float *mean,
-                      const float *rstd, T *dx, float *partial, cudaStream_t stream) {
+int32_t backward_rows(const Layout &l, int blocks, int32_t rows, int32_t n, const T *dy, const T *x, int rd_mean, const T *w, const float *mean, const float *rstd,
+                      T *dx, float *partial, cudaStream_t stream) {
     constexpr int kVec = 16 / (int)sizeof(T);
-    Layout l = backward_layout(n, kVec, aligned16(x) && aligned16(dy) && aligned16(w) && aligned16(dx));
     const float inv_n = 1.f / (float)n;
     const int32_t pitch = column_pitch(n);
-    const int64_t sums = COLUMNS ? 2 * (int64_t)n * (int64_t)sizeof(float) : 0;
-    // the kernels' static arrays take half a KiB; the attribute is the same for every size, so that two threads' calls cannot undo each
-    // other's
-    const int64_t smem_most = info.max_smem_optin - 1024;
-    const bool fits = sums <= smem_most;
-    if (l.threads == 1024 && !fits) l = {1, 0, 0};
+    const size_t sums = COLUMNS ? 2 * (size_t)n * sizeof(float) : 0;
 #define CPMK_LN_BACKWARD(VEC, NV, BLOCK, THREADS, SMEM) \
     ln_rows_backward_kernel<T, VEC, NV, BLOCK, COLUMNS><<<blocks, THREADS, SMEM, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch)
+// (the attribute is the same for every size, so that two threads' calls cannot undo each other's)
 #define CPMK_LN_BACKWARD_LONG(VEC, NV) \
     { \
-        if (COLUMNS) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_most)); \
-        ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS><<<blocks, 1024, sums, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch); \
+        if constexpr (!COLUMNS || VEC == 1 || kSumsBesideVectors<T>) { \
+            if (COLUMNS) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSums)); \
+            ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS><<<blocks, 1024, sums, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch); \
+        } \
     }
 #define CPMK_LN_BACKWARD_IF(VEC, EACH) \
     else if (l.vec == VEC && l.threads == 32 && l.nv == EACH) CPMK_LN_BACKWARD(VEC, EACH, false, 256, 8 * sums); \
@@ -665,12 +707,7 @@ int32_t backward_rows(const DeviceInfo &info, int blocks, int32_t rows, int32_t 
     else if (l.vec == VEC && l.threads == 1024) CPMK_LN_BACKWARD_LONG(VEC, 4 * EACH) \
     else if (l.vec == VEC && l.nv == EACH) CPMK_LN_BACKWARD(VEC, EACH, true, l.threads, 0); \
     else if (l.vec == VEC) CPMK_LN_BACKWARD(VEC, 2 * EACH, true, l.threads, 0);
-    if (l.threads == 0) {
-        const int in_smem = COLUMNS && fits;
-        if (in_smem) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_wide_kernel<T, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_most));
-        ln_rows_backward_wide_kernel<T, COLUMNS><<<blocks, 1024, in_smem ? sums : 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch,
-                                                                                              in_smem);
-    }
+    if (l.threads == 0) ln_rows_backward_wide_kernel<T><<<blocks, 1024, 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx);
     CPMK_LN_BACKWARD_IF(kVec, 1)
     CPMK_LN_BACKWARD_IF(1, 4)
 #undef CPMK_LN_BACKWARD_IF
@@ -685,13 +722,28 @@ int32_t backward(const DeviceInfo &info, int32_t rows, int32_t n, const void *dy
                  const float *rstd, void *dxv, void *dw, void *db, float *partial, cudaStream_t stream) {
     const T *dy = static_cast<const T *>(dyv), *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     T *dx = static_cast<T *>(dxv);
+    constexpr int kVec = 16 / (int)sizeof(T);
     const int blocks = backward_blocks(info, rows, n);
-    if (!dw && !db) return backward_rows<T, false>(info, blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, nullptr, stream);
-    const int32_t rc = backward_rows<T, true>(info, blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, partial, stream);
-    if (rc) return rc;
-    CPMK_CUDA_TRY(launch_after_prior(ln_rows_columns_kernel<T>, dim3((n + 31) / 32, 2), dim3(kColumnThreads), 0, stream, blocks, n, column_pitch(n),
-                                     static_cast<const float *>(partial), static_cast<T *>(dw), static_cast<T *>(db)));
-    return CPMK_OK;
+    const Layout l = backward_layout(n, kVec, aligned16(x) && aligned16(dy) && aligned16(w) && aligned16(dx));
+    const bool sums = dw || db, strips = sums && strips_for<T>(l);
+    int32_t rc = CPMK_OK;
+    int parts = blocks;
+    if (strips) {
+        const int vec = n % kVec == 0 && aligned16(x) && aligned16(dy) ? kVec : 1;
+        const int64_t across = ceil_div64(n, kStripThreads * vec), down = std::max<int64_t>(1, 8 * info.sm_count / across);
+        parts = (int)std::min<int64_t>(parts, down);
+        if (vec > 1) ln_rows_strip_kernel<T, kVec><<<dim3((unsigned)across, (unsigned)parts), kStripThreads, 0, stream>>>(rows, n, dy, x, mean, rstd, partial, column_pitch(n));
+        else ln_rows_strip_kernel<T, 1><<<dim3((unsigned)across, (unsigned)parts), kStripThreads, 0, stream>>>(rows, n, dy, x, mean, rstd, partial, column_pitch(n));
+        CPMK_LAUNCH_CHECK();
+    } else if (sums) {
+        rc = backward_rows<T, true>(l, blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, partial, stream);
+        if (rc) return rc;
+    }
+    if (sums)
+        CPMK_CUDA_TRY(launch_after_prior(ln_rows_columns_kernel<T>, dim3((n + 31) / 32, 2), dim3(kColumnThreads), 0, stream, parts, n, column_pitch(n),
+                                         static_cast<const float *>(partial), static_cast<T *>(dw), static_cast<T *>(db)));
+    if (dx && (strips || !sums)) rc = backward_rows<T, false>(l, blocks, rows, n, dy, x, rd_mean, w, mean, rstd, dx, nullptr, stream);
+    return rc;
 }
 
 }  // namespace
