@@ -24,7 +24,8 @@ namespace {
 //     34.2 -> 25.8 us, 4096 x 4095 34.1 -> 23.7, 1027 x 5001 12.8 -> 10.2, 2048 x 12289 61.4 -> 39.8, one row of 5001 5.5 -> 3.5;
 //     but 8192 x 511 12.1 -> 13.2, 2048 x 20001 65 -> 100 (weights gathered per row), fp32 8192 x 1023 18.3 -> 18.1, and the backward
 //     pass, which holds two rows, 4096 x 4095 36.6 -> 40.5.
-//   * rows too long for that: a block walks the row several times (it is in L1 and L2 after the first).
+//   * rows too long for that: a block walks the row several times (it is in L1 and L2 after the first), by vectors where it can (1000 x
+//     60000 fp16 62 us, by single elements 110).
 // load_once, store_once: data that passes through once leaves L2 first, so that the partial sums stay there (16384 x 4096: 79 -> 77 us).
 template <typename T, int VEC> struct Pack;
 template <typename T> struct Pack<T, 1> {
@@ -234,31 +235,50 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
 
 constexpr int kWideThreads = 512;
 
-template <typename T>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kWideThreads) ln_rows_forward_wide_kernel(int32_t n, float inv_n, float eps, int rd_mean, const T *__restrict__ x,
                                                                             const T *__restrict__ w, const T *__restrict__ b, T *__restrict__ y,
                                                                             float *__restrict__ mean_out, float *__restrict__ rstd_out) {
     __shared__ float red[2][32];
     const int64_t row = blockIdx.x;
     const T *xr = x + row * n;
+    const int32_t first = threadIdx.x * VEC, step = kWideThreads * VEC;
     float mean = 0.f;
     if (rd_mean) {
         float s = 0.f;
-        for (int i = threadIdx.x; i < n; i += kWideThreads) s += to_f32(xr[i]);
+        for (int32_t i = first; i < n; i += step) {
+            Pack<T, VEC> px;
+            px.load(xr + i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += to_f32(px.v[e]);
+        }
         mean = row_sum<true>(s, red[0]) * inv_n;
     }
     float q = 0.f;
-    for (int i = threadIdx.x; i < n; i += kWideThreads) {
-        const float d = to_f32(xr[i]) - mean;
-        q = fmaf(d, d, q);
+    for (int32_t i = first; i < n; i += step) {
+        Pack<T, VEC> px;
+        px.load(xr + i);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float d = to_f32(px.v[e]) - mean;
+            q = fmaf(d, d, q);
+        }
     }
     const float rstd = 1.f / sqrtf(row_sum<true>(q, red[1]) * inv_n + eps);
     if (threadIdx.x == 0 && rstd_out) {
         mean_out[row] = mean;
         rstd_out[row] = rstd;
     }
-    for (int i = threadIdx.x; i < n; i += kWideThreads)
-        y[row * n + i] = from_f32<T>(fmaf((to_f32(xr[i]) - mean) * rstd, to_f32(w[i]), b ? to_f32(b[i]) : 0.f));
+    for (int32_t i = first; i < n; i += step) {
+        Pack<T, VEC> px, pw, pb, out;
+        px.load(xr + i);
+        pw.load(w + i);
+        if (b) pb.load(b + i);
+        else pb.clear();
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf((to_f32(px.v[e]) - mean) * rstd, to_f32(pw.v[e]), to_f32(pb.v[e])));
+        out.store(y + row * n + i);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -468,29 +488,46 @@ __global__ void __launch_bounds__(1024, 1) ln_rows_backward_long_kernel(int32_t 
     }
 }
 
-// Rows too long for registers, any length and alignment, dx only: the row is read twice.
-template <typename T>
+// Rows too long for registers, dx only: the row is read twice (1000 x 60000 fp16 95 us, by single elements 195).
+template <typename T, int VEC>
 __global__ void __launch_bounds__(1024) ln_rows_backward_wide_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const T *__restrict__ dy,
                                                                      const T *__restrict__ x, const float *__restrict__ mean_in,
                                                                      const float *__restrict__ rstd_in, const T *__restrict__ w, T *__restrict__ dx) {
     __shared__ float red[2][32];
+    const int32_t begin = threadIdx.x * VEC, step = 1024 * VEC;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * n, *dyr = dy + row * n;
         const float mean = mean_in[row], rstd = rstd_in[row];
         float s1 = 0.f, s2 = 0.f;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += 1024) {
-            const float g = to_f32(dyr[i]) * to_f32(w[i]);
-            s1 += g;
-            s2 = fmaf(g, (to_f32(xr[i]) - mean) * rstd, s2);
-        }
+        auto walk = [&](auto use) {
+#pragma unroll VEC == 1 ? 4 : 2
+            for (int32_t i = begin; i < n; i += step) {
+                Pack<T, VEC> px, pd, pw;
+                px.load(xr + i);
+                pd.load(dyr + i);
+                pw.load(w + i);
+                use(px, pd, pw, i);
+            }
+        };
+        walk([&](const Pack<T, VEC> &px, const Pack<T, VEC> &pd, const Pack<T, VEC> &pw, int32_t) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float g = to_f32(pd.v[e]) * to_f32(pw.v[e]);
+                s1 += g;
+                s2 = fmaf(g, (to_f32(px.v[e]) - mean) * rstd, s2);
+            }
+        });
         const float c1 = row_sum<true>(s1, red[0]) * (rd_mean ? inv_n : 0.f);
         const float c2 = row_sum<true>(s2, red[1]) * inv_n;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += 1024) {
-            const float g = to_f32(dyr[i]) * to_f32(w[i]), xh = (to_f32(xr[i]) - mean) * rstd;
-            dx[row * n + i] = from_f32<T>(rstd * (g - c1 - xh * c2));
-        }
+        walk([&](const Pack<T, VEC> &px, const Pack<T, VEC> &pd, const Pack<T, VEC> &pw, int32_t i) {
+            Pack<T, VEC> out;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float g = to_f32(pd.v[e]) * to_f32(pw.v[e]), xh = (to_f32(px.v[e]) - mean) * rstd;
+                out.v[e] = from_f32<T>(rstd * (g - c1 - xh * c2));
+            }
+            out.store(dx + row * n + i);
+        });
     }
 }
 
@@ -601,7 +638,7 @@ Layout layout_of(int32_t n, int per_vector, bool aligned, int per_warp, int most
     for (int i = 2; i <= most; i *= 2)
         if (units <= 512 * i * each) return {vec, i * each, threads(i * each)};
     if (units <= 1024 * 4 * each) return {vec, 4 * each, 1024};
-    return {1, 0, 0};
+    return {vec, 0, 0};
 }
 Layout forward_layout(int32_t n, int per_vector, bool aligned) { return layout_of(n, per_vector, aligned, 2, 4); }
 // a column's two sums are registers too: at most two vectors a thread
@@ -656,7 +693,8 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
     if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, false, false, false, 128); \
     else CPMK_LN_FORWARD(VEC, 2 * EACH, false, false, false, 128)
     if (l.threads == 0) {
-        ln_rows_forward_wide_kernel<T><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
+        if (l.vec > 1) ln_rows_forward_wide_kernel<T, kVec><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
+        else ln_rows_forward_wide_kernel<T, 1><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
     } else if (shift) {
         if constexpr (sizeof(T) == 2) { CPMK_LN_FORWARD_BLOCK(kVec, 1, true); }
     } else if (l.vec == kVec) {
@@ -707,7 +745,8 @@ int32_t backward_rows(const Layout &l, int blocks, int32_t rows, int32_t n, cons
     else if (l.vec == VEC && l.threads == 1024) CPMK_LN_BACKWARD_LONG(VEC, 4 * EACH) \
     else if (l.vec == VEC && l.nv == EACH) CPMK_LN_BACKWARD(VEC, EACH, true, l.threads, 0); \
     else if (l.vec == VEC) CPMK_LN_BACKWARD(VEC, 2 * EACH, true, l.threads, 0);
-    if (l.threads == 0) ln_rows_backward_wide_kernel<T><<<blocks, 1024, 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx);
+    if (l.threads == 0 && l.vec > 1) ln_rows_backward_wide_kernel<T, kVec><<<blocks, 1024, 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx);
+    else if (l.threads == 0) ln_rows_backward_wide_kernel<T, 1><<<blocks, 1024, 0, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx);
     CPMK_LN_BACKWARD_IF(kVec, 1)
     CPMK_LN_BACKWARD_IF(1, 4)
 #undef CPMK_LN_BACKWARD_IF
