@@ -17,6 +17,18 @@ def test_host_tensors_are_refused():
         ct.gated_feed_forward(x, w, w, torch.ones((16, 8), dtype=torch.half))
 
 
+def test_refusals_say_what_is_wanted():
+    x, w = torch.ones((4, 16), dtype=torch.half), torch.ones((8, 16), dtype=torch.half)
+    with pytest.raises(AssertionError, match="contiguous CUDA tensor"):
+        ct.layernorm_rows(x, 1e-5, x[0])
+    with pytest.raises(AssertionError, match="contiguous CUDA tensor"):
+        ct.gated_linear(x, w, w)
+    with pytest.raises(AssertionError):
+        ct.gated_linear(x, w, w, "tanh")
+    with pytest.raises(TypeError):
+        ct.layernorm_rows(None, 1e-5, x[0])
+
+
 def test_launchers_check_sizes():
     with pytest.raises(AssertionError):
         ck.layernorm_rows_forward(1, 0, cpmk.F16, 0, 1e-5, True, 0, 0, 0, 0, 0, 0)
