@@ -132,6 +132,7 @@ int32_t launch_simt(const Call &call, SimtParams prm) {
         else gated_simt_kernel<__nv_bfloat16, EPI, CPMK_ACT_GELU><<<grid, 256, 0, call.stream>>>(prm);
     }
     CPMK_LAUNCH_CHECK();
+    call.launched = false;                               // (nothing waits for it early)
     return CPMK_OK;
 }
 

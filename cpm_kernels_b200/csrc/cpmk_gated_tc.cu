@@ -365,7 +365,7 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
     const bool leader = rank == 0;
-    if (prm.split_pairs) launch_dependents();
+    launch_dependents();                               // the join, or the call's next product
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
@@ -387,6 +387,7 @@ gated_tc_kernel(const __grid_constant__ TcMaps maps, const TcParams prm) {
     cluster_sync_all();                                // barriers of both CTAs are initialised before anyone signals them
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    wait_for_prior_grid();                             // of the same call: this CTA started when one of its CTAs left the SM
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(256) tc_join_kernel(const TcParams prm, void *
     const int tile_row = part / kAcross * 32 + (threadIdx.x & 31), tile_col = part % kAcross * kJoinBlockColumns + (threadIdx.x >> 5) * kJoinColumns;
     const int row = it.row + tile_row, col = it.col + tile_col;
     const int first = owner_of(prm, t * prm.blocks), last = owner_of(prm, (t + 1) * prm.blocks - 1);
+    launch_dependents();
     wait_for_prior_grid();
     const int C = it.C;
     if (row >= it.R || col >= C) return;
@@ -624,8 +626,10 @@ int32_t launch(const Call &call, const TcMaps &maps, TcParams prm, const Plan &p
     CPMK_REQUIRE(plan.whole + plan.split_tiles < (int64_t(1) << 30) && plan.split_tiles * plan.blocks < (int64_t(1) << 30), "too many output tiles");
     const int64_t pairs = call.info.sm_count / 2;        // advisory: a pair that is not resident at launch starts when another retires
     const int64_t used = plan.whole < pairs ? (plan.whole > plan.split_pairs ? plan.whole : plan.split_pairs) : pairs;
-    kernel<<<(unsigned)(2 * used), kThreads, kSmemBytes, call.stream>>>(maps, prm);
+    if (call.launched) CPMK_CUDA_TRY(launch_after_prior(kernel, dim3((unsigned)(2 * used)), dim3(kThreads), kSmemBytes, call.stream, maps, prm));
+    else kernel<<<(unsigned)(2 * used), kThreads, kSmemBytes, call.stream>>>(maps, prm);
     CPMK_LAUNCH_CHECK();
+    call.launched = true;
     if (!plan.split_tiles) return CPMK_OK;
     const int64_t parts = (EPI == kEpiGated ? kTileC / 2 : kTileC) / kJoinBlockColumns * (kTileR / 32);
     CPMK_CUDA_TRY(launch_after_prior(tc_join_kernel<BF16, EPI, ACT>, dim3((unsigned)(plan.split_tiles * parts)), dim3(256), 0, call.stream, prm, out0, out1,
