@@ -279,3 +279,73 @@ def test_gradients_against_differences():
             up = loss(*args)
             args[i].view(-1)[j] -= 2 * h
             assert abs((up - loss(*args)) / (2 * h) - g.view(-1)[j].item()) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("name", ["fp16", "bf16"])
+@pytest.mark.parametrize("rows,n", [(1300, 4099), (700, 1031), (9, 5001), (300, 12289), (200, 16365)])
+def test_rows_that_share_a_vector_keep_to_themselves(rows, n, name):
+    """Odd widths: a 16-byte vector holds the end of one row and the start of the next; a third of the rows is NaN or infinite.  Weight
+    and bias at an odd address."""
+    x, w, b, dy = make(rows, n, TYPES[name], 9)
+    w, b = (torch.cat([t[:1], t])[1:] for t in (w, b))
+    assert w.data_ptr() % 16 and x.data_ptr() % 16 == 0
+    y = ct.layernorm_rows(x, EPS, w, b)
+    want, bound = exact(x, w, b, dy, EPS, True)
+    check(y, want[0], bound[0], name, "y")
+    bad = x.clone()
+    bad[1::3] = float("nan")
+    bad[4::9] = float("inf")
+    z = ct.layernorm_rows(bad, EPS, w, b)
+    keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+    keep[1::3] = False
+    assert torch.equal(z[keep], y[keep])
+    assert torch.isnan(z[~keep]).all()
+
+
+@pytest.mark.parametrize("name", ["fp16", "fp32"])
+@pytest.mark.parametrize("rows,n", [(1300, 4099), (90, 20000), (50, 33001), (9, 66000)])
+def test_long_and_odd_rows_write_their_outputs_only(rows, n, name):
+    t, code = TYPES[name], cpmk.F16 if name == "fp16" else cpmk.F32
+    x, w, b, dy = make(rows, n, t, 6)
+    s = torch.cuda.current_stream().cuda_stream
+    pad = 64
+    y = torch.full((rows * n + 2 * pad,), 7.0, dtype=t, device="cuda")
+    dx, dw, db = y.clone(), torch.full((n + 2 * pad,), 7.0, dtype=t, device="cuda"), torch.full((n + 2 * pad,), 7.0, dtype=t, device="cuda")
+    stats = torch.empty((2, rows), device="cuda")
+    need = ck.layernorm_rows_backward_scratch(rows, n)
+    scratch = torch.full((need + 256,), 77, dtype=torch.uint8, device="cuda")
+    at = lambda v: v.data_ptr() + pad * v.element_size()
+    ck.layernorm_rows_forward(rows, n, code, x.data_ptr(), EPS, True, w.data_ptr(), b.data_ptr(), at(y), stats[0].data_ptr(), stats[1].data_ptr(), s)
+    ck.layernorm_rows_backward(rows, n, code, dy.data_ptr(), x.data_ptr(), True, w.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(), at(dx), at(dw),
+                               at(db), scratch.data_ptr(), s)
+    for v in (y, dx, dw, db):
+        assert (v[:pad] == 7).all() and (v[-pad:] == 7).all()
+    assert (scratch[need:] == 77).all()
+    want, bound = exact(x, w, b, dy, EPS, True)
+    for got, v, e, what in zip((y[pad:-pad].view(rows, n), dx[pad:-pad].view(rows, n), dw[pad:-pad], db[pad:-pad]), want, bound, "yxwb"):
+        check(got, v, e, name, what)
+
+
+@pytest.mark.parametrize("n", [2051, 20000])
+def test_offsets_beyond_32_bits_of_odd_and_long_rows(n):
+    """2.2e9 elements per tensor, as above; the gradient is zero but in one row behind the 2^31st element, so that the sums over the rows
+    are that row's."""
+    rows = 2_200_000_000 // n
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty((rows, n), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    dy = torch.zeros_like(x)
+    dy[rows - 3].normal_(generator=g)
+    w = (torch.ones(n, dtype=torch.bfloat16, device="cuda") * 1.5).requires_grad_()
+    x.requires_grad_()
+    y = ct.layernorm_rows(x, EPS, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    middle = 2 ** 31 // n
+    for at in (0, middle - 4, rows - 3):
+        at = at // 8 * 8                                 # rows 8 apart start at the same place of a vector: the same sums
+        part = x.detach()[at:at + 8].clone().requires_grad_()
+        z = ct.layernorm_rows(part, EPS, w)
+        assert torch.equal(z, y[at:at + 8])
+        ex, ew = torch.autograd.grad(z, (part, w), dy[at:at + 8].clone())
+        assert torch.equal(ex, dx[at:at + 8])
+        if at <= rows - 3 < at + 8:
+            assert torch.equal(ew, dw)
