@@ -22,8 +22,8 @@ namespace {
 //     16-byte vector, but rows 8 apart start at the same place of one.  A block takes every 8th (16th, ...) row, so that the shift and the
 //     weights behind a thread's elements stay the same, and reads whole vectors.  Single elements -> shifted vectors: 8192 x 2047
 //     34.2 -> 25.8 us, 4096 x 4095 34.1 -> 23.7, 1027 x 5001 12.8 -> 10.2, 2048 x 12289 61.4 -> 39.8, one row of 5001 5.5 -> 3.5;
-//     but 8192 x 511 12.1 -> 13.2, 2048 x 20001 65 -> 100 (weights gathered per row), fp32 8192 x 1023 18.3 -> 18.1, and the backward
-//     pass, which holds two rows, 4096 x 4095 36.6 -> 40.5.
+//     but 8192 x 511 12.1 -> 13.2 (in a warp, by single elements: 9.0), 2048 x 20001 65 -> 100 (weights gathered per row), fp32
+//     8192 x 1023 18.3 -> 18.1, and the backward pass, which holds two rows, 4096 x 4095 36.6 -> 40.5.
 //   * rows too long for that: a block walks the row several times (it is in L1 and L2 after the first), by vectors where it can (1000 x
 //     60000 fp16 62 us, by single elements 110).
 // load_once, store_once: data that passes through once leaves L2 first, so that the partial sums stay there (16384 x 4096: 79 -> 77 us).
@@ -134,10 +134,10 @@ __device__ __forceinline__ void prefetch_row(const T *row, int32_t n) {
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-// BLOCK: the whole block shares one row; otherwise each warp has its own.  MANY: more than 512 threads share it; with 64 registers a
-// thread the next row is asked for in L2 instead of in registers.
-template <typename T, int VEC, int NV, bool BLOCK, bool MANY, bool SHIFT>
-__global__ void __launch_bounds__(MANY ? 1024 : BLOCK ? 512 : 128, MANY ? 1 : VEC * NV > 16 ? 1 : BLOCK ? 2 : 8)
+// BLOCK: the whole block shares one row; otherwise each warp has its own.  MOST: threads of a block at most.  With more than 512 that share
+// a row (64 registers each) the next row is asked for in L2 instead of in registers.
+template <typename T, int VEC, int NV, bool BLOCK, int MOST, bool SHIFT>
+__global__ void __launch_bounds__(MOST, MOST == 1024 ? 1 : MOST == 512 ? (VEC * NV > 16 ? 1 : 2) : VEC * NV > 16 ? 5 : 8)
 ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_mean, const T *__restrict__ x, const T *__restrict__ w,
                        const T *__restrict__ b, T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
     __shared__ float red[2][2][32];
@@ -147,7 +147,8 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
     const int shift = SHIFT ? (int)((first * n) % VEC) : 0;         // where the walker's rows start in a vector
     // SHIFT: weight and bias are gathered by element, once, and kept in the thread's own slots of shared memory (64 registers hold no more),
     // with four vectors a thread in registers (of which there are 128 then)
-    static_assert(!SHIFT || (BLOCK && !MANY), "shifted rows are a block's of 512 threads at most");
+    constexpr bool kMany = MOST == 1024;
+    static_assert(!SHIFT || (BLOCK && MOST == 512), "shifted rows are a block's of 512 threads at most");
     constexpr bool kKeep = SHIFT && NV <= 2, kHold = SHIFT && NV > 2;
     __shared__ uint4 kept[kKeep ? 2 * NV : 1][kKeep ? 512 : 1];
     Pack<T, VEC> held[kHold ? 2 * NV : 1];
@@ -184,7 +185,7 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
             for (int e = 0; e < VEC; ++e) v[j][e] = to_f32(in[j].v[e]);
         }
         if (row + step < rows) {
-            if (MANY) prefetch_row(x + (row + step) * n, n);
+            if (kMany) prefetch_row(x + (row + step) * n, n);
             else request(row + step);
         }
         if (rd_mean) {
@@ -229,7 +230,7 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
             for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf(v[j][e] * rstd, to_f32(pw.v[e]), to_f32(pb.v[e])));
             store_part<SHIFT>(out, y + row * n, i, n);
         }
-        if (MANY && row + step < rows) request(row + step);
+        if (kMany && row + step < rows) request(row + step);
     }
 }
 
@@ -640,7 +641,15 @@ Layout layout_of(int32_t n, int per_vector, bool aligned, int per_warp, int most
     if (units <= 1024 * 4 * each) return {vec, 4 * each, 1024};
     return {vec, 0, 0};
 }
-Layout forward_layout(int32_t n, int per_vector, bool aligned) { return layout_of(n, per_vector, aligned, 2, 4); }
+// Many rows: few threads with four vectors each, since a row's sums cost every warp that shares it the same (two vectors and twice the
+// threads -> four: 30000 x 1024 fp16 31.7 -> 22.3 us, 30000 x 768 26.6 -> 18.5, 16384 x 4096 bf16 53.1 -> 49.2; 148 x 4096 2.8 -> 3.3), unless
+// that leaves an eighth of the threads idle (4000 x 2560 10.5 -> 10.9).
+Layout forward_layout(int32_t n, int per_vector, bool aligned, bool many_rows) {
+    Layout l = layout_of(n, per_vector, aligned, many_rows ? 4 : 2, 4);
+    const int units = n / l.vec, threads = (units + 127) / 128 * 32;
+    if (many_rows && l.vec > 1 && l.threads > 32 && threads <= 128 && units * 8 >= threads * 4 * 7) l = {l.vec, 4, threads};
+    return l;
+}
 // a column's two sums are registers too: at most two vectors a thread
 Layout backward_layout(int32_t n, int per_vector, bool aligned) { return layout_of(n, per_vector, aligned, 2, 2); }
 
@@ -673,25 +682,28 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
     T *y = static_cast<T *>(yv);
     constexpr int kVec = 16 / (int)sizeof(T);
     const bool rows_aligned = aligned16(x) && aligned16(y), aligned = rows_aligned && aligned16(w) && aligned16(b);
-    Layout l = forward_layout(n, kVec, aligned);
+    const bool many_rows = rows >= 8 * info.sm_count;
+    Layout l = forward_layout(n, kVec, aligned, many_rows);
     // shifted rows touch up to a vector more at each end; the layout of the next longer row whose length is whole vectors
     const bool shift = sizeof(T) == 2 && rows_aligned && l.vec == 1 && n > 1024 && n <= 4 * 8 * 512 - 16;
-    if (shift) l = forward_layout((n + 2 * (kVec - 1)) / kVec * kVec, kVec, true);
+    if (shift) l = forward_layout((n + 2 * (kVec - 1)) / kVec * kVec, kVec, true, false);
     const float inv_n = 1.f / (float)n;
-    // as many blocks as the SMs hold (launch bounds: 1024 threads of 64 registers, 512 of 128 with four vectors)
+    // as many blocks as the SMs hold (launch bounds: 1024 threads of 64 registers; with four vectors 640 of 102 or, in large blocks, 512 of 128)
     const int64_t threads = l.threads == 32 ? 128 : l.threads, lanes = l.threads == 32 ? 4 : 1;
-    const int64_t per_sm = l.threads == 0 ? 1 : (l.vec * l.nv > 16 ? 512 : 1024) / threads;
+    const bool narrow = l.vec > 1 && l.nv == 4 && l.threads <= 128 && !shift;
+    const int64_t per_sm = l.threads == 0 ? 1 : (l.vec * l.nv <= 16 ? 1024 : narrow ? 640 : 512) / threads;
     const int64_t want = ceil_div64(rows, lanes), most = info.sm_count * (per_sm > 0 ? per_sm : 1);
     const unsigned grid = (unsigned)(want <= most ? want : shift ? most / 8 * 8 : most);         // shifted: one row each, or a multiple of 8 walkers
-#define CPMK_LN_FORWARD(VEC, NV, BLOCK, MANY, SHIFT, THREADS) \
-    ln_rows_forward_kernel<T, VEC, NV, BLOCK, MANY, SHIFT><<<grid, THREADS, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd)
+#define CPMK_LN_FORWARD(VEC, NV, BLOCK, MOST, SHIFT, THREADS) \
+    ln_rows_forward_kernel<T, VEC, NV, BLOCK, MOST, SHIFT><<<grid, THREADS, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd)
 #define CPMK_LN_FORWARD_BLOCK(VEC, EACH, SHIFT) \
-    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, true, false, SHIFT, l.threads); \
-    else if (l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, true, false, SHIFT, l.threads); \
-    else CPMK_LN_FORWARD(VEC, 4 * EACH, true, false, SHIFT, l.threads)
+    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, true, 512, SHIFT, l.threads); \
+    else if (l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, true, 512, SHIFT, l.threads); \
+    else CPMK_LN_FORWARD(VEC, 4 * EACH, true, 512, SHIFT, l.threads)
 #define CPMK_LN_FORWARD_WARP(VEC, EACH) \
-    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, false, false, false, 128); \
-    else CPMK_LN_FORWARD(VEC, 2 * EACH, false, false, false, 128)
+    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, false, 128, false, 128); \
+    else if (l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, false, 128, false, 128); \
+    else CPMK_LN_FORWARD(VEC, 4 * EACH, false, 128, false, 128)
     if (l.threads == 0) {
         if (l.vec > 1) ln_rows_forward_wide_kernel<T, kVec><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
         else ln_rows_forward_wide_kernel<T, 1><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
@@ -699,11 +711,12 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
         if constexpr (sizeof(T) == 2) { CPMK_LN_FORWARD_BLOCK(kVec, 1, true); }
     } else if (l.vec == kVec) {
         if (l.threads == 32) { CPMK_LN_FORWARD_WARP(kVec, 1); }
-        else if (l.threads == 1024) CPMK_LN_FORWARD(kVec, 4, true, true, false, 1024);
+        else if (l.threads == 1024) CPMK_LN_FORWARD(kVec, 4, true, 1024, false, 1024);
+        else if (narrow) CPMK_LN_FORWARD(kVec, 4, true, 128, false, l.threads);
         else { CPMK_LN_FORWARD_BLOCK(kVec, 1, false); }
     } else {
         if (l.threads == 32) { CPMK_LN_FORWARD_WARP(1, 4); }
-        else if (l.threads == 1024) CPMK_LN_FORWARD(1, 16, true, true, false, 1024);
+        else if (l.threads == 1024) CPMK_LN_FORWARD(1, 16, true, 1024, false, 1024);
         else { CPMK_LN_FORWARD_BLOCK(1, 4, false); }
     }
 #undef CPMK_LN_FORWARD_BLOCK
