@@ -19,7 +19,8 @@ TINY = {"fp16": 2.0 ** -25, "bf16": 2.0 ** -134, "fp32": 2.0 ** -150}
 SIZES = [(1, 1), (1, 4096), (3, 8), (5, 7), (2, 31), (33, 32), (7, 33), (130, 129), (64, 256), (9, 1000), (300, 1024), (257, 1032), (31, 4096),
          (1000, 64), (5, 8192), (4, 16384), (3, 16392), (2, 20001), (12, 5001), (2, 33000), (700, 520), (37, 16385), (300, 9000), (9, 3),
          (4000, 77), (5000, 515), (2500, 1003), (1300, 4099), (400, 9003), (600, 2050), (20, 1001), (150, 16367), (450, 16369),
-         (130, 16400), (90, 33001), (45, 66000)]
+         (130, 16400), (90, 33001), (45, 66000),
+         (5000, 1024), (4800, 1000), (6001, 300), (5003, 769), (4737, 333), (1300, 2048), (1200, 3584)]
 
 
 def make(rows, n, t, seed=0, offset=0.25):
