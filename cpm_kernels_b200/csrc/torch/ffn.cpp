@@ -167,7 +167,9 @@ void check_gated(const Tensor &x, const Tensor &w_gate, const Tensor &w_up) {
     want(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "gated block: x must be fp16 or bf16");
     want(w_gate.dim() == 2, "gated block: w_gate must be a matrix");
     const int64_t n = w_gate.size(0), k = w_gate.size(1);
-    want(n >= 1 && k >= 1 && x.size(-1) == k && x.numel() / k <= kMost, "gated block: w_gate must be (N, K) for x (..., K), with 2^30 rows of x at most");
+    // the C entry points take 32-bit extents
+    want(n >= 1 && k >= 1 && n <= kMost && k <= kMost && x.size(-1) == k && x.numel() / k <= kMost,
+         "gated block: w_gate must be (N, K) for x (..., K), with N, K and the rows of x at most 2^30");
     want(goes_with(w_gate, x, {n, k}) && goes_with(w_up, x, {n, k}), "gated block: w_gate and w_up must be contiguous, alike, of x's type and on its device");
 }
 
@@ -280,8 +282,8 @@ struct GatedFeedForward : torch::autograd::Function<GatedFeedForward> {
 
 Tensor gated_feed_forward(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Tensor &w_down, int64_t activation) {
     check_gated(x, w_gate, w_up);
-    want(w_down.dim() == 2 && w_down.size(0) >= 1 && goes_with(w_down, x, {w_down.size(0), w_gate.size(0)}),
-         "gated_feed_forward: w_down must be (M, N), contiguous, of x's type and on its device");
+    want(w_down.dim() == 2 && w_down.size(0) >= 1 && w_down.size(0) <= kMost && goes_with(w_down, x, {w_down.size(0), w_gate.size(0)}),
+         "gated_feed_forward: w_down must be (M, N), M at most 2^30, contiguous, of x's type and on its device");
     if (tracked(x, w_gate, w_up, w_down)) return GatedFeedForward::apply(x, w_gate, w_up, w_down, activation);
     Tensor h;
     return block_forward(x, w_gate, w_up, w_down, activation, false, &h);
