@@ -76,6 +76,13 @@ struct Place {
     explicit Place(const Tensor &t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
 };
 
+// Forward-mode differentiation would lose its tangents on the direct path, silently: refused whether or not gradients are recorded.
+template <typename... T>
+void refuse_tangents(const T &...t) {
+    if ((... || (t.defined() && t._fw_grad(/*level=*/0).defined())))
+        throw std::runtime_error("forward-mode differentiation (torch.autograd.forward_ad) is not available for this operator");
+}
+
 // Whether anything is to be differentiated.
 template <typename... T>
 bool tracked(const T &...t) {
@@ -155,6 +162,7 @@ Tensor layernorm_rows(const Tensor &x, double eps, const Tensor &weight, const s
     want(goes_with(weight, x, {n}), "layernorm_rows: weight must be contiguous, (n), of x's type and on its device");
     want(!bias || goes_with(*bias, x, {n}), "layernorm_rows: bias must be contiguous, (n), of x's type and on its device");
     const Tensor b = bias ? *bias : Tensor();
+    refuse_tangents(x, weight, b);
     if (tracked(x, weight, b)) return LayerNormRows::apply(x, weight, bias, eps, rd_mean);
     return layernorm_forward(x, weight, b, eps, rd_mean, nullptr);
 }
@@ -227,6 +235,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 
 Tensor gated_linear(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, int64_t activation) {
     check_gated(x, w_gate, w_up);
+    refuse_tangents(x, w_gate, w_up);
     if (tracked(x, w_gate, w_up)) return GatedLinear::apply(x, w_gate, w_up, activation);
     return gated_forward(x, w_gate, w_up, activation, nullptr);
 }
@@ -284,6 +293,7 @@ Tensor gated_feed_forward(const Tensor &x, const Tensor &w_gate, const Tensor &w
     check_gated(x, w_gate, w_up);
     want(w_down.dim() == 2 && w_down.size(0) >= 1 && w_down.size(0) <= kMost && goes_with(w_down, x, {w_down.size(0), w_gate.size(0)}),
          "gated_feed_forward: w_down must be (M, N), M at most 2^30, contiguous, of x's type and on its device");
+    refuse_tangents(x, w_gate, w_up, w_down);
     if (tracked(x, w_gate, w_up, w_down)) return GatedFeedForward::apply(x, w_gate, w_up, w_down, activation);
     Tensor h;
     return block_forward(x, w_gate, w_up, w_down, activation, false, &h);

@@ -4,7 +4,7 @@ What a caller of cpm_kernels composes from ``bmm`` (torch/gemm.py:233-239), ``ge
 with both projections, the activation and the product in one pass, and the activation's derivative in the epilogue of the product
 before it on the way back.  fp16 and bf16, fp32 sums.
 
-N, K, M and the rows of x are at most 2^30 each.
+N, K, M and the rows of x are at most 2^30 each.  Forward-mode differentiation raises a RuntimeError.
 
 The first call on a device is made outside a CUDA-graph capture (it allocates the library's status word); after that calls may be
 captured, the backward pass too.  As with PyTorch's own operators, a backward pass is captured only while no graph of an earlier,

@@ -11,7 +11,7 @@ from ._ext import ext
 def layernorm_rows(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, rd_mean: bool = True) -> torch.Tensor:
     """Layer norm of ``x`` (..., n) over its last axis, times ``weight`` (n), plus ``bias`` (n) if given; ``rd_mean`` False leaves the
     mean in (the RMS form).  fp16, bf16 or fp32, the same type for all three; statistics in fp32.  Differentiable in x, weight and bias
-    (once).  Any n >= 1 and any number of rows, none included.
+    (once; forward-mode differentiation raises a RuntimeError).  Any n >= 1 and any number of rows, none included.
 
     Calls may be captured into a CUDA graph, the backward pass too.  As with PyTorch's own operators, a backward pass is captured only
     while no graph of an earlier, uncaptured call on the same leaves is alive: PyTorch ties a leaf's gradient to the stream of that call."""

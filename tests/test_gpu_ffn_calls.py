@@ -1,10 +1,22 @@
 """Calls of the row layer norm and the gated feed-forward block at the edges of what their documentation allows."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import cpm_kernels_b200.torch as ct
 
 pytestmark = pytest.mark.gpu
+OPERATORS = ["layernorm_rows", "gated_linear", "gated_feed_forward"]
+
+
+def operands_of(name, tokens=6):
+    """Small fp16 operands of an operator, and the call that takes them."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    r = lambda *s: (torch.randn(*s, generator=g, device="cuda") * 0.3).half()
+    if name == "layernorm_rows":
+        return [r(tokens, 64), 1 + r(64), r(64)], lambda x, w, b: ct.layernorm_rows(x, 1e-5, w, b)
+    operands = [r(tokens, 64), r(72, 64), r(72, 64), r(40, 72)]
+    return (operands[:3], ct.gated_linear) if name == "gated_linear" else (operands, ct.gated_feed_forward)
 
 
 @pytest.mark.parametrize("which", ["k", "n", "m"])
@@ -17,3 +29,18 @@ def test_extents_beyond_32_bits_are_refused(which):
     if which != "m":
         with pytest.raises(AssertionError):
             ct.gated_linear(x, w, w)
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_forward_mode_differentiation_is_refused(name):
+    """A tangent on any one operand: an error, not an output without a tangent."""
+    operands, call = operands_of(name)
+    want = call(*operands)
+    for i in range(len(operands)):
+        with forward_ad.dual_level():
+            duals = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(operands)]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(*duals)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(*duals)
+            assert torch.equal(call(*operands), want)    # others are not concerned
