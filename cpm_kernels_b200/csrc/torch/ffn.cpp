@@ -89,18 +89,18 @@ bool tracked(const T &...t) {
     return at::GradMode::is_enabled() && (... || (t.defined() && t.requires_grad()));
 }
 
-// What is returned while a graph of the gradients is asked for raises when that graph is differentiated: once is all there is.
+// A gradient that is returned while a graph of the gradients is asked for (create_graph) raises when it is differentiated again: once is all
+// there is.  `on`: the tensors that it is computed from.  Where none of them requires a gradient it is a constant, and stays one; the
+// incoming gradient alone does not tell (that of y.sum() requires none, but dx depends on x and the weights all the same).
 struct Once : torch::autograd::Function<Once> {
     static Tensor forward(AutogradContext *, const Tensor &g) { return g.view_as(g); }
     static variable_list backward(AutogradContext *, variable_list) {
         throw std::runtime_error("trying to differentiate twice a function that is differentiable once");
     }
 };
-variable_list once(variable_list grads, const variable_list &from) {
-    if (!at::GradMode::is_enabled() || !from[0].defined() || !from[0].requires_grad()) return grads;
-    for (Tensor &g : grads)
-        if (g.defined()) g = Once::apply(g.detach().requires_grad_(true));
-    return grads;
+template <typename... T>
+Tensor once(const Tensor &g, const T &...on) {
+    return g.defined() && tracked(on...) ? Once::apply(g.detach().requires_grad_(true)) : g;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -148,7 +148,7 @@ struct LayerNormRows : torch::autograd::Function<LayerNormRows> {
         check(api.layernorm_rows_backward((int32_t)rows, (int32_t)n, dtype_of(x), dy.data_ptr(), x.data_ptr(), ctx->saved_data["rd_mean"].toBool(),
                                           weight.data_ptr(), mean, mean + rows, address(dx), address(dweight), address(dbias), address(scratch), place.stream),
               "cpmk_layernorm_rows_backward");
-        return once({dx, dweight, dbias, Tensor(), Tensor()}, grads);
+        return {once(dx, grads[0], x, weight), once(dweight, grads[0], x), once(dbias, grads[0]), Tensor(), Tensor()};
     }
 };
 
@@ -229,7 +229,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
                                         x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), part(gu, 0), part(gu, 1), part(dgu, 0), part(dgu, 1), address(dx),
                                         address(dw_gate), address(dw_up), address(scratch), place.stream),
               "cpmk_gated_linear_backward");
-        return once({dx, dw_gate, dw_up, Tensor()}, grads);
+        return {once(dx, grads[0], x, w_gate, w_up), once(dw_gate, grads[0], x, w_gate, w_up), once(dw_up, grads[0], x, w_gate), Tensor()};
     }
 };
 
@@ -285,7 +285,8 @@ struct GatedFeedForward : torch::autograd::Function<GatedFeedForward> {
                                               part(hgu, 0), part(dgu, 0), part(dgu, 1), address(dx), address(dw_gate), address(dw_up), address(dw_down),
                                               address(scratch), place.stream),
               "cpmk_gated_feed_forward_backward");
-        return once({dx, dw_gate, dw_up, dw_down, Tensor()}, grads);
+        return {once(dx, grads[0], x, w_gate, w_up, w_down), once(dw_gate, grads[0], x, w_gate, w_up, w_down), once(dw_up, grads[0], x, w_gate, w_down),
+                once(dw_down, grads[0], x, w_gate, w_up), Tensor()};
     }
 };
 

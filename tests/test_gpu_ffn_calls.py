@@ -44,3 +44,32 @@ def test_forward_mode_differentiation_is_refused(name):
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 call(*duals)
             assert torch.equal(call(*operands), want)    # others are not concerned
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+@pytest.mark.parametrize("dy_requires_grad", [False, True])
+def test_a_gradient_is_not_differentiated_again(name, dy_requires_grad):
+    """A penalty on a gradient raises, beside another loss too; it must not count as a constant."""
+    operands, call = operands_of(name)
+    operands = [t.requires_grad_() for t in operands]
+    y = call(*operands)
+    dy = torch.ones_like(y).requires_grad_(dy_requires_grad)
+    plain = torch.autograd.grad(y, operands, dy.detach(), retain_graph=True)
+    for i, (g, p) in enumerate(zip(torch.autograd.grad(y, operands, dy, create_graph=True), plain)):
+        assert torch.equal(g, p)
+        if name == "layernorm_rows" and i == 2 and not dy_requires_grad:
+            assert not g.requires_grad                   # dbias is the sum of dy: a constant
+            continue
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (y.sum() + g.square().sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_gradients_of_some_operands_with_a_graph_of_them(name):
+    """Only one operand requires a gradient: its gradient depends on itself, or on constants only (then it is one)."""
+    constants = {"layernorm_rows": (1, 2), "gated_linear": (2,), "gated_feed_forward": (2, 3)}[name]
+    for i in range(len(operands_of(name)[0])):
+        operands, call = operands_of(name)
+        y = call(*[t.requires_grad_(j == i) for j, t in enumerate(operands)])
+        (g,) = torch.autograd.grad(y, operands[i], torch.ones_like(y), create_graph=True)
+        assert g.requires_grad == (i not in constants)
