@@ -111,16 +111,96 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Sum over the threads that share a row (a warp, or the block); every thread gets it.  `red`: one float per warp, not written again
-// before the block's next barrier but one (callers alternate between two arrays), so one barrier per sum is enough.
-template <bool BLOCK>
+// The sums of up to four warps of a block, read by everyone.
+__device__ __forceinline__ float four_warps(const float *red) {
+    const float4 v = *reinterpret_cast<const float4 *>(red);
+    return (v.x + v.y) + (v.z + v.w);
+}
+
+// Sum over the threads that share a row (a warp, or the block, of MOST threads at most); every thread gets it.  `red`: one float per warp,
+// not written again before the block's next barrier but one (callers alternate between two arrays), so one barrier per sum is enough.
+// MOST = 128: `red` is 16-byte aligned, and zero behind the block's last warp.
+template <bool BLOCK, int MOST>
 __device__ __forceinline__ float row_sum(float v, float *red) {
     v = warp_sum(v);
     if (!BLOCK) return v;
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
+    if (MOST == 128) return four_warps(red);
     return warp_sum(lane < warps ? red[lane] : 0.f);
+}
+// The sum over a block and what its rounding left out, where the warps' sums are exact: their upper 12 bits and the rest are added up apart,
+// each without rounding.  Of up to 16 warps, the lower lanes add up the one and the upper lanes the other.
+template <int MOST>
+__device__ __forceinline__ float2 row_sum_and_rest(float v, float *red) {
+    v = warp_sum(v);
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, from = MOST > 512 ? lane : lane & 15;
+    if (lane == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = from < warps ? red[from] : 0.f;
+    float high = __uint_as_float(__float_as_uint(v) & 0xfffff000u), low = v - high;
+    if (MOST > 512) {
+        high = warp_sum(high);
+        low = warp_sum(low);
+    } else {
+        v = lane & 16 ? low : high;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        low = __shfl_xor_sync(0xffffffffu, v, 16);
+        high = lane & 16 ? low : v;
+        low = lane & 16 ? v : low;
+    }
+    const float sum = high + low;
+    return make_float2(sum, (high - sum) + low);
+}
+// Two sums at a time.  Of up to 16 warps, the lower lanes add up one and the upper ones the other.
+template <bool BLOCK, int MOST>
+__device__ __forceinline__ float2 row_sums(float a, float b, float (*red)[32]) {
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (!BLOCK) return make_float2(a, b);
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) {
+        red[0][threadIdx.x >> 5] = a;
+        red[1][threadIdx.x >> 5] = b;
+    }
+    __syncthreads();
+    if (MOST == 128) return make_float2(four_warps(red[0]), four_warps(red[1]));
+    if (MOST > 512) return make_float2(warp_sum(lane < warps ? red[0][lane] : 0.f), warp_sum(lane < warps ? red[1][lane] : 0.f));
+    float v = (lane & 15) < warps ? red[lane >> 4][lane & 15] : 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const float w = __shfl_xor_sync(0xffffffffu, v, 16);
+    return lane & 16 ? make_float2(w, v) : make_float2(v, w);
+}
+
+// A row's mean is rounded, and the deviations d from it are off by what it is off by, `off`: some 2^-24 of the values, far more than the
+// spread of a row whose values are alike (1000 times 1000.0, mean by a reciprocal: 6e-5, and y 0.02 for 0).  So the variance is
+// mean(d^2) - off^2 and y = (d - off) r w + b.  Where off comes from:
+//   * 16-bit values that are alike are 12 bits in one unit.  A warp's 1024 of them at most have a sum that is exact, a block's 4096 too, and of
+//     more row_sum_and_rest has what the rounding leaves out: off is what is left of the division, (sum + rest - n mean) / n.
+//     16384 x 4096 bf16 50.0 us with and without it, 30000 x 256 8.6 -> 9.0, 4096 x 8192 28.7 -> 30.4, 4096 x 4095 23.6 -> 24.9.
+//   * fp32 values, and the longest rows: off is the mean of the deviations, a sum of small numbers beside that of the squares.  8192 x 1024
+//     fp32 13.3 -> 13.5 us, 8192 x 1023 18.5 -> 20.7; as the only way it took 16384 x 4096 bf16 from 50 to 55, and so did a branch for
+//     the rows that need it.
+struct Spread {
+    float off, rstd;
+};
+template <bool BLOCK, int MOST, bool EXACT_SUM>
+__device__ __forceinline__ Spread spread_of(float left, float sum_d, float sum_d2, int rd_mean, float inv_n, float eps, float (*red)[32]) {
+    float off = 0.f, squares;
+    if (EXACT_SUM || !rd_mean) {
+        off = left * inv_n;                              // 0 without a mean
+        squares = row_sum<BLOCK, MOST>(sum_d2, red[0]);
+    } else {
+        const float2 s = row_sums<BLOCK, MOST>(sum_d, sum_d2, red);
+        off = s.x * inv_n;
+        squares = s.y;
+    }
+    // (a NaN stays in `off`; the squares of a row without a mean may be one)
+    const float variance = squares * inv_n, reduced = fmaf(-off, off, variance);
+    return {off, 1.f / sqrtf((off == 0.f ? variance : fmaxf(reduced, 0.f)) + eps)};
 }
 
 // Asks L2 for a row that the block reads next: one request per 128-byte line, no registers.
@@ -140,7 +220,11 @@ template <typename T, int VEC, int NV, bool BLOCK, int MOST, bool SHIFT>
 __global__ void __launch_bounds__(MOST, MOST == 1024 ? 1 : MOST == 512 ? (VEC * NV > 16 ? 1 : 2) : VEC * NV > 16 ? 5 : 8)
 ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_mean, const T *__restrict__ x, const T *__restrict__ w,
                        const T *__restrict__ b, T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-    __shared__ float red[2][2][32];
+    __shared__ __align__(16) float red[2][3][32];
+    if (BLOCK && MOST == 128) {
+        for (int i = threadIdx.x; i < 2 * 3 * 32; i += blockDim.x) red[0][0][i] = 0.f;
+        __syncthreads();
+    }
     const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, stride = (BLOCK ? blockDim.x : 32) * VEC;
     const int64_t first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int64_t step = BLOCK ? gridDim.x : (int64_t)gridDim.x * 4;
@@ -148,6 +232,7 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
     // SHIFT: weight and bias are gathered by element, once, and kept in the thread's own slots of shared memory (64 registers hold no more),
     // with four vectors a thread in registers (of which there are 128 then)
     constexpr bool kMany = MOST == 1024;
+    constexpr bool kExactSum = sizeof(T) == 2, kRest = kExactSum && BLOCK && MOST > 128;
     static_assert(!SHIFT || (BLOCK && MOST == 512), "shifted rows are a block's of 512 threads at most");
     constexpr bool kKeep = SHIFT && NV <= 2, kHold = SHIFT && NV > 2;
     __shared__ uint4 kept[kKeep ? 2 * NV : 1][kKeep ? 512 : 1];
@@ -177,7 +262,7 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
     if (first < rows) request(first);
     int parity = 0;
     for (int64_t row = first; row < rows; row += step, parity ^= 1) {
-        float v[NV][VEC], mean = 0.f;
+        float v[NV][VEC], mean = 0.f, left = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             clean<SHIFT>(in[j], t * VEC + j * stride - shift, n);
@@ -194,20 +279,33 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
             for (int j = 0; j < NV; ++j)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) s += v[j][e];
-            mean = row_sum<BLOCK>(s, red[parity][0]) * inv_n;
+            float rest = 0.f;
+            if constexpr (kRest) {
+                const float2 both = row_sum_and_rest<MOST>(s, red[parity][0]);
+                s = both.x;
+                rest = both.y;
+            } else {
+                s = row_sum<BLOCK, MOST>(s, red[parity][0]);
+            }
+            mean = s / (float)n;
+            left = fmaf(-mean, (float)n, s) + rest;
         }
-        float q = 0.f;
+        float d = 0.f, q = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const int i = t * VEC + j * stride - shift;
                 v[j][e] -= mean;
-                if (SHIFT ? i + e >= 0 && i + e < n : i < n) q = fmaf(v[j][e], v[j][e], q);
+                if (SHIFT ? i + e >= 0 && i + e < n : i < n) {
+                    d += v[j][e];
+                    q = fmaf(v[j][e], v[j][e], q);
+                }
             }
-        const float rstd = 1.f / sqrtf(row_sum<BLOCK>(q, red[parity][1]) * inv_n + eps);
+        const Spread spread = spread_of<BLOCK, MOST, kExactSum>(left, d, q, rd_mean, inv_n, eps, red[parity] + 1);
+        const float rstd = spread.rstd, back = rd_mean ? -spread.off * rstd : 0.f;
         if (t == 0 && rstd_out) {
-            mean_out[row] = mean;
+            mean_out[row] = mean + spread.off;
             rstd_out[row] = rstd;
         }
 #pragma unroll
@@ -227,7 +325,7 @@ ln_rows_forward_kernel(int32_t rows, int32_t n, float inv_n, float eps, int rd_m
                 else pb.clear();
             }
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf(v[j][e] * rstd, to_f32(pw.v[e]), to_f32(pb.v[e])));
+            for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf(fmaf(v[j][e], rstd, back), to_f32(pw.v[e]), to_f32(pb.v[e])));
             store_part<SHIFT>(out, y + row * n, i, n);
         }
         if (kMany && row + step < rows) request(row + step);
@@ -240,7 +338,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(kWideThreads) ln_rows_forward_wide_kernel(int32_t n, float inv_n, float eps, int rd_mean, const T *__restrict__ x,
                                                                             const T *__restrict__ w, const T *__restrict__ b, T *__restrict__ y,
                                                                             float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-    __shared__ float red[2][32];
+    __shared__ float red[3][32];
     const int64_t row = blockIdx.x;
     const T *xr = x + row * n;
     const int32_t first = threadIdx.x * VEC, step = kWideThreads * VEC;
@@ -253,21 +351,23 @@ __global__ void __launch_bounds__(kWideThreads) ln_rows_forward_wide_kernel(int3
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s += to_f32(px.v[e]);
         }
-        mean = row_sum<true>(s, red[0]) * inv_n;
+        mean = row_sum<true, kWideThreads>(s, red[0]) / (float)n;
     }
-    float q = 0.f;
+    float sum_d = 0.f, q = 0.f;
     for (int32_t i = first; i < n; i += step) {
         Pack<T, VEC> px;
         px.load(xr + i);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const float d = to_f32(px.v[e]) - mean;
+            sum_d += d;
             q = fmaf(d, d, q);
         }
     }
-    const float rstd = 1.f / sqrtf(row_sum<true>(q, red[1]) * inv_n + eps);
+    const Spread spread = spread_of<true, kWideThreads, false>(0.f, sum_d, q, rd_mean, inv_n, eps, red + 1);
+    const float rstd = spread.rstd, back = rd_mean ? -spread.off * rstd : 0.f;
     if (threadIdx.x == 0 && rstd_out) {
-        mean_out[row] = mean;
+        mean_out[row] = mean + spread.off;
         rstd_out[row] = rstd;
     }
     for (int32_t i = first; i < n; i += step) {
@@ -277,7 +377,7 @@ __global__ void __launch_bounds__(kWideThreads) ln_rows_forward_wide_kernel(int3
         if (b) pb.load(b + i);
         else pb.clear();
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf((to_f32(px.v[e]) - mean) * rstd, to_f32(pw.v[e]), to_f32(pb.v[e])));
+        for (int e = 0; e < VEC; ++e) out.v[e] = from_f32<T>(fmaf(fmaf(to_f32(px.v[e]) - mean, rstd, back), to_f32(pw.v[e]), to_f32(pb.v[e])));
         out.store(y + row * n + i);
     }
 }
@@ -518,8 +618,8 @@ __global__ void __launch_bounds__(1024) ln_rows_backward_wide_kernel(int32_t row
                 s2 = fmaf(g, (to_f32(px.v[e]) - mean) * rstd, s2);
             }
         });
-        const float c1 = row_sum<true>(s1, red[0]) * (rd_mean ? inv_n : 0.f);
-        const float c2 = row_sum<true>(s2, red[1]) * inv_n;
+        const float c1 = row_sum<true, 1024>(s1, red[0]) * (rd_mean ? inv_n : 0.f);
+        const float c2 = row_sum<true, 1024>(s2, red[1]) * inv_n;
         walk([&](const Pack<T, VEC> &px, const Pack<T, VEC> &pd, const Pack<T, VEC> &pw, int32_t i) {
             Pack<T, VEC> out;
 #pragma unroll

@@ -73,3 +73,58 @@ def test_gradients_of_some_operands_with_a_graph_of_them(name):
         y = call(*[t.requires_grad_(j == i) for j, t in enumerate(operands)])
         (g,) = torch.autograd.grad(y, operands[i], torch.ones_like(y), create_graph=True)
         assert g.requires_grad == (i not in constants)
+
+
+def alike(n, t, kind):
+    """Rows of values that are alike: constant ones, and constant ones but for a few values a step of their type away."""
+    rows = []
+    for c in (1000.0, 2.0, 0.1, -777.7, 1025.0, 3.0e-5):
+        row = torch.full((n,), c, device="cuda", dtype=torch.float64).to(t)
+        if kind == "steps":
+            row[:: max(1, n // 3)] = (row[0].double() * (1 + torch.finfo(t).eps)).to(t)
+        rows.append(row)
+    return torch.stack(rows)
+
+
+@pytest.mark.parametrize("kind", ["constant", "steps"])
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [3, 41, 47, 256, 511, 1000, 1024, 1032, 2047, 2560, 4095, 4096, 5000, 5001, 8191, 8192, 12289, 16384, 20000, 20001, 32768, 33001, 66000])
+def test_rows_of_values_that_are_alike(n, t, kind):
+    """The rounding of the mean must not show.  With K = (n / 32 + 18) 2^-24 the relative error of a sum (32 or more threads share it, a tree
+    joins them) and o = K mean|x| r what the mean may be off by in units of the spread: what it is off by is known to K (1 + o), the spread
+    to K (1 + o^2), and three more roundings of 2^-24 follow; then y is rounded once.  Without that o itself would be the error.  Many
+    rows and few, so that all forms of the kernel are met; with and without a mean to take off; weight and bias."""
+    x = alike(n, t, kind)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    w, b = ((1 + 0.2 * torch.randn(n, generator=g, device="cuda")).to(t), torch.randn(n, generator=g, device="cuda").to(t))
+    d = x.double()
+    mean = d.mean(-1, keepdim=True)
+    r = 1 / ((d - mean).square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    xh, u = (d - mean) * r, 2.0 ** -24
+    want = xh * w.double() + b.double()
+    k = (n / 32 + 18) * u
+    o = k * d.abs().mean(-1, keepdim=True) * r
+    bound = w.double().abs() * (k * (1 + o) + (k * (1 + o * o) + 4 * u) * xh.abs() + 4 * u * o) + 2 * u * (want.abs() + (xh * w.double()).abs())
+    tol = bound + torch.finfo(t).eps / 2 * (want.abs() + bound) + 2.0 ** -25
+    for copies in (1, 250):
+        many = x.repeat(copies, 1) if copies * n < 5_000_000 else x
+        y = ct.layernorm_rows(many, 1e-5, w, b)
+        off = (y.double().view(-1, *x.shape) - want).abs()
+        assert (off <= tol).all(), "off by %.3g where %.3g is allowed" % (off.max(), tol.expand_as(off).flatten()[(off - tol).argmax()])
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [41, 1000, 4095, 5000, 12289, 20001, 33001])
+def test_gradients_of_constant_rows(n, t):
+    """xh = 0: dweight is zero, dx = r (g - mean g) with K as above for the sum of g."""
+    x = alike(n, t, "constant").requires_grad_()
+    g = torch.Generator(device="cuda").manual_seed(n)
+    w = (1 + 0.2 * torch.randn(n, generator=g, device="cuda")).to(t).requires_grad_()
+    dy = torch.randn(x.shape, generator=g, device="cuda").to(t)
+    dx, dw = torch.autograd.grad(ct.layernorm_rows(x, 1e-5, w), (x, w), dy)
+    assert not dw.any()
+    gw = dy.double() * w.detach().double()
+    r, k = 1e-5 ** -0.5, (n / 32 + 18) * 2.0 ** -24
+    want = r * (gw - gw.mean(-1, keepdim=True))
+    bound = r * k * (gw.abs() + gw.abs().mean(-1, keepdim=True))
+    assert ((dx.double() - want).abs() <= bound + torch.finfo(t).eps / 2 * (want.abs() + bound) + 2.0 ** -25).all()
