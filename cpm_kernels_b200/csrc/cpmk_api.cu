@@ -7,6 +7,7 @@
 #include <map>
 #include <mutex>
 #include <utility>
+#include <vector>
 
 #include "cpmk_common.cuh"
 
@@ -108,35 +109,78 @@ int32_t get_workspace(cudaStream_t stream, Workspace *ws) {
     return CPMK_OK;
 }
 
-constexpr int kMaxDevices = 64;
-static uint32_t *g_device_status[kMaxDevices];
+// Status words of calls that keep no workspace, a device's in one allocation.  Word 0: of captured calls, and of streams beyond kStatusWords.
+constexpr int kStatusWords = 4096;
+struct StatusWords {
+    uint32_t *words = nullptr;
+    int used = 1;
+    std::map<cudaStream_t, int> of;      // the streams' words
+    std::vector<int> released;
+};
+static std::map<int, StatusWords> g_status_words;
 
-int32_t get_device_status(uint32_t **status) {
+int32_t get_status_word(cudaStream_t stream, uint32_t **word) {
     int dev = 0;
     CPMK_CUDA_TRY(cudaGetDevice(&dev));
-    CPMK_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d is beyond the %d this library keeps a status word for", dev, kMaxDevices);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    CPMK_CUDA_TRY(cudaStreamIsCapturing(stream, &capture));
     std::lock_guard<std::mutex> lock(g_mutex);
-    if (!g_device_status[dev]) {
+    StatusWords &sw = g_status_words[dev];
+    if (!sw.words) {
         void *p = nullptr;
-        CPMK_CUDA_TRY(cudaMalloc(&p, 256));
-        const cudaError_t e = cudaMemset(p, 0, 256);
+        CPMK_CUDA_TRY(cudaMalloc(&p, kStatusWords * sizeof(uint32_t)));
+        const cudaError_t e = cudaMemset(p, 0, kStatusWords * sizeof(uint32_t));
         if (e != cudaSuccess) {
             (void)cudaFree(p);
-            set_error("clearing the device's status word failed: %s", cudaGetErrorString(e));
+            set_error("clearing the device's status words failed: %s", cudaGetErrorString(e));
             return CPMK_ECUDA;
         }
-        g_device_status[dev] = static_cast<uint32_t *>(p);
+        sw.words = static_cast<uint32_t *>(p);
     }
-    *status = g_device_status[dev];
+    int at = 0;
+    if (capture == cudaStreamCaptureStatusNone) {        // a graph may be replayed on any stream
+        const auto it = sw.of.find(stream);
+        if (it != sw.of.end()) {
+            at = it->second;
+        } else if (!sw.released.empty()) {
+            at = sw.of[stream] = sw.released.back();
+            sw.released.pop_back();
+        } else if (sw.used < kStatusWords) {
+            at = sw.of[stream] = sw.used++;
+        }
+    }
+    *word = sw.words + at;
     return CPMK_OK;
 }
 
-// Reads and clears the device's status word (0 when it has none yet).  The caller holds g_mutex and has synchronised.
-static int32_t collect_device_status(int dev, uint32_t *word) {
-    *word = 0;
-    if (dev < 0 || dev >= kMaxDevices || !g_device_status[dev]) return CPMK_OK;
-    CPMK_CUDA_TRY(cudaMemcpy(word, g_device_status[dev], sizeof(*word), cudaMemcpyDeviceToHost));
-    if (*word != 0) CPMK_CUDA_TRY(cudaMemset(g_device_status[dev], 0, 256));
+// Reads the current device's words (0 when it has none yet) and clears them.  The caller holds g_mutex and has synchronised the device.
+static int32_t collect_status_words(int dev, uint32_t *first) {
+    *first = 0;
+    const auto it = g_status_words.find(dev);
+    if (it == g_status_words.end() || !it->second.words) return CPMK_OK;
+    std::vector<uint32_t> words(it->second.used);
+    CPMK_CUDA_TRY(cudaMemcpy(words.data(), it->second.words, words.size() * sizeof(uint32_t), cudaMemcpyDeviceToHost));
+    for (uint32_t w : words)
+        if (*first == 0) *first = w;
+    if (*first != 0) CPMK_CUDA_TRY(cudaMemset(it->second.words, 0, words.size() * sizeof(uint32_t)));
+    return CPMK_OK;
+}
+
+// The word of a stream whose work is done, which is cleared, and the one of captured calls, which is left for the streams that are asked
+// after this one.  The caller holds g_mutex.
+static int32_t collect_status_of_stream(int dev, cudaStream_t stream, uint32_t *own, uint32_t *captured) {
+    *own = *captured = 0;
+    const auto it = g_status_words.find(dev);
+    if (it == g_status_words.end() || !it->second.words) return CPMK_OK;
+    const StatusWords &sw = it->second;
+    const auto at = sw.of.find(stream);
+    CPMK_CUDA_TRY(cudaMemcpyAsync(captured, sw.words, sizeof(uint32_t), cudaMemcpyDeviceToHost, stream));
+    if (at != sw.of.end()) CPMK_CUDA_TRY(cudaMemcpyAsync(own, sw.words + at->second, sizeof(uint32_t), cudaMemcpyDeviceToHost, stream));
+    CPMK_CUDA_TRY(cudaStreamSynchronize(stream));
+    if (*own != 0) {
+        CPMK_CUDA_TRY(cudaMemsetAsync(sw.words + at->second, 0, sizeof(uint32_t), stream));
+        CPMK_CUDA_TRY(cudaStreamSynchronize(stream));
+    }
     return CPMK_OK;
 }
 
@@ -184,7 +228,7 @@ int32_t cpmk_read_status(uint32_t *status_out) {
         if (word != 0 && worst == 0) worst = word;
     }
     uint32_t word = 0;
-    const int32_t rc = cpmk::collect_device_status(dev, &word);
+    const int32_t rc = cpmk::collect_status_words(dev, &word);
     if (rc) return rc;
     *status_out = worst ? worst : word;
     return CPMK_OK;
@@ -195,17 +239,22 @@ int32_t cpmk_check_stream(cpmk_stream_t stream) {
     CPMK_CUDA_TRY(cudaGetDevice(&dev));
     CPMK_CUDA_TRY(cudaStreamSynchronize(cpmk::as_stream(stream)));
     std::lock_guard<std::mutex> lock(cpmk::g_mutex);
-    uint32_t word = 0, of_device = 0;
+    uint32_t word = 0, own = 0, captured = 0;
     auto it = cpmk::g_workspaces.find(std::make_pair(dev, cpmk::as_stream(stream)));
     if (it != cpmk::g_workspaces.end()) {
         const int32_t rc = cpmk::collect_status(it->second, &word);
         if (rc) return rc;
     }
-    const int32_t rc = cpmk::collect_device_status(dev, &of_device);
+    const int32_t rc = cpmk::collect_status_of_stream(dev, cpmk::as_stream(stream), &own, &captured);
     if (rc) return rc;
-    if (word == 0) word = of_device;
+    if (word == 0) word = own;
     if (word != 0) {
         cpmk::set_error("a kernel on this stream gave up a bounded wait (code 0x%x); its output is incomplete", word);
+        return CPMK_EDEVICE;
+    }
+    if (captured != 0) {
+        cpmk::set_error("a kernel of a captured call gave up a bounded wait on this device, on this stream or another (code 0x%x); its output is "
+                        "incomplete; cpmk_read_status clears this", captured);
         return CPMK_EDEVICE;
     }
     return CPMK_OK;
@@ -217,6 +266,17 @@ int32_t cpmk_release_workspace(cpmk_stream_t stream) {
     cpmk::Workspace w;
     {
         std::lock_guard<std::mutex> lock(cpmk::g_mutex);
+        auto words = cpmk::g_status_words.find(dev);
+        if (words != cpmk::g_status_words.end()) {
+            cpmk::StatusWords &sw = words->second;
+            const auto at = sw.of.find(cpmk::as_stream(stream));
+            if (at != sw.of.end()) {
+                CPMK_CUDA_TRY(cudaDeviceSynchronize());
+                CPMK_CUDA_TRY(cudaMemset(sw.words + at->second, 0, sizeof(uint32_t)));
+                sw.released.push_back(at->second);
+                sw.of.erase(at);
+            }
+        }
         auto it = cpmk::g_workspaces.find(std::make_pair(dev, cpmk::as_stream(stream)));
         if (it == cpmk::g_workspaces.end()) return CPMK_OK;
         w = it->second;

@@ -72,9 +72,10 @@ int32_t current_device_info(DeviceInfo *info);
 // The workspace of (current device, stream); allocates it on first use.
 int32_t get_workspace(cudaStream_t stream, Workspace *ws);
 
-// The status word of the current device for kernels whose calls keep no workspace per stream (the gated feed-forward block): they may
-// be captured on a stream that has never been used.  Allocated on the device's first such call, which is made outside a capture.
-int32_t get_device_status(uint32_t **status);
+// The status word of (current device, stream) for kernels whose calls keep no workspace (the gated feed-forward block): they may be captured
+// on a stream that has never been used.  A captured call's is one word for the device, since the graph may be replayed on any stream.  The
+// words are allocated on the device's first such call, which is made outside a capture.
+int32_t get_status_word(cudaStream_t stream, uint32_t **word);
 
 // Element-wise GELU over `count` fp16 values (cpmk_gelu.cu); in == out is allowed.
 int32_t launch_gelu(int64_t count, const void *in, void *out, cudaStream_t stream);

@@ -637,10 +637,7 @@ int32_t launch(const Call &call, const TcMaps &maps, TcParams prm, const Plan &p
     return CPMK_OK;
 }
 
-int32_t prepare(TcParams *prm, const Plan &plan, void *scratch) {
-    uint32_t *status;
-    const int32_t rc = get_device_status(&status);
-    if (rc) return rc;
+int32_t prepare(const Call &call, TcParams *prm, const Plan &plan, void *scratch) {
     CPMK_REQUIRE(scratch || !plan.bytes, "scratch is needed");
     memset(prm, 0, sizeof(*prm));
     prm->blocks0 = (int32_t)plan.blocks0;
@@ -649,7 +646,7 @@ int32_t prepare(TcParams *prm, const Plan &plan, void *scratch) {
     prm->split_tiles = (int32_t)plan.split_tiles;
     prm->split_pairs = (int32_t)plan.split_pairs;
     prm->partial = static_cast<float *>(scratch);
-    prm->status = status;
+    prm->status = call.status;
     return CPMK_OK;
 }
 void add_product(TcParams *prm, int64_t R, int64_t C, int64_t width, bool p_t, bool q_t) {
@@ -686,7 +683,7 @@ int32_t tc_products(const Call &call, int32_t K, bool transposed, const Product 
     for (int i = 0; i < count; ++i) total += tiles_of(products[i].R, products[i].C, kTileC);
     const Plan plan = plan_of(call.info, total, K, 0);
     TcParams prm;
-    const int32_t rc = prepare(&prm, plan, scratch);
+    const int32_t rc = prepare(call, &prm, plan, scratch);
     if (rc) return rc;
     TcMaps maps;
     memset(&maps, 0, sizeof(maps));
@@ -710,7 +707,7 @@ int32_t tc_products(const Call &call, int32_t K, bool transposed, const Product 
 int32_t tc_sum(const Call &call, int32_t R, int32_t C, int32_t K, const void *p0, const void *q0, const void *p1, const void *q1, void *out, void *scratch) {
     const Plan plan = plan_of(call.info, tiles_of(R, C, kTileC), K, K);
     TcParams prm;
-    const int32_t rc = prepare(&prm, plan, scratch);
+    const int32_t rc = prepare(call, &prm, plan, scratch);
     if (rc) return rc;
     add_product(&prm, R, C, kTileC, false, true);
     TcMaps maps;
@@ -726,7 +723,7 @@ int32_t tc_gated(const Call &call, int32_t tokens, int32_t k, int32_t n, const v
                  void *scratch) {
     const Plan plan = plan_of(call.info, tiles_of(tokens, n, kTileC / 2), k, 0);
     TcParams prm;
-    const int32_t rc = prepare(&prm, plan, scratch);
+    const int32_t rc = prepare(call, &prm, plan, scratch);
     if (rc) return rc;
     add_product(&prm, tokens, n, kTileC / 2, false, false);
     prm.g = g;
@@ -749,7 +746,7 @@ int32_t tc_dact(const Call &call, int32_t tokens, int32_t n, int32_t m, const vo
                 void *scratch) {
     const Plan plan = plan_of(call.info, tiles_of(tokens, n, kTileC), m, 0);
     TcParams prm;
-    const int32_t rc = prepare(&prm, plan, scratch);
+    const int32_t rc = prepare(call, &prm, plan, scratch);
     if (rc) return rc;
     add_product(&prm, tokens, n, kTileC, false, true);
     prm.g = g;

@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(32) bounded_wait_selftest_kernel(uint64_t limi
         // phase 0 of a barrier that expects one arrival and gets none: the wait can only end by running out
         const bool ok = mbar_wait(smem_u32(&bar), 0u, &abort_word, status, kErrSelfTestWait, limit_ns);
         // 1: the wait gave up and raised the abort flag (expected); 2: it returned true (a bug); 3: gave up without the flag
-        *result = ok ? 2u : (abort_word ? 1u : 3u);
+        if (result) *result = ok ? 2u : (abort_word ? 1u : 3u);
     }
 }
 
@@ -53,5 +53,18 @@ extern "C" int32_t cpmk_selftest_bounded_wait(uint32_t limit_us, cpmk_stream_t s
         set_error("bounded-wait self-test: the kernel reported %u (1 = the wait ran out as it should)", verdict);
         return CPMK_EDEVICE;
     }
+    return CPMK_OK;
+}
+
+extern "C" int32_t cpmk_selftest_bounded_wait_gated(uint32_t limit_us, cpmk_stream_t stream) {
+    DeviceInfo info;
+    int32_t rc = current_device_info(&info);
+    if (rc) return rc;
+    CPMK_REQUIRE(limit_us >= 1 && limit_us <= 100000, "limit_us must be 1..100000 (got %u)", limit_us);
+    uint32_t *status;
+    rc = get_status_word(as_stream(stream), &status);
+    if (rc) return rc;
+    bounded_wait_selftest_kernel<<<1, 32, 0, as_stream(stream)>>>((uint64_t)limit_us * 1000ull, status, nullptr);
+    CPMK_LAUNCH_CHECK();
     return CPMK_OK;
 }

@@ -29,6 +29,7 @@ SIGNATURES = {
     "cpmk_check_stream": [_p],
     "cpmk_release_workspace": [_p],
     "cpmk_selftest_bounded_wait": [c_uint32, _p],
+    "cpmk_selftest_bounded_wait_gated": [c_uint32, _p],
     "cpmk_quantize_rows_pair_scatter": [_i, _p, _i, POINTER(c_void_p), POINTER(c_void_p), _i, _p, _p, _p, _i, _p],
     "cpmk_linear_int8_scatter": [_i, _i, _i, _p, _p, _p, _p, _p, _p, _i, POINTER(c_void_p), ctypes.c_int64, _i, _p],
     "cpmk_gemm_int8_dequant_multicast": [_i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _p, _p, ctypes.c_int64, _p],

@@ -6,7 +6,7 @@ before it on the way back.  fp16 and bf16, fp32 sums.
 
 N, K, M and the rows of x are at most 2^30 each.  Forward-mode differentiation raises a RuntimeError.
 
-The first call on a device is made outside a CUDA-graph capture (it allocates the library's status word); after that calls may be
+The first call on a device is made outside a CUDA-graph capture (it allocates the library's status words); after that calls may be
 captured, the backward pass too.  As with PyTorch's own operators, a backward pass is captured only while no graph of an earlier,
 uncaptured call on the same leaves is alive: PyTorch ties a leaf's gradient to the stream of that call."""
 import torch

@@ -63,14 +63,16 @@ int32_t cpmk_read_status(uint32_t *status_out);
 /* Waits for `stream`, then reports whether a kernel that ran on it gave up a bounded wait: CPMK_EDEVICE (with the
  * kernel's code in cpmk_last_error) if so, CPMK_OK otherwise.  After a failure the status word and the library's
  * ticket counters of that stream are cleared, so later calls on the stream work again; what the failed kernel should
- * have written is undefined.  Unlike cpmk_read_status it synchronises one stream, not the device.  No counterpart
- * in the reference. */
+ * have written is undefined.  Unlike cpmk_read_status it synchronises one stream, not the device.  A gated
+ * feed-forward call that was captured may run on any stream that replays the graph: its failure is reported for every
+ * stream of the device, until cpmk_read_status clears it.  No counterpart in the reference. */
 int32_t cpmk_check_stream(cpmk_stream_t stream);
 
 /* Frees the library's workspace of (current device, stream): call it before destroying a stream that ran calls which
  * use the workspace (int8 / fp16 GEMM, column quantisation, transposed GEMV, layer norm), so that a process that
  * creates and destroys streams does not accumulate 16 MiB per stream.  Waits for the device.  At most 256 streams per
- * device hold a workspace at a time (CPMK_ENOMEM beyond).  No counterpart in the reference. */
+ * device hold a workspace at a time (CPMK_ENOMEM beyond).  Gives back the stream's status word of gated feed-forward
+ * calls too.  No counterpart in the reference. */
 int32_t cpmk_release_workspace(cpmk_stream_t stream);
 
 /* Self-test of the give-up path of the library's device-side waits: a one-block kernel waits up to `limit_us`
@@ -78,6 +80,10 @@ int32_t cpmk_release_workspace(cpmk_stream_t stream);
  * recorded its code (0x901) in the stream's status word and returned; the next cpmk_check_stream on that stream
  * then returns CPMK_EDEVICE once.  Synchronises the stream.  No counterpart in the reference. */
 int32_t cpmk_selftest_bounded_wait(uint32_t limit_us, cpmk_stream_t stream);
+
+/* The same wait, its code recorded where a gated feed-forward call on this stream records its own.  Does not synchronise and
+ * may be captured.  No counterpart in the reference. */
+int32_t cpmk_selftest_bounded_wait_gated(uint32_t limit_us, cpmk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Quantisation passes (cuda/gemm.cu)
@@ -339,8 +345,8 @@ int32_t cpmk_layernorm_rows_backward(int32_t rows, int32_t n, int32_t dtype, con
  * ------------------------------------------------------------------------------------------
  * dtype is CPMK_F16 or CPMK_BF16 for every tensor of a call; products are accumulated in fp32.  Any sizes: extents k, n, m that are
  * multiples of 8 with 16-byte aligned pointers run on the tensor cores, others on a generic kernel.  Outputs must not overlap inputs.
- * The first call on a device is made outside a stream capture (it allocates the status word that cpmk_read_status and
- * cpmk_check_stream report: one per device); after that calls may be captured on any stream. */
+ * The first call on a device is made outside a stream capture (it allocates the status words that cpmk_read_status and
+ * cpmk_check_stream report); after that calls may be captured on any stream. */
 
 /* Bytes of device scratch that cpmk_gated_linear_forward (m = 0) and cpmk_gated_feed_forward_forward want for these sizes on the
  * current device (0: none).  `scratch` (16-byte aligned) is the caller's and not kept; calls that overlap need scratch of their own. */
