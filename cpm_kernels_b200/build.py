@@ -1,12 +1,13 @@
 """Builds ``lib/libcpmk_b200.so`` from ``csrc/*.cu`` and the loadable kernel modules ``lib/gemm.fatbin`` /
 ``lib/gemv.fatbin`` from ``csrc/modules/*_module.cu`` with nvcc for sm_100a (cross-compiles without a GPU), and the autograd module
-``lib/cpmk_torch.so`` from ``csrc/torch/ffn.cpp`` with the host compiler.
+``lib/cpmk_torch.*.so`` from ``csrc/torch/ffn.cpp`` with the host compiler, where PyTorch is installed.
 
 Usage: ``python -m cpm_kernels_b200.build [--force] [--verbose]``
 """
 from __future__ import annotations
 
 import glob
+import importlib.metadata
 import os
 import subprocess
 import sys
@@ -24,7 +25,21 @@ NVCC_FLAGS = [
 ]
 
 
-EXT_PATH = os.path.join(LIB_DIR, "cpmk_torch.so")
+def _torch_version() -> str | None:
+    """Of the installed PyTorch, which need not be imported for it; None without one."""
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return None
+
+
+def ext_path() -> str:
+    """Path of the autograd module for the running Python and the installed PyTorch, whose C++ interface it is compiled against: another
+    version of either asks for another file."""
+    return os.path.join(LIB_DIR, "cpmk_torch.%s.torch-%s.so" % (sys.implementation.cache_tag, _torch_version()))
+
+
+EXT_PATH = ext_path()
 EXT_SOURCE = os.path.join(CSRC, "torch", "ffn.cpp")
 
 MODULES = {"gemm": "gemm_module.cu", "gemv": "gemv_module.cu", "transpose": "transpose_module.cu"}
@@ -52,6 +67,8 @@ def _ext_inputs() -> list[str]:
 
 
 def _ext_is_stale() -> bool:
+    if _torch_version() is None:
+        return False                                     # nothing to compile it against; the library does not need it
     return not os.path.exists(EXT_PATH) or any(os.path.getmtime(p) > os.path.getmtime(EXT_PATH) for p in _ext_inputs())
 
 
@@ -83,7 +100,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     nvcc = os.environ.get("NVCC", "nvcc")
     os.makedirs(LIB_DIR, exist_ok=True)
     # the autograd module is compiled beside the library
-    ext_cmd = _ext_command() if force or _ext_is_stale() else None
+    ext_cmd = _ext_command() if _ext_is_stale() or (force and _torch_version()) else None
     ext = subprocess.Popen(ext_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) if ext_cmd else None
     try:
         _compile_cuda(nvcc, verbose)

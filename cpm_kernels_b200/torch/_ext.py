@@ -1,9 +1,11 @@
-"""Loads ``lib/cpmk_torch.so`` (csrc/torch/ffn.cpp: autograd of the row layer norm and the gated block in C++) and hands it the entry
-points of the C library that the ctypes layer has loaded."""
+"""``ext``: the autograd module ``lib/cpmk_torch.*.so`` (csrc/torch/ffn.cpp: autograd of the row layer norm and the gated block in C++) with
+the entry points of the C library that the ctypes layer has loaded.  Loaded on first use, so that a module that is missing or does not fit
+the installed PyTorch concerns these operators only."""
 import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import threading
 
 import torch  # noqa: F401  (its libraries are what the module links to)
 
@@ -26,4 +28,13 @@ def _load():
     return module
 
 
-ext = _load()
+_lock = threading.Lock()
+
+
+def __getattr__(name: str):
+    if name != "ext":
+        raise AttributeError("module %r has no attribute %r" % (__name__, name))
+    with _lock:
+        if "ext" not in globals():
+            globals()["ext"] = _load()
+    return globals()["ext"]

@@ -12,7 +12,7 @@ uncaptured call on the same leaves is alive: PyTorch ties a leaf's gradient to t
 import torch
 
 from ..library import cpmk
-from ._ext import ext
+from . import _ext
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "gelu") -> torch.Tensor:
@@ -20,7 +20,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     or "silu", applied to the fp32 sums.  fp16 or bf16.  Differentiable (once) in x and both weights; a call that is differentiated
     keeps the two projections, in the tensors' type."""
     assert activation in cpmk.ACTIVATIONS
-    return ext.gated_linear(x, w_gate, w_up, cpmk.ACTIVATIONS[activation])
+    return _ext.ext.gated_linear(x, w_gate, w_up, cpmk.ACTIVATIONS[activation])
 
 
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "gelu") -> torch.Tensor:
@@ -28,4 +28,4 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     The hidden activations between the two are rounded to the tensors' type.  Differentiable (once) in x and the three weights; a call
     that is differentiated keeps the two projections and the hidden activations."""
     assert activation in cpmk.ACTIVATIONS
-    return ext.gated_feed_forward(x, w_gate, w_up, w_down, cpmk.ACTIVATIONS[activation])
+    return _ext.ext.gated_feed_forward(x, w_gate, w_up, w_down, cpmk.ACTIVATIONS[activation])

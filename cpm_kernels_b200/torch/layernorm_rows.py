@@ -5,7 +5,7 @@ from typing import Optional
 
 import torch
 
-from ._ext import ext
+from . import _ext
 
 
 def layernorm_rows(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, rd_mean: bool = True) -> torch.Tensor:
@@ -15,4 +15,4 @@ def layernorm_rows(x: torch.Tensor, eps: float, weight: torch.Tensor, bias: Opti
 
     Calls may be captured into a CUDA graph, the backward pass too.  As with PyTorch's own operators, a backward pass is captured only
     while no graph of an earlier, uncaptured call on the same leaves is alive: PyTorch ties a leaf's gradient to the stream of that call."""
-    return ext.layernorm_rows(x, eps, weight, bias, rd_mean)
+    return _ext.ext.layernorm_rows(x, eps, weight, bias, rd_mean)

@@ -60,3 +60,39 @@ def test_a_missing_autograd_module_fails_loudly(monkeypatch, tmp_path):
     monkeypatch.setattr(_ext, "EXT_PATH", str(tmp_path / "nope.so"))
     with pytest.raises(RuntimeError, match="no fallback"):
         _ext._load()
+
+
+def test_another_pytorch_asks_for_another_autograd_module(built_library, monkeypatch):
+    from cpm_kernels_b200 import build
+    assert build.EXT_PATH == build.ext_path() and not build._ext_is_stale()
+    monkeypatch.setattr(build, "_torch_version", lambda: "0.0.1")
+    assert build.ext_path() != build.EXT_PATH
+    monkeypatch.setattr(build, "EXT_PATH", build.ext_path())
+    assert build._ext_is_stale() and build.is_stale()
+    monkeypatch.setattr(build, "_torch_version", lambda: None)
+    assert not build._ext_is_stale()                     # no PyTorch: the library alone
+
+
+def test_the_other_operators_do_not_need_the_autograd_module(built_library, tmp_path):
+    import os
+    import subprocess
+    import sys
+    script = """
+import cpm_kernels_b200.build as build
+build.EXT_PATH = %r
+import cpm_kernels_b200.torch as ct
+assert ct.bmm and ct.gelu and ct.transpose
+import torch
+for call in (lambda: ct.layernorm_rows(torch.ones(4), 1e-5, torch.ones(4)), lambda: ct.gated_linear(torch.ones(4), torch.ones(4, 4), torch.ones(4, 4))):
+    try:
+        call()
+    except %s as e:
+        continue
+    raise SystemExit("the call went through without its module")
+"""
+    broken = tmp_path / "broken.so"
+    broken.write_bytes(b"not a shared library")
+    for path, error in ((str(tmp_path / "nope.so"), "RuntimeError"), (str(broken), "ImportError")):
+        done = subprocess.run([sys.executable, "-c", script % (path, error)], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                              capture_output=True, text=True)
+        assert done.returncode == 0, done.stderr
