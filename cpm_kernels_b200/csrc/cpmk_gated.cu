@@ -1,6 +1,10 @@
 // Gated feed-forward block: h = act(x Wg^T) * (x Wu^T), y = h Wd^T, and its backward pass, in fp16 and bf16 with fp32 sums.
 //
 //   backward   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
+// Rounded to 16 bits on the way, once each: h, dg and du, because they are operands of the 16-bit products behind them (an operand in fp32
+// would be two of them, and twice the products); g and u for the backward pass, because fp32 would double what a step keeps.  dh never
+// leaves the chip.  Measured against 64 bits, in roundings of the result: y 1.4, gradients up to 1.9 (independent errors of as many
+// roundings as each has behind it: sqrt 2 for y; g, u, dg and its own for dw_gate).
 #include "cpmk_gated.cuh"
 
 namespace cpmk {

@@ -36,6 +36,11 @@ __device__ __forceinline__ F2 operator*(F2 a, F2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
     F2 r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
@@ -54,22 +59,43 @@ __device__ __forceinline__ F2 logistic2(F2 minus_z_log2e) {
 
 constexpr float kLog2e = 1.4426950408889634f, kGeluTwoC = 1.5957691216057308f, kGeluCube = 0.044715f;
 
-// act(v); SLOPE: and act'(v)
+// the larger and the smaller of two values, NaN if one is
+__device__ __forceinline__ float larger_of(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float smaller_of(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// act(v); SLOPE: and act'(v), of a v that was stored in 16 bits: beyond 65504 an fp16 one is infinite, though it was not when h was worked
+// out.  Both have their limits there (0 and 0, infinity and 1), not the NaN of 0 times infinity: v is held above -L, where s is 0 already
+// (L = 30, silu 128), and the v of the slope's second term below L, where 1 - s is.
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ void act2(F2 v, F2 &value, F2 &slope) {
-    F2 s, dz = f2(1.f);
+    constexpr float kLimit = ACT == CPMK_ACT_SILU ? 128.f : 30.f;
+    float2 x = both(v);
+    if (SLOPE) {
+        x = make_float2(larger_of(x.x, -kLimit), larger_of(x.y, -kLimit));
+        v = f2(x.x, x.y);
+    }
+    F2 s, c = v, dz = f2(1.f);
     if (ACT == CPMK_ACT_SILU) {
         s = logistic2(v * f2(-kLog2e));
     } else {
-        const float2 x = both(v);
-        const F2 c = f2(fminf(fmaxf(x.x, -30.f), 30.f), fminf(fmaxf(x.y, -30.f), 30.f)), c2 = c * c;
+        c = f2(smaller_of(larger_of(x.x, -kLimit), kLimit), smaller_of(larger_of(x.y, -kLimit), kLimit));
+        const F2 c2 = c * c;
         s = logistic2(c * fma2(c2, f2(-kLog2e * kGeluTwoC * kGeluCube), f2(-kLog2e * kGeluTwoC)));
         if (SLOPE) dz = fma2(c2, f2(3.f * kGeluTwoC * kGeluCube), f2(kGeluTwoC));
     }
     value = v * s;
     if (SLOPE) {
-        const F2 rest = value * fma2(s, f2(-1.f), f2(1.f));          // v s (1 - s)
-        slope = ACT == CPMK_ACT_SILU ? fma2(rest, f2(1.f), s) : fma2(rest, dz, s);
+        if (ACT == CPMK_ACT_SILU) c = f2(smaller_of(x.x, kLimit), smaller_of(x.y, kLimit));
+        const F2 rest = c * s * fma2(s, f2(-1.f), f2(1.f));          // v s (1 - s)
+        slope = ACT == CPMK_ACT_SILU ? rest + s : fma2(rest, dz, s);
     }
 }
 template <int ACT>

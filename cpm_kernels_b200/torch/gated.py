@@ -4,6 +4,10 @@ What a caller of cpm_kernels composes from ``bmm`` (torch/gemm.py:233-239), ``ge
 with both projections, the activation and the product in one pass, and the activation's derivative in the epilogue of the product
 before it on the way back.  fp16 and bf16, fp32 sums.
 
+What is handed from one product to the next, or kept for the backward pass, has the tensors' type, its precision and its range: in fp16,
+hidden activations beyond 65504 are infinite, kept projections too (for the gate's, the activation's limits are taken: 0, or infinity with
+slope 1), and the gradients of the projections are zero below 2^-25, as between operators of their own.  bf16 has the range of fp32.
+
 N, K, M and the rows of x are at most 2^30 each.  Forward-mode differentiation raises a RuntimeError.
 
 The first call on a device is made outside a CUDA-graph capture (it allocates the library's status words); after that calls may be

@@ -128,3 +128,45 @@ def test_gradients_of_constant_rows(n, t):
     want = r * (gw - gw.mean(-1, keepdim=True))
     bound = r * k * (gw.abs() + gw.abs().mean(-1, keepdim=True))
     assert ((dx.double() - want).abs() <= bound + torch.finfo(t).eps / 2 * (want.abs() + bound) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("tokens,k,n,m", [(5, 64, 72, 40), (300, 64, 72, 40), (300, 64, 136, 4096), (700, 64, 512, 64), (7, 5, 3, 2)])
+def test_gate_projections_beyond_the_range_of_fp16(tokens, k, n, m, act):
+    """A gate projection of -120000 is kept as minus infinity.  The activation and its slope are zero there as they are at -60000, so
+    the hidden activations and all gradients are those of a call whose projection is -60000; at +120000 the slope is 1 as at +60000."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    wg, wu, wd = ((r(n, k) / k ** 0.5).half(), (r(n, k) / k ** 0.5).half(), (r(m, n) / n ** 0.5).half())
+    wg[:, 0] = -2.0
+    wu[:, 0] = 2.0 ** -6
+    dy, dh, x = r(tokens, m).half(), r(tokens, n).half(), r(tokens, k).half()
+    x[1] = 0
+
+    def step(size):
+        inputs = x.clone()
+        inputs[1, 0] = size
+        ts = [t.clone().requires_grad_() for t in (inputs, wg, wu, wd)]
+        y, h = ct.gated_feed_forward(*ts, activation=act), ct.gated_linear(*ts[:3], activation=act)
+        return (y.detach(), h.detach(), *torch.autograd.grad(y, ts, dy), *torch.autograd.grad(h, ts[:3], dh))
+
+    for got, want in zip(step(60000.0), step(30000.0)):
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+
+    # g = 120000: dg = dh u (du is infinite), seen in the gradient of w_gate, dg^T x
+    ts = [t.clone().requires_grad_() for t in (-60000.0 * torch.eye(1, k, device="cuda").half(), wg, wu * 2.0 ** -8)]
+    (dwg,) = torch.autograd.grad(ct.gated_linear(*ts, activation=act), ts[1], dh[:1] * 2.0 ** -8)
+    u = (ts[0].detach().double() @ ts[2].detach().double().T).half().double()
+    dg = ((dh[:1] * 2.0 ** -8).double() * u).half().double()
+    assert torch.equal(dwg.double(), (dg.T @ ts[0].detach().double()).half().double())
+
+
+@pytest.mark.parametrize("tokens", [3, 300])
+def test_hidden_activations_have_the_range_of_their_type(tokens):
+    """act(g) u = 260 * 260 is beyond fp16 and infinite there, and not in bf16."""
+    for t, infinite in ((torch.float16, True), (torch.bfloat16, False)):
+        x = torch.ones((tokens, 8), device="cuda", dtype=t)
+        w, w_down = torch.full((16, 8), 32.5, device="cuda", dtype=t), torch.full((8, 16), 2.0 ** -10, device="cuda", dtype=t)
+        assert torch.isinf(ct.gated_linear(x, w, w)).all() == infinite
+        y = ct.gated_feed_forward(x, w, w, w_down)
+        assert torch.isinf(y).all() if infinite else (y - 260.0 * 260 * 16 / 1024).abs().max() <= 1056 * 2.0 ** -7
