@@ -765,14 +765,30 @@ int backward_blocks(const DeviceInfo &info, int32_t rows, const Layout &l) {
     const int64_t blocks = ceil_div64(rows, warps ? 32 : 4), held = (int64_t)info.sm_count * (threads >= most ? 1 : most / threads);
     return (int)(blocks < held ? blocks : held);
 }
-// room for the partial rows of any type and alignment
-int64_t most_backward_blocks(const DeviceInfo &info, int32_t rows, int32_t n) {
-    int64_t most = 0;
-    for (const Layout &l : {backward_layout(info, rows, n, 8, true), backward_layout(info, rows, n, 4, true), backward_layout(info, rows, n, 8, false)})
-        most = std::max<int64_t>(most, backward_blocks(info, rows, l));
+int32_t column_pitch(int32_t n) { return (n + 31) / 32 * 32; }
+
+// Whether dw and db take a pass of their own.  Beside a row in shared memory (one pass) -> pass of their own, bf16 or fp16: 2048 x 16384
+// 73.7 -> 68.7 us, 2048 x 8200 47.9 -> 46.2, 20 x 16384 24.0 -> 15.9; the rows move half the bytes of their sums there.  fp32 rows and single
+// elements keep to one pass (2048 x 8192 fp32 43.0 against 61, 2048 x 12289 bf16 63.5 against 88).
+constexpr bool sums_beside_vectors(int element_size) { return element_size == 4; }
+bool strips_for(const Layout &l, int element_size) { return l.threads == 0 || (l.threads == 1024 && l.vec > 1 && !sums_beside_vectors(element_size)); }
+// Rows of partial sums: one per block, of that pass as many as fill the SMs with strips of `vec` columns a thread, no more than that.
+int partial_rows(const DeviceInfo &info, int32_t rows, int32_t n, const Layout &l, int element_size, int vec) {
+    const int blocks = backward_blocks(info, rows, l);
+    if (!strips_for(l, element_size)) return blocks;
+    return (int)std::min<int64_t>(blocks, std::max<int64_t>(1, 8 * info.sm_count / ceil_div64(n, kStripThreads * vec)));
+}
+// room for those of any type and alignment
+int64_t most_partial_rows(const DeviceInfo &info, int32_t rows, int32_t n) {
+    int most = 0;
+    for (const int element_size : {2, 4})
+        for (const bool aligned : {false, true})
+            for (const bool strip_aligned : {false, true}) {
+                const int per_vector = 16 / element_size, vec = strip_aligned && n % per_vector == 0 ? per_vector : 1;
+                most = std::max(most, partial_rows(info, rows, n, backward_layout(info, rows, n, per_vector, aligned), element_size, vec));
+            }
     return most;
 }
-int32_t column_pitch(int32_t n) { return (n + 31) / 32 * 32; }
 
 int32_t check_common(DeviceInfo *info, int32_t rows, int32_t n, int32_t dtype) {
     const int32_t rc = current_device_info(info);
@@ -835,13 +851,6 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
     return CPMK_OK;
 }
 
-// Whether dw and db take a pass of their own.  Beside a row in shared memory (one pass) -> pass of their own, bf16 or fp16: 2048 x 16384
-// 73.7 -> 68.7 us, 2048 x 8200 47.9 -> 46.2, 20 x 16384 24.0 -> 15.9; the rows move half the bytes of their sums there.  fp32 rows and single
-// elements keep to one pass (2048 x 8192 fp32 43.0 against 61, 2048 x 12289 bf16 63.5 against 88).
-template <typename T>
-constexpr bool kSumsBesideVectors = sizeof(T) == 4;
-template <typename T>
-bool strips_for(const Layout &l) { return l.threads == 0 || (l.threads == 1024 && l.vec > 1 && !kSumsBesideVectors<T>); }
 // in shared memory: of a row that 1024 threads take, of eight that a warp takes each
 constexpr int kMostSums = 2 * 16384 * (int)sizeof(float), kMostWarpSums = 8 * 2 * 1024 * (int)sizeof(float);
 
@@ -857,7 +866,7 @@ int32_t backward_rows(const Layout &l, int blocks, int32_t rows, int32_t n, cons
 // (the attribute is the same for every size, so that two threads' calls cannot undo each other's)
 #define CPMK_LN_BACKWARD_LONG(VEC, NV) \
     { \
-        if constexpr (!COLUMNS || VEC == 1 || kSumsBesideVectors<T>) { \
+        if constexpr (!COLUMNS || VEC == 1 || sums_beside_vectors(sizeof(T))) { \
             if (COLUMNS) CPMK_CUDA_TRY(cudaFuncSetAttribute(ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSums)); \
             ln_rows_backward_long_kernel<T, VEC, NV, COLUMNS><<<blocks, 1024, sums, stream>>>(rows, n, inv_n, rd_mean, dy, x, mean, rstd, w, dx, partial, pitch); \
         } \
@@ -894,13 +903,11 @@ int32_t backward(const DeviceInfo &info, int32_t rows, int32_t n, const void *dy
     constexpr int kVec = 16 / (int)sizeof(T);
     const Layout l = backward_layout(info, rows, n, kVec, aligned16(x) && aligned16(dy) && aligned16(w) && aligned16(dx));
     const int blocks = backward_blocks(info, rows, l);
-    const bool sums = dw || db, strips = sums && strips_for<T>(l);
+    const bool sums = dw || db, strips = sums && strips_for(l, sizeof(T));
+    const int vec = n % kVec == 0 && aligned16(x) && aligned16(dy) ? kVec : 1, parts = partial_rows(info, rows, n, l, sizeof(T), vec);
     int32_t rc = CPMK_OK;
-    int parts = blocks;
     if (strips) {
-        const int vec = n % kVec == 0 && aligned16(x) && aligned16(dy) ? kVec : 1;
-        const int64_t across = ceil_div64(n, kStripThreads * vec), down = std::max<int64_t>(1, 8 * info.sm_count / across);
-        parts = (int)std::min<int64_t>(parts, down);
+        const int64_t across = ceil_div64(n, kStripThreads * vec);
         if (vec > 1) ln_rows_strip_kernel<T, kVec><<<dim3((unsigned)across, (unsigned)parts), kStripThreads, 0, stream>>>(rows, n, dy, x, mean, rstd, partial, column_pitch(n));
         else ln_rows_strip_kernel<T, 1><<<dim3((unsigned)across, (unsigned)parts), kStripThreads, 0, stream>>>(rows, n, dy, x, mean, rstd, partial, column_pitch(n));
         CPMK_LAUNCH_CHECK();
@@ -946,7 +953,7 @@ int32_t cpmk_layernorm_rows_backward_scratch(int32_t rows, int32_t n, int64_t *b
     const int32_t rc = check_common(&info, rows, n, CPMK_F16);
     if (rc) return rc;
     CPMK_REQUIRE(bytes, "null pointer");
-    *bytes = most_backward_blocks(info, rows, n) * 2 * column_pitch(n) * (int64_t)sizeof(float);
+    *bytes = most_partial_rows(info, rows, n) * 2 * column_pitch(n) * (int64_t)sizeof(float);
     return CPMK_OK;
 }
 

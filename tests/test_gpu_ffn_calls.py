@@ -3,7 +3,9 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
+import cpm_kernels_b200.kernels as ck
 import cpm_kernels_b200.torch as ct
+from cpm_kernels_b200.library import cpmk
 
 pytestmark = pytest.mark.gpu
 OPERATORS = ["layernorm_rows", "gated_linear", "gated_feed_forward"]
@@ -170,3 +172,33 @@ def test_hidden_activations_have_the_range_of_their_type(tokens):
         assert torch.isinf(ct.gated_linear(x, w, w)).all() == infinite
         y = ct.gated_feed_forward(x, w, w, w_down)
         assert torch.isinf(y).all() if infinite else (y - 260.0 * 260 * 16 / 1024).abs().max() <= 1056 * 2.0 ** -7
+
+
+@pytest.mark.parametrize("rows,n", [(3000, 60000), (600, 20_000_000), (40, 100_000_000)])
+def test_scratch_of_long_rows_stays_small(rows, n):
+    """Partial sums for as many rows as fill the device with strips of columns, one at least: not one per block (24 GB at 600 x 20 million)."""
+    assert ck.layernorm_rows_backward_scratch(rows, n) <= 8 * (n + 64) + 16 * 2 ** 20
+
+
+@pytest.mark.parametrize("t,code", [(torch.float16, cpmk.F16), (torch.float32, cpmk.F32)])
+@pytest.mark.parametrize("rows,n", [(700, 16400), (700, 33000), (300, 66004), (5, 9000), (400, 9000)])
+def test_scratch_suffices_whatever_the_alignment(rows, n, t, code):
+    """Each tensor at an odd address in turn, so that every layout meets the same scratch; nothing behind it is written."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    s, need = torch.cuda.current_stream().cuda_stream, ck.layernorm_rows_backward_scratch(rows, n)
+    make = lambda *shape: torch.randn(*shape, generator=g, device="cuda").to(t)
+    plain = {"dy": make(rows, n), "x": make(rows, n), "w": make(n), "dx": make(rows, n)}
+    moved = {k: torch.empty(v.numel() + 1, device="cuda", dtype=t)[1:].view(v.shape).copy_(v) for k, v in plain.items()}
+    mean, rstd = plain["x"].double().mean(-1), 1 / (plain["x"].double().var(-1, unbiased=False) + 1e-5).sqrt()
+    stats = torch.stack([mean, rstd]).float()
+    want = (plain["dy"].double() * (plain["x"].double() - mean[:, None]) * rstd[:, None]).sum(0)
+    size = (plain["dy"].double() * (plain["x"].double() - mean[:, None]) * rstd[:, None]).abs().sum(0)
+    for odd in ((), ("x",), ("dy",), ("x", "dy"), ("w",), ("dx",), ("x", "dy", "w", "dx")):
+        at = {k: moved[k] if k in odd else plain[k] for k in plain}
+        scratch = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+        dw, db = torch.empty(n, device="cuda", dtype=t), torch.empty(n, device="cuda", dtype=t)
+        ck.layernorm_rows_backward(rows, n, code, at["dy"].data_ptr(), at["x"].data_ptr(), True, at["w"].data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(),
+                                   at["dx"].data_ptr(), dw.data_ptr(), db.data_ptr(), scratch.data_ptr(), s)
+        assert (scratch[need:] == 77).all()
+        # at most rows + 8 roundings of 2^-24 of the sum of magnitudes, the statistics' among them, and that of the output
+        assert ((dw.double() - want).abs() <= (rows + 8) * 2.0 ** -24 * size * 2 + torch.finfo(t).eps / 2 * want.abs() * 1.01 + 2.0 ** -25).all()
