@@ -127,12 +127,13 @@ int32_t launch_simt(const Call &call, SimtParams prm) {
     const int64_t tiles = prm.tiles_c * ceil_div64(prm.R, kSimtTile);
     CPMK_REQUIRE(tiles < (int64_t(1) << 31), "too many output tiles");
     const dim3 grid((unsigned)tiles);
-    const bool silu = EPI != kEpiStore && call.act == CPMK_ACT_SILU;
+    constexpr int kSilu = EPI == kEpiStore ? CPMK_ACT_GELU : CPMK_ACT_SILU;              // a plain product has no activation
+    const bool silu = call.act == kSilu;
     if (call.dtype == CPMK_F16) {
-        if (silu) gated_simt_kernel<__half, EPI, CPMK_ACT_SILU><<<grid, 256, 0, call.stream>>>(prm);
+        if (silu) gated_simt_kernel<__half, EPI, kSilu><<<grid, 256, 0, call.stream>>>(prm);
         else gated_simt_kernel<__half, EPI, CPMK_ACT_GELU><<<grid, 256, 0, call.stream>>>(prm);
     } else {
-        if (silu) gated_simt_kernel<__nv_bfloat16, EPI, CPMK_ACT_SILU><<<grid, 256, 0, call.stream>>>(prm);
+        if (silu) gated_simt_kernel<__nv_bfloat16, EPI, kSilu><<<grid, 256, 0, call.stream>>>(prm);
         else gated_simt_kernel<__nv_bfloat16, EPI, CPMK_ACT_GELU><<<grid, 256, 0, call.stream>>>(prm);
     }
     CPMK_LAUNCH_CHECK();

@@ -298,7 +298,8 @@ int32_t run(const Call &call, int32_t tokens, int32_t rows, int32_t k, const voi
         kernel<<<plan.ctas, kThreads, kSmemBytes, call.stream>>>(maps, prm);
         CPMK_LAUNCH_CHECK();
     }
-    auto join = call.act == CPMK_ACT_SILU && GATED ? few_join_kernel<T, GATED, CPMK_ACT_SILU> : few_join_kernel<T, GATED, CPMK_ACT_GELU>;
+    constexpr int kSilu = GATED ? CPMK_ACT_SILU : CPMK_ACT_GELU;                         // a plain product has no activation
+    auto join = call.act == kSilu ? few_join_kernel<T, GATED, kSilu> : few_join_kernel<T, GATED, CPMK_ACT_GELU>;
     CPMK_CUDA_TRY(launch_after_prior(join, dim3((unsigned)ceil_div64((int64_t)tokens * (rows / 4), 256)), dim3(256), 0, call.stream, tokens, rows, plan.units,
                                      plan.blocks, plan.ctas, static_cast<const float *>(partial), static_cast<T *>(out), static_cast<T *>(g),
                                      static_cast<T *>(u)));

@@ -598,14 +598,13 @@ bool encode_output(CUtensorMap *map, const void *ptr, int64_t R, int64_t C) {
 }
 
 struct Plan {
-    int64_t blocks0, blocks, total, whole, split_tiles, split_pairs, bytes;
+    int64_t blocks0, blocks, whole, split_tiles, split_pairs, bytes;
 };
 // `total` tiles; K1: the second pair's k when its product is added (0: none).
 Plan plan_of(const DeviceInfo &info, int64_t total, int64_t K0, int64_t K1) {
     Plan p;
     p.blocks0 = ceil_div64(K0, kStageK);
     p.blocks = p.blocks0 + ceil_div64(K1, kStageK);
-    p.total = total;
     const int64_t pairs = info.sm_count / 2, left = total % pairs;
     // at least eight k blocks per piece; a k block takes a pair 0.3 us, a piece's sums 1/12 us to write and read back, a join 3 us
     const int64_t most = left * p.blocks / 8, split = most < pairs ? most : pairs;

@@ -821,10 +821,10 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
     const unsigned grid = (unsigned)(want <= most ? want : shift ? most / 8 * 8 : most);         // shifted: one row each, or a multiple of 8 walkers
 #define CPMK_LN_FORWARD(VEC, NV, BLOCK, MOST, SHIFT, THREADS) \
     ln_rows_forward_kernel<T, VEC, NV, BLOCK, MOST, SHIFT><<<grid, THREADS, 0, stream>>>(rows, n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd)
-#define CPMK_LN_FORWARD_BLOCK(VEC, EACH, SHIFT) \
-    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, true, 512, SHIFT, l.threads); \
-    else if (l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, true, 512, SHIFT, l.threads); \
-    else CPMK_LN_FORWARD(VEC, 4 * EACH, true, 512, SHIFT, l.threads)
+#define CPMK_LN_FORWARD_BLOCK(VEC, EACH) \
+    if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, true, 512, false, l.threads); \
+    else if (l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, true, 512, false, l.threads); \
+    else CPMK_LN_FORWARD(VEC, 4 * EACH, true, 512, false, l.threads)
 #define CPMK_LN_FORWARD_WARP(VEC, EACH) \
     if (l.nv == EACH) CPMK_LN_FORWARD(VEC, EACH, false, 128, false, 128); \
     else if (l.nv == 2 * EACH) CPMK_LN_FORWARD(VEC, 2 * EACH, false, 128, false, 128); \
@@ -833,16 +833,19 @@ int32_t forward(const DeviceInfo &info, int32_t rows, int32_t n, const void *xv,
         if (l.vec > 1) ln_rows_forward_wide_kernel<T, kVec><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
         else ln_rows_forward_wide_kernel<T, 1><<<rows, kWideThreads, 0, stream>>>(n, inv_n, eps, rd_mean, x, w, b, y, mean, rstd);
     } else if (shift) {
-        if constexpr (sizeof(T) == 2) { CPMK_LN_FORWARD_BLOCK(kVec, 1, true); }
+        if constexpr (sizeof(T) == 2) {                  // (129 vectors and more: two or four a thread)
+            if (l.nv == 2) CPMK_LN_FORWARD(kVec, 2, true, 512, true, l.threads);
+            else CPMK_LN_FORWARD(kVec, 4, true, 512, true, l.threads);
+        }
     } else if (l.vec == kVec) {
         if (l.threads == 32) { CPMK_LN_FORWARD_WARP(kVec, 1); }
         else if (l.threads == 1024) CPMK_LN_FORWARD(kVec, 4, true, 1024, false, 1024);
         else if (narrow) CPMK_LN_FORWARD(kVec, 4, true, 128, false, l.threads);
-        else { CPMK_LN_FORWARD_BLOCK(kVec, 1, false); }
+        else { CPMK_LN_FORWARD_BLOCK(kVec, 1); }
     } else {
         if (l.threads == 32) { CPMK_LN_FORWARD_WARP(1, 4); }
         else if (l.threads == 1024) CPMK_LN_FORWARD(1, 16, true, 1024, false, 1024);
-        else { CPMK_LN_FORWARD_BLOCK(1, 4, false); }
+        else { CPMK_LN_FORWARD_BLOCK(1, 4); }
     }
 #undef CPMK_LN_FORWARD_BLOCK
 #undef CPMK_LN_FORWARD_WARP
