@@ -335,8 +335,9 @@ int32_t cpmk_layernorm_rows_backward_scratch(int32_t rows, int32_t n, int64_t *b
 /* Gradients of cpmk_layernorm_rows_forward for the output gradient dy (rows, n), from x and the statistics that the forward call
  * wrote: with xh = (x - m) r and g = dy weight,
  *   dx = r (g - mean(g) [only when rd_mean] - xh mean(g xh)),   dweight = sum over rows of dy xh,   dbias = sum over rows of dy.
- * Each of dx, dweight, dbias may be NULL; outputs must not overlap inputs.  Sums in fp32 in an order that depends on the sizes and the device
- * only.  `scratch` (16-byte aligned) is the caller's and not kept; calls that overlap need scratch of their own. */
+ * Each of dx, dweight, dbias may be NULL; outputs must not overlap inputs.  Sums in fp32, in an order that depends on the sizes, the element type,
+ * the device and which of x, dy, weight and dx start on a 16-byte boundary, and on nothing else.  `scratch` (16-byte aligned) is the
+ * caller's and not kept; calls that overlap need scratch of their own. */
 int32_t cpmk_layernorm_rows_backward(int32_t rows, int32_t n, int32_t dtype, const void *dy, const void *x, int32_t rd_mean, const void *weight,
                                      const void *mean, const void *rstd, void *dx, void *dweight, void *dbias, void *scratch, cpmk_stream_t stream);
 

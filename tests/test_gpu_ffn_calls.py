@@ -202,3 +202,18 @@ def test_scratch_suffices_whatever_the_alignment(rows, n, t, code):
         assert (scratch[need:] == 77).all()
         # at most rows + 8 roundings of 2^-24 of the sum of magnitudes, the statistics' among them, and that of the output
         assert ((dw.double() - want).abs() <= (rows + 8) * 2.0 ** -24 * size * 2 + torch.finfo(t).eps / 2 * want.abs() * 1.01 + 2.0 ** -25).all()
+
+
+def test_the_same_bits_at_every_address_of_the_same_alignment():
+    """The order of the sums depends on sizes, type, device and alignment: copies elsewhere, aligned alike, give the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for rows, n in ((700, 1000), (300, 4099), (90, 20000)):
+        x, w, dy = (torch.randn(s, generator=g, device="cuda").half() for s in ((rows, n), (n,), (rows, n)))
+        for odd in (0, 1):
+            results = []
+            for lead in (0, 8, 4096):
+                moved = [torch.empty(t.numel() + lead + odd, device="cuda", dtype=t.dtype)[lead + odd:].view(t.shape).copy_(t) for t in (x, w, dy)]
+                leaves = [t.requires_grad_() for t in moved[:2]]
+                y = ct.layernorm_rows(leaves[0], 1e-5, leaves[1])
+                results.append((y.detach(), *torch.autograd.grad(y, leaves, moved[2])))
+            assert all(torch.equal(p, q) for r in results[1:] for p, q in zip(results[0], r))
