@@ -394,7 +394,7 @@ ln_rows_backward_kernel(int32_t rows, int32_t n, float inv_n, int rd_mean, const
                         const float *__restrict__ mean_in, const float *__restrict__ rstd_in, const T *__restrict__ w, T *__restrict__ dx,
                         float *__restrict__ partial, int32_t pitch) {
     __shared__ float red[2][2][32];
-    extern __shared__ float columns[];                   // warps with rows of their own: their sums, 2 n each
+    extern __shared__ __align__(16) float columns[];     // warps with rows of their own: their sums, 2 n each
     if (COLUMNS) launch_dependents();
     const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, stride = (BLOCK ? blockDim.x : 32) * VEC;
     const int64_t first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(1024, 1) ln_rows_backward_long_kernel(int32_t 
                                                                         const float *__restrict__ rstd_in, const T *__restrict__ w, T *__restrict__ dx,
                                                                         float *__restrict__ partial, int32_t pitch) {
     __shared__ float red[2][2][32];
-    extern __shared__ float columns[];                   // 2 n
+    extern __shared__ __align__(16) float columns[];     // 2 n
     if (COLUMNS) launch_dependents();
     const int t = threadIdx.x, stride = 1024 * VEC, lane = t & 31;
     if (COLUMNS)
