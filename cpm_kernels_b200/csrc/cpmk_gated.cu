@@ -256,7 +256,7 @@ int32_t begin(Call *call, int32_t tokens, int32_t k, int32_t n, int32_t m, int32
     call->dtype = dtype;
     call->act = act;
     call->stream = as_stream(stream);
-    return tokens > 0 ? get_status_word(call->stream, &call->status) : CPMK_OK;
+    return CPMK_OK;
 }
 
 // dx, dWg, dWu from dg, du, and dWd from dy, h

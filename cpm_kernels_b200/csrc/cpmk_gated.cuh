@@ -115,8 +115,13 @@ struct Call {
     // A tile kernel (or its join) of this call is the stream's last: the next starts while it drains, and waits for it.  Block of 1467
     // tokens, 832 / 2136: 35.4 -> 33.8 us, its backward pass 65.9 -> 64.5; 4096 tokens, 4096 / 10240: 1419 -> 1412.
     mutable bool launched = false;
-    uint32_t *status = nullptr;          // the word of the call's stream
+    mutable uint32_t *status = nullptr;  // the word of the call's stream, once a kernel that waits is launched (status_of)
 };
+inline int32_t status_of(const Call &call, uint32_t **word) {
+    const int32_t rc = call.status ? CPMK_OK : get_status_word(call.stream, &call.status);
+    *word = call.status;
+    return rc;
+}
 
 // Tensor-core products on 256 x 256 tiles (cpmk_gated_tc.cu): extents multiples of 8, pointers 16-byte aligned, scratch as many bytes as
 // the _scratch function of the product says.

@@ -284,7 +284,8 @@ int32_t run(const Call &call, int32_t tokens, int32_t rows, int32_t k, const voi
     while (prm.tmem_columns < 2 * prm.padded) prm.tmem_columns *= 2;
     prm.after_prior = after_prior;
     prm.partial = partial;
-    prm.status = call.status;
+    const int32_t rc = status_of(call, &prm.status);
+    if (rc) return rc;
     if (!(encode_rows(&maps.w[0], w0, rows, k, GATED ? 64 : kRows) && (!GATED || encode_rows(&maps.w[1], w1, rows, k, 64)) &&
           encode_rows(&maps.x, x, tokens, k, (uint32_t)prm.padded))) {
         set_error("cuTensorMapEncodeTiled failed");

@@ -637,6 +637,9 @@ int32_t launch(const Call &call, const TcMaps &maps, TcParams prm, const Plan &p
 }
 
 int32_t prepare(const Call &call, TcParams *prm, const Plan &plan, void *scratch) {
+    uint32_t *status;
+    const int32_t rc = status_of(call, &status);
+    if (rc) return rc;
     CPMK_REQUIRE(scratch || !plan.bytes, "scratch is needed");
     memset(prm, 0, sizeof(*prm));
     prm->blocks0 = (int32_t)plan.blocks0;
@@ -645,7 +648,7 @@ int32_t prepare(const Call &call, TcParams *prm, const Plan &plan, void *scratch
     prm->split_tiles = (int32_t)plan.split_tiles;
     prm->split_pairs = (int32_t)plan.split_pairs;
     prm->partial = static_cast<float *>(scratch);
-    prm->status = call.status;
+    prm->status = status;
     return CPMK_OK;
 }
 void add_product(TcParams *prm, int64_t R, int64_t C, int64_t width, bool p_t, bool q_t) {

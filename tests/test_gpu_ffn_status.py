@@ -72,3 +72,24 @@ def test_the_limit_is_checked():
     for limit in (0, 10_000_000):
         with pytest.raises(RuntimeError, match="limit_us"):
             cpmk.call("cpmk_selftest_bounded_wait_gated", limit, None)
+
+
+def test_a_first_call_without_waits_may_be_captured():
+    """Sizes of the generic kernel, and the layer norm: no status words are allocated, so that even a process's first call may be captured."""
+    import os
+    import subprocess
+    import sys
+    script = """
+import torch
+import cpm_kernels_b200.torch as ct
+x, w, n = (torch.ones(s, device="cuda", dtype=torch.half) for s in ((4, 7), (5, 7), (7,)))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    h = ct.gated_linear(ct.layernorm_rows(x, 1e-5, n, rd_mean=False), w, w)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(h, ct.gated_linear(ct.layernorm_rows(x, 1e-5, n, rd_mean=False), w, w)) and h.any()
+"""
+    done = subprocess.run([sys.executable, "-c", script], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
