@@ -20,7 +20,8 @@ namespace {
 //   * the same with single elements (VEC = 1), for rows whose length or address is no multiple of 16 bytes.
 //   * forward, 16-bit rows of 1025 to about 16,000 elements (SHIFT): a row whose length is no multiple of 16 bytes starts anywhere in a
 //     16-byte vector, but rows 8 apart start at the same place of one.  A block takes every 8th (16th, ...) row, so that the shift and the
-//     weights behind a thread's elements stay the same, and reads whole vectors.  Single elements -> shifted vectors: 8192 x 2047
+//     weights behind a thread's elements stay the same, and reads whole vectors.  Single elements -> shifted vectors, both without the
+//     correction of the mean (spread_of; with it 8192 x 2047 takes 28.3 us, 4096 x 4095 24.6, 1027 x 5001 10.8, 2048 x 12289 40.7): 8192 x 2047
 //     34.2 -> 25.8 us, 4096 x 4095 34.1 -> 23.7, 1027 x 5001 12.8 -> 10.2, 2048 x 12289 61.4 -> 39.8, one row of 5001 5.5 -> 3.5;
 //     but 8192 x 511 12.1 -> 13.2 (in a warp, by single elements: 9.0), 2048 x 20001 65 -> 100 (weights gathered per row), fp32
 //     8192 x 1023 18.3 -> 18.1, and the backward pass, which holds two rows, 4096 x 4095 36.6 -> 40.5.
@@ -180,9 +181,9 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float (*red)[32]) {
 // mean(d^2) - off^2 and y = (d - off) r w + b.  Where off comes from:
 //   * 16-bit values that are alike are 12 bits in one unit.  A warp's 1024 of them at most have a sum that is exact, a block's 4096 too, and of
 //     more row_sum_and_rest has what the rounding leaves out: off is what is left of the division, (sum + rest - n mean) / n.
-//     16384 x 4096 bf16 50.0 us with and without it, 30000 x 256 8.6 -> 9.0, 4096 x 8192 28.7 -> 30.4, 4096 x 4095 23.6 -> 24.9.
+//     16384 x 4096 bf16 50.0 us with and without it, 30000 x 256 8.6 -> 9.0, 4096 x 8192 28.7 -> 30.5, 4096 x 4095 23.6 -> 24.6.
 //   * fp32 values, and the longest rows: off is the mean of the deviations, a sum of small numbers beside that of the squares.  8192 x 1024
-//     fp32 13.3 -> 13.5 us, 8192 x 1023 18.5 -> 20.7; as the only way it took 16384 x 4096 bf16 from 50 to 55, and so did a branch for
+//     fp32 13.3 -> 13.4 us, 8192 x 1023 18.5 -> 21.0; as the only way it took 16384 x 4096 bf16 from 50 to 55, and so did a branch for
 //     the rows that need it.
 struct Spread {
     float off, rstd;

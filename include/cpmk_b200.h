@@ -345,7 +345,8 @@ int32_t cpmk_layernorm_rows_backward(int32_t rows, int32_t n, int32_t dtype, con
  * Gated feed-forward block
  * ------------------------------------------------------------------------------------------
  * dtype is CPMK_F16 or CPMK_BF16 for every tensor of a call; products are accumulated in fp32.  Any sizes: extents k, n, m that are
- * multiples of 8 with 16-byte aligned pointers run on the tensor cores, others on a generic kernel.  Outputs must not overlap inputs.
+ * multiples of 8 with 16-byte aligned pointers run on the tensor cores, others on a generic kernel (some 25 times slower at 1000 tokens).
+ * Outputs must not overlap inputs.
  * The first call on a device is made outside a stream capture (it allocates the status words that cpmk_read_status and
  * cpmk_check_stream report); after that calls may be captured on any stream. */
 
