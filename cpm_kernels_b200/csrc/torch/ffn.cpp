@@ -52,9 +52,12 @@ struct Refused : std::runtime_error {
 void want(bool ok, const char *what) {
     if (!ok) throw Refused(what);
 }
-// of the type and on the device of x, contiguous, with these extents
+// contiguous, and what its memory holds (a view such as z.conj().imag is to be read negated)
+bool as_it_lies(const Tensor &t) { return t.is_contiguous() && !t.is_neg(); }
+Tensor laid_out(const Tensor &t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+// of the type and on the device of x, as it lies, with these extents
 bool goes_with(const Tensor &t, const Tensor &x, at::IntArrayRef sizes) {
-    return t.defined() && t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == sizes && t.is_contiguous();
+    return t.defined() && t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == sizes && as_it_lies(t);
 }
 constexpr int64_t kMost = int64_t{1} << 30;
 
@@ -133,7 +136,7 @@ struct LayerNormRows : torch::autograd::Function<LayerNormRows> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
         const int64_t n = weight.numel(), rows = x.numel() / n;
-        const Tensor dy = grads[0].contiguous();
+        const Tensor dy = laid_out(grads[0]);
         const Place place(x);
         Tensor dx, dweight, dbias, scratch;
         if (ctx->needs_input_grad(0)) dx = fresh(x.sizes(), x);
@@ -153,7 +156,7 @@ struct LayerNormRows : torch::autograd::Function<LayerNormRows> {
 };
 
 Tensor layernorm_rows(const Tensor &x, double eps, const Tensor &weight, const std::optional<Tensor> &bias, bool rd_mean) {
-    want(x.is_cuda() && x.dim() >= 1 && x.is_contiguous(), "layernorm_rows: x must be a contiguous CUDA tensor of one axis or more");
+    want(x.is_cuda() && x.dim() >= 1 && as_it_lies(x), "layernorm_rows: x must be a contiguous CUDA tensor of one axis or more");
     const at::ScalarType type = x.scalar_type();
     want(type == at::kHalf || type == at::kBFloat16 || type == at::kFloat, "layernorm_rows: x must be fp16, bf16 or fp32");
     const int64_t n = x.size(-1);
@@ -171,7 +174,7 @@ Tensor layernorm_rows(const Tensor &x, double eps, const Tensor &weight, const s
 // gated feed-forward block
 // ------------------------------------------------------------------------------------------------
 void check_gated(const Tensor &x, const Tensor &w_gate, const Tensor &w_up) {
-    want(x.is_cuda() && x.dim() >= 1 && x.is_contiguous(), "gated block: x must be a contiguous CUDA tensor of one axis or more");
+    want(x.is_cuda() && x.dim() >= 1 && as_it_lies(x), "gated block: x must be a contiguous CUDA tensor of one axis or more");
     want(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "gated block: x must be fp16 or bf16");
     want(w_gate.dim() == 2, "gated block: w_gate must be a matrix");
     const int64_t n = w_gate.size(0), k = w_gate.size(1);
@@ -215,7 +218,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w_gate = saved[1], &w_up = saved[2], &gu = saved[3];
         const int64_t n = w_gate.size(0), k = w_gate.size(1), tokens = x.numel() / k;
-        const Tensor dh = grads[0].contiguous();
+        const Tensor dh = laid_out(grads[0]);
         const Place place(x);
         const Tensor dgu = fresh(gu.sizes(), gu);
         Tensor dx, dw_gate, dw_up;
@@ -269,7 +272,7 @@ struct GatedFeedForward : torch::autograd::Function<GatedFeedForward> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w_gate = saved[1], &w_up = saved[2], &w_down = saved[3], &hgu = saved[4];
         const int64_t n = w_gate.size(0), k = w_gate.size(1), m = w_down.size(0), tokens = x.numel() / k;
-        const Tensor dy = grads[0].contiguous();
+        const Tensor dy = laid_out(grads[0]);
         const Place place(x);
         const Tensor dgu = fresh({2, tokens, n}, x);
         Tensor dx, dw_gate, dw_up, dw_down;

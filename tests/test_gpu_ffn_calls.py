@@ -217,3 +217,19 @@ def test_the_same_bits_at_every_address_of_the_same_alignment():
                 y = ct.layernorm_rows(leaves[0], 1e-5, leaves[1])
                 results.append((y.detach(), *torch.autograd.grad(y, leaves, moved[2])))
             assert all(torch.equal(p, q) for r in results[1:] for p, q in zip(results[0], r))
+
+
+def test_negated_views():
+    """The imaginary part of a conjugate is read negated; where it counts as contiguous, operands are refused and an output gradient is
+    taken as what it stands for."""
+    lazy = torch.tensor([[1 + 2j]], device="cuda").conj().imag
+    assert lazy.is_neg() and lazy.is_contiguous() and lazy.item() == -2
+    w = torch.ones(1, device="cuda", requires_grad=True)
+    x = torch.full((1, 1), 3.0, device="cuda", requires_grad=True)
+    with pytest.raises(AssertionError):
+        ct.layernorm_rows(lazy, 1e-5, w)
+    with pytest.raises(AssertionError):
+        ct.layernorm_rows(x, 1e-5, lazy[0])
+    step = lambda dy: torch.autograd.grad(ct.layernorm_rows(x, 1e-5, w, w, rd_mean=False), (x, w), dy)
+    for got, want in zip(step(lazy), step(torch.full((1, 1), -2.0, device="cuda"))):
+        assert torch.equal(got, want)
